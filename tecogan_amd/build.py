@@ -7,7 +7,10 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libtecogan_hip.so")
 SOURCES = ["conv_igemm.hip", "conv3x3.hip", "conv3x3_ws.hip", "conv3x3_dma.hip", "conv3x3_wr.hip", "conv4x4s2.hip", "resblock_lat.hip", "resblock_chain.hip", "resblock_plane.hip", "resblock_thr.hip", "hr_bwd_lat.hip", "hr_fwd_lat.hip", "conv_wgrad.hip", "conv_wgrad_tr.hip", "warp.hip", "pointwise.hip", "schedule.hip", "losses.hip", "runtime.hip"]
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics", "-Wno-unused-result"]
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32.  The compiler forms them from ordinary float code at -O3, and some of their operand
+# forms have given wrong results on MI355X now and then; the host pass does not know the feature and says so (harmless)
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics", "-Wno-unused-result",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _newer(a, b):
