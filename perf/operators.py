@@ -464,7 +464,7 @@ def _own_scan(K, s, c, kept):
                 kept["d_h0"] = torch.empty(B, D, device=DEV, dtype=F32)
             s["ws"] = torch.empty(K.gated_scan_ws(B, T, D), device=DEV, dtype=F32)
     how = dict(h0=s["h0"], floor=s["floor"], lengths=s["lengths"], reset=s["reset"])
-    K.gated_scan_forward(s["x"], s["g"], kept["y"], kept["hT"], s["carry"], **how)
+    K.gated_scan_forward(s["x"], s["g"], kept["y"], kept["hT"], s["carry"], keep=train, **how)
     if train:
         K.gated_scan_backward(s["x"], s["g"], s["d_y"], s["d_hT"], s["carry"], kept["d_x"], kept["d_g"], s["ws"],
                               d_h0=kept.get("d_h0"), d_floor=kept.get("d_floor"), **how)
