@@ -31,6 +31,9 @@ extern "C" {
 
 #define TG_F32   0
 #define TG_BF16  1
+/* 8-bit floating point (OCP), operands of tg_fp8_* only */
+#define TG_FP8_E4M3 2   /* largest value 448, no infinity */
+#define TG_FP8_E5M2 3   /* largest value 57344             */
 
 /* activation codes for conv epilogues / pointwise */
 #define TG_ACT_NONE    0
@@ -38,6 +41,7 @@ extern "C" {
 #define TG_ACT_LRELU   2   /* lrelu(x, alpha)                 lib/ops.py:84-85        */
 #define TG_ACT_TANH    3   /* tanh(x) * alpha                 lib/frvsr.py:39         */
 #define TG_ACT_SIGMOID 4   /* tf.nn.sigmoid                   lib/Teco.py:72          */
+#define TG_ACT_SILU    5   /* v * sigmoid(v): gates of tg_gated_norm_* only            */
 
 int         tg_version(void);
 const char* tg_last_error_string(void);
@@ -473,6 +477,93 @@ int tg_gauss_down4_preprocess(const float* hr, float* lr, float* target /*nullab
 /* save_img (lib/ops.py:521-523): out = uint8(clip(frame * 255, 0, 255)) (truncation), RGB or BGR byte order. */
 int tg_frame_to_u8(const float* frame /*[npix][3] in [0,1]*/, unsigned char* out /*[npix][3]*/, int64_t npix, int bgr,
                    void* stream);
+
+/* ------------------------------------------------------------------------ *
+ * Sequence-block operators: what a block over rows of features (a frame's pixels, a sequence's steps) is made of -- the boundary
+ * between two blocks, its projections in 8-bit floating point, a gated linear recurrence along the sequence.  No counterpart in the
+ * reference, whose blocks are conv - ReLU - conv + skip (lib/frvsr.py:50-57) and whose recurrence is unrolled (lib/Teco.py:130-160).
+ * Beside the header's conventions: rows may have a stride (in elements), sizes are free, a workspace belongs to the calls of one
+ * stream at a time (two graphs that may run at once need one each), and results are the same bits for the same inputs (no atomics).
+ * ------------------------------------------------------------------------ */
+#define TG_NORM_NONE  0
+#define TG_NORM_RMS   1   /* z / sqrt(mean(z^2) + eps) * w + b            */
+#define TG_NORM_LAYER 2   /* (z - mean) / sqrt(var + eps) * w + b         */
+#define TG_GATED_NORM_MAX_C 16384
+
+typedef struct tg_gated_norm_desc {
+  int64_t rows;            /* >= 0, < 2^31                                                                       */
+  int64_t rows_per_gate;   /* row r uses gate row r / rows_per_gate: 1 = a gate per row, rows = one for all      */
+  int64_t ldx, ldo, ldg, ldy, ldh;       /* row strides of x (backward: d_x), o, gate, y, h (backward: d_h)      */
+  int64_t ld_dy, ld_do, ld_dg;           /* backward: row strides of d_y, d_o, d_gate                            */
+  int32_t C;               /* 1 .. TG_GATED_NORM_MAX_C                                                           */
+  int32_t dtype;           /* o, gate, h, d_h, d_o, d_gate                                                       */
+  int32_t res_dtype;       /* x, y, d_y, d_x: dtype, or f32 beside bf16                                          */
+  int32_t post, pre;       /* TG_NORM_*                                                                          */
+  int32_t gate_act;        /* TG_ACT_NONE, SIGMOID, TANH, SILU                                                   */
+  float   alpha;           /* residual scale                                                                     */
+  float   eps;             /* in [1e-30, 1e30]                                                                   */
+} tg_gated_norm_desc;
+/* y = x + alpha * scale[c] * act(gate) * post(o);  h = pre(y).  Nullable: o (then also gate and y: h = pre(x) alone), gate, h (iff
+ * pre is NONE), every fp32 [C] parameter (1 for weights and scale, 0 for biases).  y may be x itself. */
+int tg_gated_norm_forward(const tg_gated_norm_desc* d, const void* x, const void* o /*nullable*/, const void* gate /*nullable*/,
+                          const float* w_post, const float* b_post, const float* scale, const float* w_pre, const float* b_pre,
+                          void* y, void* h, void* stream);
+/* fp32 values of the backward pass's workspace */
+int tg_gated_norm_ws(int64_t rows, int C, int64_t rows_per_gate, int64_t* floats);
+/* The gradients, from y (x where there is no o), o and gate as the forward pass had them; the statistics are taken again.  d_y, d_h
+ * nullable (zero); every output nullable (not wanted).  d_x may be d_y itself.  Parameter gradients are overwritten, not added to;
+ * d_gate of a shared gate row is the sum over its rows, rounded once. */
+int tg_gated_norm_backward(const tg_gated_norm_desc* d, const void* d_y, const void* d_h, const void* y, const void* o, const void* gate,
+                           const float* w_post, const float* b_post, const float* scale, const float* w_pre, const float* b_pre,
+                           void* d_x, void* d_o, void* d_gate, float* d_w_post, float* d_b_post, float* d_scale, float* d_w_pre,
+                           float* d_b_pre, float* ws, int64_t ws_floats, void* stream);
+
+/* 8-bit operands with a power-of-two scale for each block of 128 along the reduction.
+ * x [rows][cols] (f32 / bf16, row stride ldx) ->
+ *   q  [rows][pad128(cols)], scale  [rows][pad4(cols / 128)]: blocks along the columns (tile != 0: a scale per 128 x 128 tile,
+ *      scale [rows / 128][pad4(cols / 128)]);
+ *   qt [cols][pad128(rows)], scale_t [cols][pad4(rows / 128)]: the transposed copy, blocks along the rows (tile: the same scales).
+ * Divisions round up; padding is zeros; a scale is the byte e + 127 of 2^e.  Either copy may be NULL with its scales. */
+int tg_fp8_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int fmt, int tile, void* q /*nullable*/,
+                    void* scale, void* qt /*nullable*/, void* scale_t, void* stream);
+typedef struct tg_fp8_matmul_desc {
+  int64_t M, N, K;         /* K: a multiple of 128, the padded row of both operands */
+  int64_t ldo;             /* row stride of out */
+  int32_t a_fmt, b_fmt;    /* TG_FP8_* */
+  int32_t a_tile, b_tile;  /* scales per 128 x 128 tile instead of per row */
+  int32_t out_dtype;       /* TG_F32, TG_BF16 */
+  int32_t accumulate;      /* out += (f32 only) */
+} tg_fp8_matmul_desc;
+/* out[M][N] = a[M][K] b[N][K]^T (+ bias[N]) (+ out) */
+int tg_fp8_matmul(const tg_fp8_matmul_desc* d, const void* a, const void* scale_a, const void* b, const void* scale_b,
+                  const float* bias /*nullable*/, void* out, void* stream);
+/* out = q(x) w^T + bias: tg_fp8_quantize (e4m3, a scale per row and block) and tg_fp8_matmul with a weight of tile scales. */
+int tg_fp8_linear_ws(int64_t M, int64_t N, int64_t K, int64_t* bytes);
+int tg_fp8_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* w /*[N][pad128(K)]*/, const void* scale_w,
+                  int64_t N, int w_fmt, const float* bias /*nullable*/, void* out, int out_dtype, int64_t ldo, void* ws,
+                  int64_t ws_bytes, void* stream);
+
+typedef struct tg_gated_scan_desc {
+  int64_t x_t, x_b, g_t, g_b, y_t, y_b;              /* strides of a step and of a batch row, in elements; channels contiguous */
+  int64_t dy_t, dy_b, dx_t, dx_b, dg_t, dg_b;        /* backward */
+  int32_t B, T, D;
+  int32_t dtype;                                     /* x, g, y and their gradients */
+} tg_gated_scan_desc;
+/* fp32 values of `carry` (written by the forward pass, read by the backward pass) and of the backward pass's workspace */
+int tg_gated_scan_sizes(int B, int T, int D, int64_t* carry_floats, int64_t* ws_floats);
+/* h[t] = f[t] h[t-1] + (1 - f[t]) x[t], f = floor + (1 - floor) sigmoid(g); y = h, hT = the last state (fp32 [B][D]).
+ * Nullable: h0 (fp32 [B][D], zero), floor (fp32 [D] in [0, 1), zero), lengths (int32 [B]: steps at and behind a row's length keep the
+ * state, y = 0 there, their x and g are not looked at), reset (bytes [B][T]: not 0 = a new sequence begins at this step, the state
+ * before it is dropped), hT, carry (only where keep == 0 and tg_gated_scan_sizes' carry serves no chunks, i.e. short sequences over
+ * many channels).  hT may be h0 itself where no backward pass follows; y may be x or g itself. */
+int tg_gated_scan_forward(const tg_gated_scan_desc* d, const void* x, const void* g, const float* h0, const float* floor,
+                          const int32_t* lengths, const unsigned char* reset, void* y, float* hT, float* carry, int64_t carry_floats,
+                          int keep /*the states that a backward pass needs*/, void* stream);
+/* Gradients of x, g, h0 and floor from d_y (nullable) and d_hT (nullable) and the carry that the forward pass kept for the same
+ * inputs; d_h0, d_floor nullable (not wanted). */
+int tg_gated_scan_backward(const tg_gated_scan_desc* d, const void* x, const void* g, const float* floor, const int32_t* lengths,
+                           const unsigned char* reset, const void* d_y, const float* d_hT, const float* carry, int64_t carry_floats,
+                           void* d_x, void* d_g, float* d_h0, float* d_floor, float* ws, int64_t ws_floats, void* stream);
 
 #ifdef __cplusplus
 }

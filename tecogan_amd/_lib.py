@@ -10,8 +10,9 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # TECOGAN_HIP_LIB: another build of the same library (A/B of compile-time layout constants, tools/build_variant.py)
 LIB_PATH = os.environ.get("TECOGAN_HIP_LIB") or os.path.join(_HERE, "libtecogan_hip.so")
 
-TG_F32, TG_BF16 = 0, 1
-ACT_NONE, ACT_RELU, ACT_LRELU, ACT_TANH, ACT_SIGMOID = 0, 1, 2, 3, 4
+TG_F32, TG_BF16, TG_FP8_E4M3, TG_FP8_E5M2 = 0, 1, 2, 3
+ACT_NONE, ACT_RELU, ACT_LRELU, ACT_TANH, ACT_SIGMOID, ACT_SILU = 0, 1, 2, 3, 4, 5
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
 CONV_COEXIST = 1
 
 
@@ -23,6 +24,21 @@ class ConvDesc(C.Structure):
                 ("in_dtype", C.c_int32), ("out_dtype", C.c_int32),
                 ("act", C.c_int32), ("act_alpha", C.c_float),
                 ("mask_act", C.c_int32), ("mask_alpha", C.c_float), ("flags", C.c_int32)]
+
+
+class GatedNormDesc(C.Structure):
+    _fields_ = [(n, C.c_int64) for n in ("rows", "rows_per_gate", "ldx", "ldo", "ldg", "ldy", "ldh", "ld_dy", "ld_do", "ld_dg")] + \
+               [(n, C.c_int32) for n in ("C", "dtype", "res_dtype", "post", "pre", "gate_act")] + [("alpha", C.c_float), ("eps", C.c_float)]
+
+
+class Fp8MatmulDesc(C.Structure):
+    _fields_ = [(n, C.c_int64) for n in ("M", "N", "K", "ldo")] + \
+               [(n, C.c_int32) for n in ("a_fmt", "b_fmt", "a_tile", "b_tile", "out_dtype", "accumulate")]
+
+
+class GatedScanDesc(C.Structure):
+    _fields_ = [(n, C.c_int64) for n in ("x_t", "x_b", "g_t", "g_b", "y_t", "y_b", "dy_t", "dy_b", "dx_t", "dx_b", "dg_t", "dg_b")] + \
+               [(n, C.c_int32) for n in ("B", "T", "D", "dtype")]
 
 
 _P, _I, _L, _F = C.c_void_p, C.c_int, C.c_int64, C.c_float
@@ -101,6 +117,18 @@ SIGNATURES["tg_prof_enable"] = [_I]
 SIGNATURES["tg_prof_collect"] = [C.POINTER(ProfEntry), _I, C.POINTER(C.c_int)]
 SIGNATURES["tg_prof_stamp"] = [_P, _P]
 SIGNATURES["tg_graph_node_count"] = [_P, C.POINTER(C.c_int), C.POINTER(C.c_int)]
+
+_GN, _MM, _GS, _LP = C.POINTER(GatedNormDesc), C.POINTER(Fp8MatmulDesc), C.POINTER(GatedScanDesc), C.POINTER(C.c_int64)
+SIGNATURES["tg_gated_norm_forward"] = [_GN] + [_P] * 11
+SIGNATURES["tg_gated_norm_ws"] = [_L, _I, _L, _LP]
+SIGNATURES["tg_gated_norm_backward"] = [_GN] + [_P] * 19 + [_L, _P]
+SIGNATURES["tg_fp8_quantize"] = [_P, _I, _L, _L, _L, _I, _I, _P, _P, _P, _P, _P]
+SIGNATURES["tg_fp8_matmul"] = [_MM] + [_P] * 7
+SIGNATURES["tg_fp8_linear_ws"] = [_L, _L, _L, _LP]
+SIGNATURES["tg_fp8_linear"] = [_P, _I, _L, _L, _L, _P, _P, _L, _I, _P, _P, _I, _L, _P, _L, _P]
+SIGNATURES["tg_gated_scan_sizes"] = [_I, _I, _I, _LP, _LP]
+SIGNATURES["tg_gated_scan_forward"] = [_GS] + [_P] * 9 + [_L, _I, _P]
+SIGNATURES["tg_gated_scan_backward"] = [_GS] + [_P] * 8 + [_L] + [_P] * 5 + [_L, _P]
 
 _lib = None
 

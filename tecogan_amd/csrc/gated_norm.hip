@@ -1,0 +1,642 @@
+// The boundary between two blocks of a network over rows of features, as one launch per direction:
+//
+//   u = post(o)                      norm after the block that ends        (none / RMS / layer)
+//   v = alpha scale[c] act(gate) u   its gate and its residual scale
+//   y = x + v                        the residual stream
+//   h = pre(y)                       norm before the block that begins     (none / RMS / layer)
+//
+// with post, pre: z^ w + b, z^ = z / sqrt(mean(z^2) + eps) (RMS) or (z - mean) / sqrt(var + eps) (layer).
+//
+// About 14 (forward) / 40 (backward) operations a value against 10 - 32 bytes: bound by HBM.  Every tensor is read once and written
+// once; a row stays in registers between its reductions.  A row belongs to LPR lanes (a power of two, 1 - 512) with 8 NV values
+// each: 16-byte loads, reductions by lane exchange inside a wave and through LDS between the waves of a row.  All sums, statistics
+// and gradients are fp32; h is taken from the fp32 y before y is rounded to its type (one rounding per output).  The backward pass
+// takes the statistics again from y and o, which it has to read anyway: nothing is kept between the passes but the tensors.
+// Parameter gradients: per-lane sums over the rows of a workgroup, one partial row per workgroup, then a second launch adds the
+// partials in a fixed order (no atomics: the same inputs give the same bits).
+#include "common.h"
+
+namespace {
+
+typedef float f4v __attribute__((ext_vector_type(4)));
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T* __restrict__ row, int c, int C, float (&f)[8]) {
+  if constexpr (VEC) {
+    if (c < C) {
+      if constexpr (sizeof(T) == 2) {
+        bf8_unpack(*reinterpret_cast<const uint4*>(row + c), f);
+      } else {
+        const f4v a = *reinterpret_cast<const f4v*>(row + c), b = *reinterpret_cast<const f4v*>(row + c + 4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { f[k] = a[k]; f[4 + k] = b[k]; }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] = 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = c + k < C ? Elem<T>::ld(row + c + k) : 0.f;
+  }
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void store8(T* __restrict__ row, int c, int C, const float (&f)[8]) {
+  if constexpr (VEC) {
+    if (c >= C) return;
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<uint4*>(row + c) = bf8_pack(f);
+    } else {
+      *reinterpret_cast<f4v*>(row + c) = f4v{f[0], f[1], f[2], f[3]};
+      *reinterpret_cast<f4v*>(row + c + 4) = f4v{f[4], f[5], f[6], f[7]};
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (c + k < C) Elem<T>::st(row + c + k, f[k]);
+  }
+}
+
+// fp32 parameter vector (nullable): its 8 values, or `other`
+template <bool VEC>
+__device__ __forceinline__ void param8(const float* __restrict__ p, int c, int C, float other, float (&f)[8]) {
+  if (p) {
+    load8<float, VEC>(p, c, C, f);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = other;
+  }
+}
+
+__device__ __forceinline__ float gate_value(float g, int act) {
+  switch (act) {
+    case TG_ACT_SIGMOID: return 1.f / (1.f + __expf(-g));
+    case TG_ACT_TANH: return tanhf(g);
+    case TG_ACT_SILU: return g / (1.f + __expf(-g));
+    default: return g;
+  }
+}
+// value and derivative
+__device__ __forceinline__ float gate_slope(float g, int act, float* value) {
+  switch (act) {
+    case TG_ACT_SIGMOID: {
+      const float p = 1.f / (1.f + __expf(-g));
+      *value = p;
+      return p * (1.f - p);
+    }
+    case TG_ACT_TANH: {
+      const float t = tanhf(g);
+      *value = t;
+      return 1.f - t * t;
+    }
+    case TG_ACT_SILU: {
+      const float p = 1.f / (1.f + __expf(-g));
+      *value = g * p;
+      return p * (1.f + g * (1.f - p));
+    }
+    default: *value = g; return 1.f;
+  }
+}
+
+constexpr int GN_MAX_LPR = 512;
+
+// Sums v[0..N) over the lanes of this lane's row.  Rows wider than a wave meet in `red` (two buffers used in turn: a buffer is
+// written again two calls later, behind the other buffer's barrier).
+template <int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], int lpr, float* red, int& turn) {
+  const int w = lpr < 64 ? lpr : 64;
+  for (int o = w >> 1; o > 0; o >>= 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o, 64);
+  }
+  if (lpr > 64) {
+    const int wave = threadIdx.x >> 6, wpr = lpr >> 6, w0 = wave & ~(wpr - 1);
+    float* buf = red + turn * (8 * 4);
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) buf[wave * 4 + i] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float s = 0.f;
+      for (int k = 0; k < wpr; ++k) s += buf[(w0 + k) * 4 + i];
+      v[i] = s;
+    }
+    turn ^= 1;
+  }
+}
+
+struct GnP {
+  tg_gated_norm_desc d;
+  const void *x, *o, *gate, *y, *d_y, *d_h;
+  const float *w_post, *b_post, *scale, *w_pre, *b_pre;
+  void *out_y, *out_h, *d_x, *d_o, *d_gate;
+  float *part, *gate_part;                   // [blocks][5][C], [items][C]
+  int lpr_log2;
+  int item_rows, pieces;                     // rows of an item; > 0: pieces of a gate row's rows (an item is one piece)
+  int64_t items;
+  int want;                                  // bit p: parameter p's gradient is asked for
+  float inv_c;
+};
+
+template <typename TO, typename TX, int NV, bool VEC>
+__global__ __launch_bounds__(512) void gated_norm_fwd_kernel(GnP p) {
+  __shared__ float red[2 * 8 * 4];
+  const tg_gated_norm_desc& d = p.d;
+  const int lpr = 1 << p.lpr_log2, lane = threadIdx.x & (lpr - 1), sub = threadIdx.x >> p.lpr_log2, rpb = blockDim.x >> p.lpr_log2;
+  const int C = d.C;
+  int turn = 0;
+  for (int64_t base = (int64_t)blockIdx.x * rpb; base < d.rows; base += (int64_t)gridDim.x * rpb) {
+    const bool on = base + sub < d.rows;
+    const int64_t row = on ? base + sub : d.rows - 1;
+    const int Cr = on ? C : 0;                                   // a row past the end reads and writes nothing
+    float x[NV][8], u[NV][8], g[NV][8];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * lpr + lane) * 8;
+      load8<TX, VEC>(static_cast<const TX*>(p.x) + row * d.ldx, c, Cr, x[v]);
+      if (p.o) load8<TO, VEC>(static_cast<const TO*>(p.o) + row * d.ldo, c, Cr, u[v]);
+      if (p.gate) load8<TO, VEC>(static_cast<const TO*>(p.gate) + (d.rows_per_gate == 1 ? row : row / d.rows_per_gate) * d.ldg, c, Cr, g[v]);
+    }
+    if (p.o) {
+      if (d.post != TG_NORM_NONE) {
+        float mu = 0.f;
+        if (d.post == TG_NORM_LAYER) {
+          float s[1] = {0.f};
+#pragma unroll
+          for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s[0] += u[v][k];
+          row_sums(s, lpr, red, turn);
+          mu = s[0] * p.inv_c;
+        }
+        float s[1] = {0.f};
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          const int c = (v * lpr + lane) * 8;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            u[v][k] = c + k < Cr ? u[v][k] - mu : 0.f;
+            s[0] += u[v][k] * u[v][k];
+          }
+        }
+        row_sums(s, lpr, red, turn);
+        const float r = rsqrtf(s[0] * p.inv_c + d.eps);
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          const int c = (v * lpr + lane) * 8;
+          float w[8], b[8];
+          param8<VEC>(p.w_post, c, C, 1.f, w);
+          param8<VEC>(p.b_post, c, C, 0.f, b);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) u[v][k] = u[v][k] * r * w[k] + b[k];
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const int c = (v * lpr + lane) * 8;
+        float sc[8];
+        param8<VEC>(p.scale, c, C, 1.f, sc);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float a = p.gate ? gate_value(g[v][k], d.gate_act) : 1.f;
+          x[v][k] += d.alpha * sc[k] * a * u[v][k];
+        }
+        store8<TX, VEC>(static_cast<TX*>(p.out_y) + row * d.ldy, c, Cr, x[v]);
+      }
+    }
+    if (d.pre != TG_NORM_NONE) {
+      float mu = 0.f;
+      if (d.pre == TG_NORM_LAYER) {
+        float s[1] = {0.f};
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          const int c = (v * lpr + lane) * 8;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) s[0] += c + k < Cr ? x[v][k] : 0.f;
+        }
+        row_sums(s, lpr, red, turn);
+        mu = s[0] * p.inv_c;
+      }
+      float s[1] = {0.f};
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const int c = (v * lpr + lane) * 8;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          x[v][k] = c + k < Cr ? x[v][k] - mu : 0.f;
+          s[0] += x[v][k] * x[v][k];
+        }
+      }
+      row_sums(s, lpr, red, turn);
+      const float r = rsqrtf(s[0] * p.inv_c + d.eps);
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const int c = (v * lpr + lane) * 8;
+        float w[8], b[8];
+        param8<VEC>(p.w_pre, c, C, 1.f, w);
+        param8<VEC>(p.b_pre, c, C, 0.f, b);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[v][k] = x[v][k] * r * w[k] + b[k];
+        store8<TO, VEC>(static_cast<TO*>(p.out_h) + row * d.ldh, c, Cr, x[v]);
+      }
+    }
+  }
+}
+
+// One item = item_rows consecutive rows of one sub-row of lanes: whole gate rows, or a piece of one (pieces > 0).
+template <typename TO, typename TX, int NV, bool VEC>
+__global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
+  __shared__ float red[2 * 8 * 4];
+  extern __shared__ float join[];                                   // [rows of the workgroup][8 lpr]: only where it has several
+  const tg_gated_norm_desc& d = p.d;
+  const int lpr = 1 << p.lpr_log2, lane = threadIdx.x & (lpr - 1), sub = threadIdx.x >> p.lpr_log2, rpb = blockDim.x >> p.lpr_log2;
+  const int C = d.C;
+  const int64_t item = (int64_t)blockIdx.x * rpb + sub;
+  int64_t start, end;
+  if (p.pieces > 0) {
+    const int64_t group = item / p.pieces, piece = item - group * p.pieces;
+    const int64_t last = (group + 1) * d.rows_per_gate;
+    start = group * d.rows_per_gate + piece * p.item_rows;
+    end = start + p.item_rows < last ? start + p.item_rows : last;
+  } else {
+    start = item * p.item_rows;
+    end = start + p.item_rows;
+  }
+  end = item < p.items ? (end < d.rows ? end : d.rows) : start;
+  const bool layer = d.pre == TG_NORM_LAYER || d.post == TG_NORM_LAYER;
+  float acc[5][NV][8] = {}, dga[NV][8] = {};                        // w_post, b_post, scale, w_pre, b_pre; the gate row
+  int turn = 0;
+  for (int j = 0; j < p.item_rows; ++j) {
+    const bool on = start + j < end;
+    const int64_t row = on ? start + j : 0;
+    const int Cr = on ? C : 0;
+    const int64_t grow = d.rows_per_gate == 1 ? row : row / d.rows_per_gate;
+    float y[NV][8], o[NV][8], g[NV][8], dh[NV][8], G[NV][8];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * lpr + lane) * 8;
+      load8<TX, VEC>(static_cast<const TX*>(p.y) + row * d.ldy, c, Cr, y[v]);
+      if (p.d_h) load8<TO, VEC>(static_cast<const TO*>(p.d_h) + row * d.ldh, c, Cr, dh[v]);
+      if (p.d_y) load8<TX, VEC>(static_cast<const TX*>(p.d_y) + row * d.ld_dy, c, Cr, G[v]);
+      if (p.o) load8<TO, VEC>(static_cast<const TO*>(p.o) + row * d.ldo, c, Cr, o[v]);
+      if (p.gate) load8<TO, VEC>(static_cast<const TO*>(p.gate) + grow * d.ldg, c, Cr, g[v]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (!p.d_h) dh[v][k] = 0.f;
+        if (!p.d_y) G[v][k] = 0.f;
+        if (!p.o) o[v][k] = 0.f;
+      }
+    }
+    float mu_y = 0.f, mu_o = 0.f;
+    if (layer) {
+      float s[2] = {0.f, 0.f};
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { s[0] += y[v][k]; s[1] += o[v][k]; }
+      row_sums(s, lpr, red, turn);
+      mu_y = d.pre == TG_NORM_LAYER ? s[0] * p.inv_c : 0.f;
+      mu_o = d.post == TG_NORM_LAYER ? s[1] * p.inv_c : 0.f;
+    }
+    float s[4] = {0.f, 0.f, 0.f, 0.f};                              // |y - mu|^2, t (y - mu), t, |o - mu|^2 with t = dh w_pre
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * lpr + lane) * 8;
+      float w[8];
+      param8<VEC>(p.w_pre, c, C, 1.f, w);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const bool in = c + k < Cr;
+        y[v][k] = in ? y[v][k] - mu_y : 0.f;
+        if (d.post != TG_NORM_NONE) o[v][k] = in ? o[v][k] - mu_o : 0.f;
+        const float t = dh[v][k] * w[k];
+        s[0] += y[v][k] * y[v][k];
+        s[1] += t * y[v][k];
+        s[2] += t;
+        s[3] += o[v][k] * o[v][k];
+      }
+    }
+    row_sums(s, lpr, red, turn);
+    const float r_y = rsqrtf(s[0] * p.inv_c + d.eps), r_o = d.post != TG_NORM_NONE ? rsqrtf(s[3] * p.inv_c + d.eps) : 1.f;
+    const float m1 = s[1] * r_y * p.inv_c, m2 = d.pre == TG_NORM_LAYER ? s[2] * p.inv_c : 0.f;
+    float q[2] = {0.f, 0.f};                                        // t o^, t with t = du w_post
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * lpr + lane) * 8;
+      float wpre[8], wpost[8], bpost[8], sc[8];
+      param8<VEC>(p.w_pre, c, C, 1.f, wpre);
+      param8<VEC>(p.w_post, c, C, 1.f, wpost);
+      param8<VEC>(p.b_post, c, C, 0.f, bpost);
+      param8<VEC>(p.scale, c, C, 1.f, sc);
+      float dg[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (d.pre != TG_NORM_NONE) {
+          const float n = y[v][k] * r_y;
+          acc[3][v][k] += dh[v][k] * n;
+          acc[4][v][k] += dh[v][k];
+          if (p.d_h) G[v][k] += r_y * (dh[v][k] * wpre[k] - n * m1 - m2);
+        }
+      }
+      if (p.d_x) store8<TX, VEC>(static_cast<TX*>(p.d_x) + row * d.ldx, c, Cr, G[v]);
+      if (p.o) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float n = o[v][k] * r_o;
+          const float u = d.post != TG_NORM_NONE ? n * wpost[k] + bpost[k] : o[v][k];
+          float a = 1.f, da = 0.f;
+          if (p.gate) da = gate_slope(g[v][k], d.gate_act, &a);
+          const float D = c + k < Cr ? d.alpha * G[v][k] : 0.f;
+          acc[2][v][k] += D * a * u;
+          dg[k] = D * sc[k] * u * da;
+          const float du = D * sc[k] * a;
+          acc[0][v][k] += du * n;
+          acc[1][v][k] += du;
+          o[v][k] = n;
+          G[v][k] = du * wpost[k];
+          q[0] += G[v][k] * n;
+          q[1] += G[v][k];
+        }
+        if (p.d_gate) {
+          if (d.rows_per_gate == 1) {
+            store8<TO, VEC>(static_cast<TO*>(p.d_gate) + row * d.ld_dg, c, Cr, dg);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) dga[v][k] += on ? dg[k] : 0.f;
+          }
+        }
+      }
+    }
+    if (p.o) {
+      if (d.post != TG_NORM_NONE) row_sums(q, lpr, red, turn);
+      if (p.d_o) {
+        const float n1 = d.post != TG_NORM_NONE ? q[0] * p.inv_c : 0.f, n2 = d.post == TG_NORM_LAYER ? q[1] * p.inv_c : 0.f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          const int c = (v * lpr + lane) * 8;
+          float out[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) out[k] = r_o * (G[v][k] - o[v][k] * n1 - n2);
+          store8<TO, VEC>(static_cast<TO*>(p.d_o) + row * d.ld_do, c, Cr, out);
+        }
+      }
+      // the last row of a gate row in this item: its sum is complete (whole gate rows only)
+      if (p.d_gate && p.pieces == 0 && d.rows_per_gate > 1 && on && (row + 1 == d.rows || (row + 1) % d.rows_per_gate == 0)) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          store8<TO, VEC>(static_cast<TO*>(p.d_gate) + grow * d.ld_dg, (v * lpr + lane) * 8, C, dga[v]);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) dga[v][k] = 0.f;
+        }
+      }
+    }
+  }
+  if (p.pieces > 0 && item < p.items) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) store8<float, VEC>(p.gate_part + item * C, (v * lpr + lane) * 8, C, dga[v]);
+  }
+#pragma unroll
+  for (int q = 0; q < 5; ++q) {
+    if (!(p.want >> q & 1)) continue;
+    float* out = p.part + ((int64_t)blockIdx.x * 5 + q) * C;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * lpr + lane) * 8;
+      if (rpb > 1) {                                                // NV == 1 here: several rows only where a row is narrow
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) join[(sub * lpr + lane) * 8 + k] = acc[q][v][k];
+        __syncthreads();
+        if (sub == 0) {
+          float t[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+          for (int s = 0; s < rpb; ++s) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) t[k] += join[(s * lpr + lane) * 8 + k];
+          }
+          store8<float, VEC>(out, c, C, t);
+        }
+      } else {
+        store8<float, VEC>(out, c, C, acc[q][v]);
+      }
+    }
+  }
+}
+
+struct GnOut {
+  float* p[5];
+};
+// d_param[c] = sum over the workgroups' partials, fixed order: 16 strided sums per column, then a tree over them
+__global__ __launch_bounds__(1024) void gated_norm_params_kernel(const float* __restrict__ part, int blocks, int C, GnOut out) {
+  __shared__ float sm[16][64];
+  const int q = blockIdx.y, cl = threadIdx.x & 63, c = blockIdx.x * 64 + cl, w = threadIdx.x >> 6;
+  float* dst = out.p[q];
+  if (!dst) return;
+  float s = 0.f;
+  if (c < C) {
+#pragma unroll 4
+    for (int b = w; b < blocks; b += 16) s += part[((int64_t)b * 5 + q) * C + c];
+  }
+  sm[w][cl] = s;
+  __syncthreads();
+  for (int h = 8; h > 0; h >>= 1) {
+    if (w < h) sm[w][cl] += sm[w + h][cl];
+    __syncthreads();
+  }
+  if (w == 0 && c < C) dst[c] = sm[0][cl];
+}
+
+// d_gate[group][c] = the sum of the pieces of its rows, in order
+template <typename TO>
+__global__ __launch_bounds__(256) void gated_norm_gate_kernel(const float* __restrict__ part, int64_t groups, int pieces, int C,
+                                                              TO* __restrict__ d_gate, int64_t ld) {
+  const int64_t n = groups * C;
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n; e += (int64_t)gridDim.x * 256) {
+    const int64_t gi = e / C;
+    const int c = (int)(e - gi * C);
+    float s = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < pieces; ++k) s += part[(gi * pieces + k) * C + c];
+    Elem<TO>::st(d_gate + gi * ld + c, s);
+  }
+}
+
+struct Geo {
+  int lpr_log2, lpr, block, nv, rpb, item_rows, pieces, blocks;
+  int64_t items;
+};
+
+void row_geometry(int C, Geo* g) {
+  const int oct = (C + 7) / 8;
+  int l = 0;
+  while ((1 << l) < oct && (1 << l) < GN_MAX_LPR) ++l;
+  g->lpr_log2 = l;
+  g->lpr = 1 << l;
+  g->nv = oct <= g->lpr ? 1 : (oct <= 2 * g->lpr ? 2 : 4);
+  g->block = g->lpr < 256 ? 256 : g->lpr;
+  g->rpb = g->block / g->lpr;
+}
+
+// The backward pass's split of the rows.  About 512 workgroups (two per compute unit), at least 4 rows per sub-row: every workgroup
+// writes 5 C partial values, a row of the operands is 5 - 8 times C values.
+void item_geometry(int64_t rows, int C, int64_t k, Geo* g) {
+  row_geometry(C, g);
+  int64_t m = cdiv64(rows, (int64_t)512 * g->rpb);
+  if (m < 4) m = 4;
+  g->pieces = 0;
+  if (k > 1 && k <= m) {
+    m = cdiv64(m, k) * k;
+  } else if (k > m) {
+    g->pieces = (int)cdiv64(k < rows ? k : rows, m);
+  }
+  g->item_rows = (int)m;
+  g->items = g->pieces > 0 ? cdiv64(rows, k) * g->pieces : cdiv64(rows, m);
+  g->blocks = (int)cdiv64(g->items, g->rpb);
+}
+
+int64_t part_floats(const Geo& g, int C) { return ((int64_t)g.blocks * 5 * C + 3) / 4 * 4; }
+
+bool shape_ok(int64_t rows, int C, int64_t k) {
+  return rows >= 0 && rows < ((int64_t)1 << 31) && C >= 1 && C <= TG_GATED_NORM_MAX_C && k >= 1 && k < ((int64_t)1 << 31);
+}
+
+bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// dtype pairs (rows of the blocks, residual stream): bf16 / bf16, bf16 / f32, f32 / f32
+bool types_ok(const tg_gated_norm_desc* d) {
+  return (d->dtype == TG_BF16 && (d->res_dtype == TG_BF16 || d->res_dtype == TG_F32)) || (d->dtype == TG_F32 && d->res_dtype == TG_F32);
+}
+bool codes_ok(const tg_gated_norm_desc* d) {
+  auto kind = [](int k) { return k == TG_NORM_NONE || k == TG_NORM_RMS || k == TG_NORM_LAYER; };
+  return kind(d->post) && kind(d->pre) &&
+         (d->gate_act == TG_ACT_NONE || d->gate_act == TG_ACT_SIGMOID || d->gate_act == TG_ACT_TANH || d->gate_act == TG_ACT_SILU);
+}
+// eps keeps 1 / sqrt(0 + eps) finite: the lanes past a row's end and rows of zeros rely on it
+bool eps_ok(const tg_gated_norm_desc* d) { return d->eps >= 1e-30f && d->eps <= 1e30f; }
+
+}  // namespace
+
+#define ST(s) static_cast<hipStream_t>(s)
+
+#define GN_PICK(KERN, VECV, ...)                                                                                \
+  do {                                                                                                          \
+    if (d->dtype == TG_F32) { GN_NV(KERN, float, float, VECV, __VA_ARGS__); }                                   \
+    else if (d->res_dtype == TG_F32) { GN_NV(KERN, u16, float, VECV, __VA_ARGS__); }                            \
+    else { GN_NV(KERN, u16, u16, VECV, __VA_ARGS__); }                                                          \
+  } while (0)
+#define GN_NV(KERN, TO, TX, VECV, ...)                                                                          \
+  do {                                                                                                          \
+    if (g.nv == 1) { TG_LAUNCH(name, flops, bytes, (KERN<TO, TX, 1, VECV>), __VA_ARGS__); }                     \
+    else if (g.nv == 2) { TG_LAUNCH(name, flops, bytes, (KERN<TO, TX, 2, VECV>), __VA_ARGS__); }                \
+    else { TG_LAUNCH(name, flops, bytes, (KERN<TO, TX, 4, VECV>), __VA_ARGS__); }                               \
+  } while (0)
+
+extern "C" int tg_gated_norm_forward(const tg_gated_norm_desc* d, const void* x, const void* o, const void* gate, const float* w_post,
+                                     const float* b_post, const float* scale, const float* w_pre, const float* b_pre, void* y, void* h,
+                                     void* stream) {
+  TG_CHECK_ARG(d != nullptr, "null descriptor");
+  TG_CHECK_ARG(shape_ok(d->rows, d->C, d->rows_per_gate), "rows in [0, 2^31), C in [1, TG_GATED_NORM_MAX_C], rows_per_gate in [1, 2^31)");
+  TG_CHECK_ARG(types_ok(d), "types: bf16 rows with a bf16 or f32 residual stream, or f32 rows with an f32 one");
+  TG_CHECK_ARG(eps_ok(d), "eps must lie in [1e-30, 1e30]");
+  TG_CHECK_ARG(codes_ok(d), "unknown norm kind or gate activation (none, sigmoid, tanh, silu)");
+  if (d->rows == 0) return TG_OK;                                   // an empty tensor has no address
+  TG_CHECK_ARG(o != nullptr || (d->post == TG_NORM_NONE && gate == nullptr && y == nullptr), "a post norm, a gate or y without a block output");
+  TG_CHECK_ARG((o == nullptr || y != nullptr) && (h != nullptr) == (d->pre != TG_NORM_NONE), "y goes with the block output, h with a pre norm");
+  TG_CHECK_ARG(o != nullptr || h != nullptr, "nothing to do: neither a block output nor a pre norm");
+  TG_CHECK_ARG(x != nullptr, "x is missing");
+  const int C = d->C;
+  TG_CHECK_ARG(d->ldx >= C && (!o || (d->ldo >= C && d->ldy >= C)) && (!gate || d->ldg >= C) && (!h || d->ldh >= C), "a row stride below C");
+  Geo g;
+  row_geometry(C, &g);
+  GnP p = {};
+  p.d = *d;
+  p.x = x; p.o = o; p.gate = gate;
+  p.w_post = w_post; p.b_post = b_post; p.scale = scale; p.w_pre = w_pre; p.b_pre = b_pre;
+  p.out_y = y; p.out_h = h;
+  p.lpr_log2 = g.lpr_log2;
+  p.inv_c = 1.f / (float)C;
+  const bool vec = C % 8 == 0 && al16(x) && al16(o) && al16(gate) && al16(y) && al16(h) && al16(w_post) && al16(b_post) && al16(scale) &&
+                   al16(w_pre) && al16(b_pre) && d->ldx % 8 == 0 && (!o || (d->ldo % 8 == 0 && d->ldy % 8 == 0)) &&
+                   (!gate || d->ldg % 8 == 0) && (!h || d->ldh % 8 == 0);
+  const char* const name = "gated_norm_fwd";
+  const double n = (double)d->rows * C, flops = 14 * n, ex = d->res_dtype == TG_F32 ? 4 : 2, eo = d->dtype == TG_F32 ? 4 : 2;
+  const double bytes = n * (ex + (o ? ex + eo : 0) + (gate && d->rows_per_gate == 1 ? eo : 0) + (h ? eo : 0));
+  const dim3 grid((unsigned)(cdiv64(d->rows, g.rpb) < 4096 ? cdiv64(d->rows, g.rpb) : 4096)), block(g.block);
+  if (vec) GN_PICK(gated_norm_fwd_kernel, true, grid, block, 0, ST(stream), p);
+  else GN_PICK(gated_norm_fwd_kernel, false, grid, block, 0, ST(stream), p);
+  TG_CHECK_LAUNCH();
+}
+
+extern "C" int tg_gated_norm_ws(int64_t rows, int C, int64_t rows_per_gate, int64_t* floats) {
+  TG_CHECK_ARG(floats != nullptr, "null pointer");
+  TG_CHECK_ARG(shape_ok(rows, C, rows_per_gate), "rows in [0, 2^31), C in [1, TG_GATED_NORM_MAX_C], rows_per_gate in [1, 2^31)");
+  Geo g;
+  item_geometry(rows, C, rows_per_gate, &g);
+  *floats = part_floats(g, C) + (g.pieces > 0 ? g.items * C : 0);
+  return TG_OK;
+}
+
+extern "C" int tg_gated_norm_backward(const tg_gated_norm_desc* d, const void* d_y, const void* d_h, const void* y, const void* o,
+                                      const void* gate, const float* w_post, const float* b_post, const float* scale,
+                                      const float* w_pre, const float* b_pre, void* d_x, void* d_o, void* d_gate, float* d_w_post,
+                                      float* d_b_post, float* d_scale, float* d_w_pre, float* d_b_pre, float* ws, int64_t ws_floats,
+                                      void* stream) {
+  TG_CHECK_ARG(d != nullptr, "null descriptor");
+  TG_CHECK_ARG(shape_ok(d->rows, d->C, d->rows_per_gate), "rows in [0, 2^31), C in [1, TG_GATED_NORM_MAX_C], rows_per_gate in [1, 2^31)");
+  TG_CHECK_ARG(types_ok(d), "types: bf16 rows with a bf16 or f32 residual stream, or f32 rows with an f32 one");
+  TG_CHECK_ARG(eps_ok(d), "eps must lie in [1e-30, 1e30]");
+  TG_CHECK_ARG(codes_ok(d), "unknown norm kind or gate activation (none, sigmoid, tanh, silu)");
+  TG_CHECK_ARG(d->rows == 0 || o != nullptr || (d->post == TG_NORM_NONE && gate == nullptr && !d_o && !d_scale),
+               "a post norm, a gate, d_o or d_scale without a block output");   // rows == 0: an empty tensor has no address
+  TG_CHECK_ARG(d->rows == 0 || d_gate == nullptr || gate != nullptr, "d_gate without a gate");
+  TG_CHECK_ARG(d->pre != TG_NORM_NONE || (d_h == nullptr && !d_w_pre && !d_b_pre), "d_h, d_w_pre or d_b_pre without a pre norm");
+  TG_CHECK_ARG(d->post != TG_NORM_NONE || (!d_w_post && !d_b_post), "d_w_post or d_b_post without a post norm");
+  const int C = d->C;
+  Geo g;
+  item_geometry(d->rows, C, d->rows_per_gate, &g);
+  const int64_t pf = part_floats(g, C), need = pf + (g.pieces > 0 ? g.items * C : 0);
+  TG_CHECK_ARG(d->rows == 0 || (y != nullptr && ws != nullptr && al16(ws) && ws_floats >= need), "y, or a workspace of tg_gated_norm_ws() floats, is missing");
+  TG_CHECK_ARG((!d_y || d->ld_dy >= C) && (!d_h || d->ldh >= C) && d->ldy >= C && (!o || d->ldo >= C) && (!gate || d->ldg >= C) &&
+                   (!d_x || d->ldx >= C) && (!d_o || d->ld_do >= C) && (!d_gate || d->ld_dg >= C),
+               "a row stride below C");
+  const int want = (d_w_post ? 1 : 0) | (d_b_post ? 2 : 0) | (d_scale ? 4 : 0) | (d_w_pre ? 8 : 0) | (d_b_pre ? 16 : 0);
+  if (d->rows > 0) {
+    GnP p = {};
+    p.d = *d;
+    p.y = y; p.o = o; p.gate = gate; p.d_y = d_y; p.d_h = d_h;
+    p.w_post = w_post; p.b_post = b_post; p.scale = scale; p.w_pre = w_pre; p.b_pre = b_pre;
+    p.d_x = d_x; p.d_o = d_o; p.d_gate = d_gate;
+    p.part = ws;
+    p.gate_part = ws + pf;
+    p.lpr_log2 = g.lpr_log2;
+    p.item_rows = g.item_rows; p.pieces = g.pieces; p.items = g.items;
+    p.want = want;
+    p.inv_c = 1.f / (float)C;
+    const bool vec = C % 8 == 0 && al16(d_y) && al16(d_h) && al16(y) && al16(o) && al16(gate) && al16(w_post) && al16(b_post) &&
+                     al16(scale) && al16(w_pre) && al16(d_x) && al16(d_o) && al16(d_gate) && (!d_y || d->ld_dy % 8 == 0) &&
+                     (!d_h || d->ldh % 8 == 0) && d->ldy % 8 == 0 && (!o || d->ldo % 8 == 0) && (!gate || d->ldg % 8 == 0) &&
+                     (!d_x || d->ldx % 8 == 0) && (!d_o || d->ld_do % 8 == 0) && (!d_gate || d->ld_dg % 8 == 0);
+    const char* const name = "gated_norm_bwd";
+    const double n = (double)d->rows * C, flops = 40 * n, ex = d->res_dtype == TG_F32 ? 4 : 2, eo = d->dtype == TG_F32 ? 4 : 2;
+    const double bytes = n * (ex * (1 + (d_y ? 1 : 0) + (d_x ? 1 : 0)) + eo * ((d_h ? 1 : 0) + (o ? 1 : 0) + (d_o ? 1 : 0)));
+    const dim3 grid((unsigned)g.blocks), block(g.block);
+    const size_t lds = g.rpb > 1 ? (size_t)g.block * 8 * sizeof(float) : 0;
+    if (vec) GN_PICK(gated_norm_bwd_kernel, true, grid, block, lds, ST(stream), p);
+    else GN_PICK(gated_norm_bwd_kernel, false, grid, block, lds, ST(stream), p);
+    if (d_gate && g.pieces > 0) {
+      const int64_t groups = cdiv64(d->rows, d->rows_per_gate);
+      const dim3 gg(grid_1d(groups * C, 256));
+      if (d->dtype == TG_F32)
+        hipLaunchKernelGGL((gated_norm_gate_kernel<float>), gg, dim3(256), 0, ST(stream), p.gate_part, groups, g.pieces, C, (float*)d_gate, d->ld_dg);
+      else
+        hipLaunchKernelGGL((gated_norm_gate_kernel<u16>), gg, dim3(256), 0, ST(stream), p.gate_part, groups, g.pieces, C, (u16*)d_gate, d->ld_dg);
+    }
+  }
+  if (want) {
+    const GnOut out = {{d_w_post, d_b_post, d_scale, d_w_pre, d_b_pre}};
+    hipLaunchKernelGGL(gated_norm_params_kernel, dim3((C + 63) / 64, 5), dim3(1024), 0, ST(stream), ws, d->rows > 0 ? g.blocks : 0, C, out);
+  }
+  TG_CHECK_LAUNCH();
+}

@@ -5,7 +5,8 @@ import ctypes as C
 import torch
 
 from . import _lib as L
-from ._lib import CONV_COEXIST, ConvDesc, TG_BF16, TG_F32, check, lib  # noqa: F401
+from ._lib import (ACT_NONE, ACT_SIGMOID, ACT_SILU, ACT_TANH, CONV_COEXIST, ConvDesc, NORM_LAYER, NORM_NONE, NORM_RMS, TG_BF16,  # noqa: F401
+                   TG_F32, TG_FP8_E4M3, TG_FP8_E5M2, check, lib)
 
 
 def _stream():
@@ -553,6 +554,316 @@ def frame_to_u8(frame, out, bgr=False):
     """frame [...,3] fp32 in [0,1] -> out uint8, truncating like save_img (lib/ops.py:521-523)."""
     check(lib().tg_frame_to_u8(_p(frame), _p(out), frame.numel() // 3, int(bgr), _stream()), "tg_frame_to_u8")
     return out
+
+
+# ---- sequence-block operators: gated residual norm, block-scaled fp8 product, gated linear recurrence ------------------------------
+# Beside the functions above: rows may have a stride, shapes and types are checked here (TecoHipError), and a call belongs to the
+# current device: tensors of another one are refused.
+_FLOATS = {torch.float32: TG_F32, torch.bfloat16: TG_BF16}
+_FP8 = {torch.float8_e4m3fn: TG_FP8_E4M3, torch.float8_e5m2: TG_FP8_E5M2}
+FP8_DTYPES = {"e4m3": torch.float8_e4m3fn, "e5m2": torch.float8_e5m2}
+
+
+def _need(ok, what):
+    if not ok:
+        raise L.TecoHipError(what)
+
+
+def _on_device(*ts):
+    """Every tensor on the current device (None: not given); the raw handle of its current stream."""
+    dev = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    for t in ts:
+        if t is not None:
+            _need(t.is_cuda, "tensor is not on the GPU: tecogan_amd has no CPU path")
+            _need(t.get_device() == dev, "tensor is on another device than the current one")
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+def _rows(t, rows, C, dtype, what):
+    """Pointer and row stride of `t`, [..., C] with `rows` rows: contiguous channels, one stride between its rows."""
+    if t is None:
+        return None, 0
+    _need(t.dtype == dtype, "%s: %s expected, got %s" % (what, dtype, t.dtype))
+    _need(t.dim() >= 1 and t.shape[-1] == C and t.numel() == rows * C, "%s: %d rows of %d expected, got %s" % (what, rows, C, tuple(t.shape)))
+    if t.is_contiguous():
+        return t.data_ptr(), C
+    _need(t.stride(-1) == 1 or C == 1, "%s: the last dimension must be contiguous" % what)
+    ld, n = None, 1                                        # innermost row dimension outwards
+    for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if size == 1:
+            continue
+        _need(ld is None or stride == ld * n, "%s: its rows have no common stride" % what)
+        ld = stride if ld is None else ld
+        n *= size
+    ld = C if ld is None else ld
+    _need(ld >= C, "%s: rows overlap" % what)
+    return t.data_ptr(), ld
+
+
+def _vector(t, n, what, dtype=torch.float32):
+    if t is None:
+        return None
+    _need(t.dtype == dtype and t.numel() == n and t.is_contiguous(), "%s: %d contiguous values of %s expected" % (what, n, dtype))
+    return t.data_ptr()
+
+
+def _norm_desc(x, o, gate, rows, Cn, post, pre, alpha, gate_act, rows_per_gate, eps):
+    rdt = _FLOATS.get(x.dtype)
+    _need(rdt is not None, "unsupported dtype %s" % x.dtype)
+    d = L.GatedNormDesc()
+    d.rows, d.rows_per_gate, d.C, d.res_dtype, d.post, d.pre = rows, rows_per_gate, Cn, rdt, post, pre
+    d.gate_act, d.alpha, d.eps = gate_act, alpha, eps
+    return d
+
+
+def _gate_rows(rows, rows_per_gate):
+    _need(rows_per_gate >= 1, "rows_per_gate must be positive")
+    return -(-rows // rows_per_gate)
+
+
+def gated_norm_forward(x, o, gate, y, h, post=NORM_NONE, pre=NORM_RMS, w_post=None, b_post=None, scale=None, w_pre=None, b_pre=None,
+                       alpha=1.0, gate_act=ACT_NONE, rows_per_gate=1, eps=1e-6):
+    """The boundary between two blocks in one launch: y = x + alpha * scale * act(gate) * post(o), h = pre(y).
+
+    x, y [..., C]: the residual stream before and after (bf16, or f32 beside bf16 blocks; y may be x).  o: the output of the block
+    that ends, h: the input of the block that begins (pre = NORM_NONE: None).  gate: None, a row for each row of o, or one for each
+    `rows_per_gate` rows in a row.  Parameters: fp32 [C] or None.  o = None (then gate and y too): h = pre(x) alone.  Returns y, h."""
+    stream = _on_device(x, o, gate, y, h, w_post, b_post, scale, w_pre, b_pre)
+    Cn = x.shape[-1] if x.dim() else 0
+    _need(Cn >= 1, "x: [..., C] with C >= 1 expected")
+    rows = x.numel() // Cn
+    like = o if o is not None else h
+    _need(like is not None, "nothing to do: neither a block output nor a pre norm")
+    d = _norm_desc(x, o, gate, rows, Cn, post, pre, alpha, gate_act, rows_per_gate, eps)
+    d.dtype = dt(like)
+    px, d.ldx = _rows(x, rows, Cn, x.dtype, "x")
+    po, d.ldo = _rows(o, rows, Cn, like.dtype, "o")
+    pg, d.ldg = _rows(gate, _gate_rows(rows, rows_per_gate), Cn, like.dtype, "gate")
+    py, d.ldy = _rows(y, rows, Cn, x.dtype, "y")
+    ph, d.ldh = _rows(h, rows, Cn, like.dtype, "h")
+    check(lib().tg_gated_norm_forward(C.byref(d), px, po, pg, _vector(w_post, Cn, "w_post"), _vector(b_post, Cn, "b_post"),
+                                      _vector(scale, Cn, "scale"), _vector(w_pre, Cn, "w_pre"), _vector(b_pre, Cn, "b_pre"), py, ph, stream),
+          "tg_gated_norm_forward")
+    return y, h
+
+
+def gated_norm_ws(rows, channels, rows_per_gate=1):
+    """fp32 values of gated_norm_backward's workspace."""
+    n = C.c_int64(0)
+    check(lib().tg_gated_norm_ws(rows, channels, rows_per_gate, C.byref(n)), "tg_gated_norm_ws")
+    return n.value
+
+
+def gated_norm_backward(d_y, d_h, y, o, gate, d_x, d_o, d_gate, ws, post=NORM_NONE, pre=NORM_RMS, w_post=None, b_post=None, scale=None,
+                        w_pre=None, b_pre=None, alpha=1.0, gate_act=ACT_NONE, rows_per_gate=1, eps=1e-6, d_w_post=None, d_b_post=None,
+                        d_scale=None, d_w_pre=None, d_b_pre=None):
+    """Gradients of gated_norm_forward from d_y, d_h (None: zero) and the forward pass's y (x where o is None), o and gate.  Outputs
+    that are None are not computed; parameter gradients are overwritten.  ws: fp32, gated_norm_ws(rows, C, rows_per_gate) values."""
+    stream = _on_device(d_y, d_h, y, o, gate, d_x, d_o, d_gate, ws, w_post, b_post, scale, w_pre, b_pre, d_w_post, d_b_post, d_scale,
+                        d_w_pre, d_b_pre)
+    Cn = y.shape[-1] if y.dim() else 0
+    _need(Cn >= 1, "y: [..., C] with C >= 1 expected")
+    rows = y.numel() // Cn
+    like = o if o is not None else (d_h if d_h is not None else y)
+    d = _norm_desc(y, o, gate, rows, Cn, post, pre, alpha, gate_act, rows_per_gate, eps)
+    d.dtype = dt(like)
+    groups = _gate_rows(rows, rows_per_gate)
+    pdy, d.ld_dy = _rows(d_y, rows, Cn, y.dtype, "d_y")
+    pdh, d.ldh = _rows(d_h, rows, Cn, like.dtype, "d_h")
+    py, d.ldy = _rows(y, rows, Cn, y.dtype, "y")
+    po, d.ldo = _rows(o, rows, Cn, like.dtype, "o")
+    pg, d.ldg = _rows(gate, groups, Cn, like.dtype, "gate")
+    pdx, d.ldx = _rows(d_x, rows, Cn, y.dtype, "d_x")
+    pdo, d.ld_do = _rows(d_o, rows, Cn, like.dtype, "d_o")
+    pdg, d.ld_dg = _rows(d_gate, groups, Cn, like.dtype, "d_gate")
+    _need(ws is not None and ws.dtype == torch.float32 and ws.is_contiguous(), "ws: contiguous fp32 values expected")
+    v = _vector
+    check(lib().tg_gated_norm_backward(C.byref(d), pdy, pdh, py, po, pg, v(w_post, Cn, "w_post"), v(b_post, Cn, "b_post"),
+                                       v(scale, Cn, "scale"), v(w_pre, Cn, "w_pre"), v(b_pre, Cn, "b_pre"), pdx, pdo, pdg,
+                                       v(d_w_post, Cn, "d_w_post"), v(d_b_post, Cn, "d_b_post"), v(d_scale, Cn, "d_scale"),
+                                       v(d_w_pre, Cn, "d_w_pre"), v(d_b_pre, Cn, "d_b_pre"), ws.data_ptr(), ws.numel(), stream),
+          "tg_gated_norm_backward")
+    return d_x
+
+
+def _fp8_shapes(rows, cols, tile):
+    kb = -(-cols // 128)
+    return (rows, kb * 128), (-(-rows // 128) if tile else rows, -(-kb // 4) * 4)
+
+
+def fp8_alloc(rows, cols, device, fmt="e4m3", tile=False, transposed=False):
+    """Storage of a [rows, cols] matrix as fp8_quantize writes it: q, scale (uint8 exponents), with `transposed` also qt, scale_t."""
+    _need(fmt in FP8_DTYPES, "8-bit types are %s" % sorted(FP8_DTYPES))
+    out = []
+    for a, b in ((rows, cols), (cols, rows))[:2 if transposed else 1]:
+        q, s = _fp8_shapes(a, b, tile)
+        out += [torch.empty(q, device=device, dtype=FP8_DTYPES[fmt]), torch.empty(s, device=device, dtype=torch.uint8)]
+    return tuple(out)
+
+
+def _fp8_operand(q, s, what):
+    """(format, rows, padded columns, scales per tile) of an operand, checked."""
+    fmt = _FP8.get(q.dtype)
+    _need(fmt is not None, "%s: float8_e4m3fn or float8_e5m2 expected, got %s" % (what, q.dtype))
+    _need(q.dim() == 2 and q.is_contiguous() and q.shape[1] % 128 == 0, "%s: contiguous [rows, columns padded to 128] expected" % what)
+    rows, cols = q.shape
+    pitch = -(-(cols // 128) // 4) * 4
+    _need(s.dtype == torch.uint8 and s.is_contiguous() and s.dim() == 2 and s.shape[1] == pitch and s.shape[0] in (rows, -(-rows // 128)),
+          "%s: its scales must be contiguous uint8 [%d or %d, %d], got %s" % (what, rows, -(-rows // 128), pitch, tuple(s.shape)))
+    return fmt, rows, cols, int(s.shape[0] != rows)
+
+
+def fp8_quantize(x, q, scale, qt=None, scale_t=None, tile=False):
+    """x [..., cols] (bf16 / f32) as 8-bit floating point with one power-of-two scale for each block of 128: q with its blocks along
+    the columns, qt (the transposed copy) with its blocks along the rows; `tile`: one scale for each 128 x 128 tile in both.  Either
+    copy may be None with its scales.  Shapes: fp8_alloc.  A NaN or infinity stays one and does not touch its block's scale."""
+    stream = _on_device(x, q, scale, qt, scale_t)
+    cols = x.shape[-1] if x.dim() else 0
+    _need(cols >= 1, "x: [..., columns] expected")
+    rows = x.numel() // cols
+    px, ld = _rows(x, rows, cols, x.dtype, "x")
+    _need(q is not None or qt is not None, "neither order is asked for")
+    fmts = set()
+    for t, s, a, b, what in ((q, scale, rows, cols, "q"), (qt, scale_t, cols, rows, "qt")):
+        _need((t is None) == (s is None), "%s goes with its scales" % what)
+        if t is not None:
+            sq, ss = _fp8_shapes(a, b, tile)
+            _need(t.dtype in _FP8 and tuple(t.shape) == sq and t.is_contiguous(), "%s: contiguous 8-bit floats %s expected" % (what, sq))
+            _need(s.dtype == torch.uint8 and tuple(s.shape) == ss and s.is_contiguous(), "%s: contiguous uint8 scales %s expected" % (what, ss))
+            fmts.add(_FP8[t.dtype])
+    _need(len(fmts) == 1, "q and qt must have the same type")
+    check(lib().tg_fp8_quantize(px, dt(x), rows, cols, ld, fmts.pop(), int(bool(tile)), _at(q), _at(scale), _at(qt), _at(scale_t), stream),
+          "tg_fp8_quantize")
+
+
+def fp8_matmul(a, scale_a, b, scale_b, out, bias=None, accumulate=False):
+    """out [M, N] (bf16 / f32) = a [M, K] b [N, K]^T (+ bias fp32 [N]) (+ out): operands and scales as fp8_quantize writes them, the
+    scales of each per row or per tile (by their shape).  fp32 sums; accumulate: f32 outputs only."""
+    stream = _on_device(a, scale_a, b, scale_b, out, bias)
+    d = L.Fp8MatmulDesc()
+    d.a_fmt, M, K, d.a_tile = _fp8_operand(a, scale_a, "a")
+    d.b_fmt, N, Kb, d.b_tile = _fp8_operand(b, scale_b, "b")
+    _need(K == Kb, "a and b differ in their padded columns: %d and %d" % (K, Kb))
+    d.M, d.N, d.K = M, N, K
+    po, d.ldo = _rows(out, M, N, out.dtype, "out")
+    d.out_dtype, d.accumulate = dt(out), int(bool(accumulate))
+    check(lib().tg_fp8_matmul(C.byref(d), a.data_ptr(), scale_a.data_ptr(), b.data_ptr(), scale_b.data_ptr(), _vector(bias, N, "bias"), po,
+                              stream), "tg_fp8_matmul")
+    return out
+
+
+def fp8_linear_ws(M, N, K):
+    """Bytes of fp8_linear's workspace."""
+    n = C.c_int64(0)
+    check(lib().tg_fp8_linear_ws(M, N, K, C.byref(n)), "tg_fp8_linear_ws")
+    return n.value
+
+
+def fp8_linear(x, w, scale_w, out, ws, bias=None):
+    """out [..., N] = x [..., K] W^T + bias with x quantised on the way (e4m3, a scale per row and 128 columns): w [N, K padded] and its
+    tile scales from fp8_quantize(W, ..., tile=True).  ws: uint8, fp8_linear_ws(rows, N, K) bytes."""
+    stream = _on_device(x, w, scale_w, out, ws, bias)
+    K = x.shape[-1] if x.dim() else 0
+    _need(K >= 1, "x: [..., K] expected")
+    M = x.numel() // K
+    fmt, N, Kp, tile = _fp8_operand(w, scale_w, "w")
+    _need(Kp == -(-K // 128) * 128, "x has %d columns, w %d (padded)" % (K, Kp))
+    _need(scale_w.shape[0] == -(-N // 128), "w: scales per tile expected")
+    px, ld = _rows(x, M, K, x.dtype, "x")
+    po, ldo = _rows(out, M, N, out.dtype, "out")
+    _need(ws.dtype == torch.uint8 and ws.is_contiguous(), "ws: contiguous bytes expected")
+    check(lib().tg_fp8_linear(px, dt(x), M, K, ld, w.data_ptr(), scale_w.data_ptr(), N, fmt, _vector(bias, N, "bias"), po, dt(out), ldo,
+                              ws.data_ptr(), ws.numel(), stream), "tg_fp8_linear")
+    return out
+
+
+def _scan_sizes(B, T, D):
+    a, b = C.c_int64(0), C.c_int64(0)
+    check(lib().tg_gated_scan_sizes(B, T, D, C.byref(a), C.byref(b)), "tg_gated_scan_sizes")
+    return a.value, b.value
+
+
+def gated_scan_carry(B, T, D):
+    """fp32 values of gated_scan_forward's carry."""
+    return _scan_sizes(B, T, D)[0]
+
+
+def gated_scan_ws(B, T, D):
+    """fp32 values of gated_scan_backward's workspace."""
+    return _scan_sizes(B, T, D)[1]
+
+
+def _steps(t, shape, dtype, what):
+    """Pointer and strides (step, batch row) of a [B, T, D] tensor with contiguous channels."""
+    if t is None:
+        return None, 0, 0
+    _need(tuple(t.shape) == shape and t.dtype == dtype, "%s: %s of %s expected, got %s of %s" % (what, shape, dtype, tuple(t.shape), t.dtype))
+    B, T, D = shape
+    sb, st, sd = t.stride()
+    _need(sd == 1 or D == 1, "%s: channels must be contiguous" % what)
+    st = D if T == 1 else st
+    sb = T * st if B == 1 else sb
+    _need(st >= D and sb >= D, "%s: steps overlap" % what)
+    return t.data_ptr(), st, sb
+
+
+def _scan_masks(B, T, lengths, reset):
+    if reset is not None:
+        _need(reset.dtype in (torch.uint8, torch.bool) and tuple(reset.shape) == (B, T) and reset.is_contiguous(),
+              "reset: contiguous bytes [B, T] expected")
+    return _vector(lengths, B, "lengths", torch.int32), _at(reset)
+
+
+def gated_scan_forward(x, g, y, hT, carry, h0=None, floor=None, lengths=None, reset=None, keep=True):
+    """h[t] = f[t] h[t-1] + (1 - f[t]) x[t], f = floor + (1 - floor) sigmoid(g), along dimension 1 of x, g, y [B, T, D] (bf16 / f32,
+    channels contiguous); y = h, hT [B, D] fp32 or None = the last state.  h0 [B, D] fp32: the state before (None: zero); floor [D]
+    fp32 in [0, 1); lengths [B] int32: steps at and behind a row's length keep the state and write y = 0; reset [B, T] bytes: not 0
+    drops the state before the step (packed sequences).  carry: fp32, gated_scan_carry(B, T, D) values; with `keep` it holds what
+    gated_scan_backward needs.  Without, carry may be None where the
+    sequence needs no scratch (up to 64 steps always; longer ones are refused where they are cut into chunks).  Returns y."""
+    stream = _on_device(x, g, y, hT, carry, h0, floor, lengths, reset)
+    _need(x.dim() == 3 and x.shape[1] >= 1, "x: [B, T, D] with T >= 1 expected")
+    shape = tuple(x.shape)
+    B, T, D = shape
+    d = L.GatedScanDesc()
+    d.B, d.T, d.D, d.dtype = B, T, D, dt(x)
+    px, d.x_t, d.x_b = _steps(x, shape, x.dtype, "x")
+    pg, d.g_t, d.g_b = _steps(g, shape, x.dtype, "g")
+    py, d.y_t, d.y_b = _steps(y, shape, x.dtype, "y")
+    pl, pr = _scan_masks(B, T, lengths, reset)
+    n = 0 if carry is None else carry.numel()
+    check(lib().tg_gated_scan_forward(C.byref(d), px, pg, _vector(h0, B * D, "h0"), _vector(floor, D, "floor"), pl, pr, py,
+                                      _vector(hT, B * D, "hT"), _vector(carry, n, "carry"), n, int(bool(keep)), stream),
+          "tg_gated_scan_forward")
+    return y
+
+
+def gated_scan_backward(x, g, d_y, d_hT, carry, d_x, d_g, ws, h0=None, floor=None, lengths=None, reset=None, d_h0=None, d_floor=None):
+    """Gradients of gated_scan_forward(..., keep=True) for the same inputs, from d_y (None: zero), d_hT (None: zero) and the carry it
+    kept; d_h0, d_floor None: not wanted.  ws: fp32, gated_scan_ws(B, T, D) values."""
+    stream = _on_device(x, g, d_y, d_hT, carry, d_x, d_g, ws, h0, floor, lengths, reset, d_h0, d_floor)
+    _need(x.dim() == 3 and x.shape[1] >= 1, "x: [B, T, D] with T >= 1 expected")
+    _need(d_h0 is None or h0 is not None, "d_h0 without h0")
+    shape = tuple(x.shape)
+    B, T, D = shape
+    d = L.GatedScanDesc()
+    d.B, d.T, d.D, d.dtype = B, T, D, dt(x)
+    px, d.x_t, d.x_b = _steps(x, shape, x.dtype, "x")
+    pg, d.g_t, d.g_b = _steps(g, shape, x.dtype, "g")
+    pe, d.dy_t, d.dy_b = _steps(d_y, shape, x.dtype, "d_y")
+    pdx, d.dx_t, d.dx_b = _steps(d_x, shape, x.dtype, "d_x")
+    pdg, d.dg_t, d.dg_b = _steps(d_g, shape, x.dtype, "d_g")
+    pl, pr = _scan_masks(B, T, lengths, reset)
+    _need(carry is not None, "the carry of the forward pass is missing")
+    n, m = carry.numel(), 0 if ws is None else ws.numel()
+    check(lib().tg_gated_scan_backward(C.byref(d), px, pg, _vector(floor, D, "floor"), pl, pr, pe, _vector(d_hT, B * D, "d_hT"),
+                                       _vector(carry, n, "carry"), n, pdx, pdg, _vector(d_h0, B * D, "d_h0"),
+                                       _vector(d_floor, D, "d_floor"), _vector(ws, m, "ws"), m, stream), "tg_gated_scan_backward")
+    return d_x
 
 
 # ---- built-in launch profiler (csrc/runtime.hip) -----------------------------------------------------
