@@ -16,6 +16,7 @@
 //
 // The instruction's rows are n and its columns m: a lane holds four neighbouring n of one m.
 #include "common.h"
+#include <type_traits>
 
 namespace {
 
@@ -27,15 +28,37 @@ struct MmP {
   const float* bias;
   void* out;
   int64_t M, N, ldo;
+  int tiles_m, tiles_n, tiles;
   int K, sp;                                                          // bytes of a row, of a row of scales
   int sh_a, sh_b;                                                     // row -> row of scales: 0, or 7 for tiles
   int out_bf16, accumulate, vec;
 };
 
-// the instruction's format codes: 0 e4m3, 1 e5m2
+// c += b a over a block of K, in place: written as assembly because the compiler, left to choose, gives the 64 accumulators of the
+// largest tile other registers from one product to the next and copies them back (1300 moves a block of K).  The wait states in
+// front cover a scale or a widened operand that vector instructions have just written (two states; the matrix unit is busy with the
+// product before, so they cost nothing); results are read by nothing but the next product into the same registers until settle().
+// The instruction's format codes: 0 e4m3, 1 e5m2.
 template <int FB, int FA>
-__device__ __forceinline__ f32x4 mfma_block(i32x8 b, i32x8 a, f32x4 c, int sb, int sa) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, c, FB, FA, 0, sb, 0, sa);
+__device__ __forceinline__ void mfma_block(f32x4& c, i32x8 b, i32x8 a, int sb, int sa) {
+#ifdef __HIP_DEVICE_COMPILE__                                           // the host pass does not know the registers
+  asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:%5 blgp:%6"
+               : "+a"(c) : "v"(b), "v"(a), "v"(sb), "v"(sa), "n"(FB), "n"(FA));
+#endif
+}
+__device__ __forceinline__ void mfma_wide(f32x4& c, bf16x8 b, bf16x8 a) {
+#ifdef __HIP_DEVICE_COMPILE__
+  asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(b), "v"(a));
+#endif
+}
+// Results are whole from here on: 32 wait states behind the last product (16 passes at most), then every accumulator passes an
+// empty statement so that no read of it is moved in front.
+template <int N>
+__device__ __forceinline__ void settle(f32x4 (&c)[N]) {
+#ifdef __HIP_DEVICE_COMPILE__
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+a"(c[i]));
+#endif
 }
 
 typedef __bf16 bf16x2m __attribute__((ext_vector_type(2)));
@@ -58,101 +81,234 @@ __device__ __forceinline__ bf16x8 widen(int lo, int hi, float scale) {
   return bf16x8{v[0][0], v[0][1], v[1][0], v[1][1], v[2][0], v[2][1], v[3][0], v[3][1]};
 }
 
-// 128 x 128 outputs, four waves of 64 x 64.  LDS rows are the 128 bytes of one block of K; the 16-byte chunk c of row r sits at
-// chunk c ^ ((r >> 1) & 7).  A lane's 32 bytes are chunks g and g + 4 (g = lane / 16) in both operands: any order of k serves.
-template <int FB, int FA, bool WIDE>
-__global__ __launch_bounds__(256) void fp8_matmul_kernel(MmP p) {
-  __shared__ __attribute__((aligned(16))) unsigned char sA[128 * 128], sB[128 * 128];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, g = lane >> 4;
-  const int64_t nb = (p.N + 127) / 128, m0 = (int64_t)(blockIdx.x / nb) * 128, n0 = (int64_t)(blockIdx.x % nb) * 128;
-  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-  f32x4 acc[4][4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const unsigned char *ra[4], *rb[4];                                 // this thread's rows, clamped: what is past the end is not stored
-  int64_t qa[4], qb[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = (tid + 256 * i) >> 3;
-    const int64_t m = m0 + row < p.M ? m0 + row : p.M - 1, n = n0 + row < p.N ? n0 + row : p.N - 1;
-    ra[i] = p.a + m * p.K + (tid & 7) * 16;
-    rb[i] = p.b + n * p.K + (tid & 7) * 16;
-    const int64_t ms = m0 + wm + 16 * i + r16, ns = n0 + wn + 16 * i + r16;
-    qa[i] = ((ms < p.M ? ms : p.M - 1) >> p.sh_a) * p.sp;
-    qb[i] = ((ns < p.N ? ns : p.N - 1) >> p.sh_b) * p.sp;
+typedef __attribute__((address_space(3))) void lds_void_m;
+// 16 bytes a lane from rsrc[voff + soff] to lds + 16 lane
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rsrc, unsigned char* lds, int voff, int soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_m*)lds, 16, voff, soff, 0, 0);
+}
+
+// 32 MF x 32 NF outputs, four waves of 16 MF x 16 NF.  A stage of LDS holds one block of K of both operands, rows of 128 bytes, filled
+// by 16-byte DMA from global memory, and the scale dwords of its rows; two stages in turn.  The 16-byte chunk c of row r sits at chunk
+// c ^ ((r >> 1) & 7) (chosen on the global side): a lane's 32 bytes are chunks g and g + 4 (g = lane / 16) in both operands -- any
+// order of k serves -- and the 16 lanes that a ds_read_b128 serves together cover all 64 banks once.
+//
+// A block of K is four quarters: half of the wave's rows x half of its columns, (a0, b0), (a0, b1), (a1, b1), (a1, b0).  Between a
+// quarter's products the fragments that the next quarters need are read, each into the registers of the one that has just been used
+// up: b1, a1 of this block, then a0 and -- column by column, as (a1, b0) finishes with them -- b0 of the next.  The one barrier of a
+// block sits in its middle: there every wave has read the last of this stage and its own DMA of the next stage has landed; the DMA
+// of the block after that goes out between the products of the second half.
+template <int FB, int FA, bool WIDE, int MF, int NF>
+__global__ __launch_bounds__(256, MF * NF >= 64 ? 1 : 2) void fp8_tile_kernel(MmP p) {
+  constexpr int TM = 32 * MF, TN = 32 * NF, STAGE = (TM + TN) * 132, HM = MF / 2, HN = NF / 2;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g = lane >> 4;
+  const int wm = wave >> 1, wn = wave & 1;
+  // tile of this workgroup: XCD x (linear id % 8) owns consecutive tiles of an order that walks 8 tile rows down before the next column
+  int t = blockIdx.x;
+  {
+    const int full = p.tiles / 8 * 8;
+    if (t < full) t = (t & 7) * (full / 8) + (t >> 3);
   }
-  for (int k = 0; k < p.K; k += 128) {
-    uint4 va[4], vb[4];
+  const int band = t / (8 * p.tiles_n), rest = t - band * 8 * p.tiles_n, left = p.tiles_m - band * 8, deep = left < 8 ? left : 8;
+  const int64_t m0 = (int64_t)__builtin_amdgcn_readfirstlane(band * 8 + rest % deep) * TM;
+  const int64_t n0 = (int64_t)__builtin_amdgcn_readfirstlane(rest / deep) * TN;
+
+  const int rows_a = (int)(p.M - m0 < TM ? p.M - m0 : TM), rows_b = (int)(p.N - n0 < TN ? p.N - n0 : TN), nkb = p.K >> 7;
+  const auto rsrcA = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.a + m0 * p.K), 0, rows_a * p.K, 0x00020000);
+  const auto rsrcB = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.b + n0 * p.K), 0, rows_b * p.K, 0x00020000);
+  int oa[MF], ob[NF];                                                 // DMA sources: rows past the end read the last one (not stored)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      va[i] = *reinterpret_cast<const uint4*>(ra[i] + k);
-      vb[i] = *reinterpret_cast<const uint4*>(rb[i] + k);
-    }
-    __syncthreads();
+  for (int i = 0; i < MF; ++i) {
+    const int row = (wave * MF + i) * 8 + (lane >> 3);
+    oa[i] = (row < rows_a ? row : rows_a - 1) * p.K + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
+  }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int s = tid + 256 * i, row = s >> 3, at = row * 128 + (((s & 7) ^ ((row >> 1) & 7)) << 4);
-      *reinterpret_cast<uint4*>(sA + at) = va[i];
-      *reinterpret_cast<uint4*>(sB + at) = vb[i];
-    }
-    __syncthreads();
-    i32x8 fa[4], fb[4];
-    int ca[4], cb[4];
+  for (int i = 0; i < NF; ++i) {
+    const int row = (wave * NF + i) * 8 + (lane >> 3);
+    ob[i] = (row < rows_b ? row : rows_b - 1) * p.K + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
+  }
+  auto dma_at = [&](int q, int stage, int kb) {                       // instruction q of block kb into stage % 2
+    unsigned char* const st = smem + (stage & 1) * STAGE;
+    if (q < MF) dma16(rsrcA, st + (wave * MF + q) * 1024, oa[q < MF ? q : 0], kb * 128);
+    else dma16(rsrcB, st + TM * 128 + (wave * NF + q - MF) * 1024, ob[q < MF ? 0 : q - MF], kb * 128);
+  };
+  // scales: a dword DMA takes the four bytes around block kb of 64 rows: wave w those of A's and of B's rows 64 w .. 64 w + 63
+  const auto rsrcSA = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.sa + (m0 >> p.sh_a) * p.sp), 0, (((rows_a - 1) >> p.sh_a) + 1) * p.sp, 0x00020000);
+  const auto rsrcSB = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.sb + (n0 >> p.sh_b) * p.sp), 0, (((rows_b - 1) >> p.sh_b) + 1) * p.sp, 0x00020000);
+  const int osa = ((tid < rows_a ? tid : rows_a - 1) >> p.sh_a) * p.sp, osb = ((tid < rows_b ? tid : rows_b - 1) >> p.sh_b) * p.sp;
+  auto dma_scales_at = [&](int stage, int kb) {
+    unsigned char* const st = smem + (stage & 1) * STAGE + (TM + TN) * 128;
+    if (wave * 64 < TM) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrcSA, (lds_void_m*)(st + wave * 256), 4, osa, kb & ~3, 0, 0);
+    if (wave * 64 < TN) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrcSB, (lds_void_m*)(st + TM * 4 + wave * 256), 4, osb, kb & ~3, 0, 0);
+  };
+
+  f32x4 acc[MF][NF];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row_a = wm + 16 * i + r16, row_b = wn + 16 * i + r16;
-      const i32x4m a0 = *reinterpret_cast<const i32x4m*>(sA + row_a * 128 + ((g ^ ((row_a >> 1) & 7)) << 4));
-      const i32x4m a1 = *reinterpret_cast<const i32x4m*>(sA + row_a * 128 + (((g + 4) ^ ((row_a >> 1) & 7)) << 4));
-      const i32x4m b0 = *reinterpret_cast<const i32x4m*>(sB + row_b * 128 + ((g ^ ((row_b >> 1) & 7)) << 4));
-      const i32x4m b1 = *reinterpret_cast<const i32x4m*>(sB + row_b * 128 + (((g + 4) ^ ((row_b >> 1) & 7)) << 4));
-      fa[i] = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
-      fb[i] = __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7);
-      ca[i] = p.sa[qa[i] + (k >> 7)];
-      cb[i] = p.sb[qb[i] + (k >> 7)];
-    }
+  for (int i = 0; i < MF; ++i)
+#pragma unroll
+    for (int j = 0; j < NF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  i32x8 fa[2][HM], fb[2][HN];
+  int ca[2][HM], cb[2][HN];
+  // this lane's addresses in the stage that is read: low and high chunks of a fragment, its scale
+  const int la = r16 * 128 + ((g ^ (r16 >> 1)) << 4);
+  const unsigned char* pal = smem + wm * 16 * MF * 128 + la;
+  const unsigned char* pah = smem + ((wm * 16 * MF * 128 + la) ^ 64);
+  const unsigned char* pbl = smem + TM * 128 + wn * 16 * NF * 128 + la;
+  const unsigned char* pbh = smem + ((TM * 128 + wn * 16 * NF * 128 + la) ^ 64);
+  const unsigned char* const psa = smem + (TM + TN) * 128 + (wm * 16 * MF + r16) * 4;
+  const unsigned char* const psb = smem + (TM + TN) * 128 + (TM + wn * 16 * NF + r16) * 4;
+  const unsigned char *qsa = psa, *qsb = psb;
+  auto frag = [](const unsigned char* lo, const unsigned char* hi) {
+    return __builtin_shufflevector(*reinterpret_cast<const i32x4m*>(lo), *reinterpret_cast<const i32x4m*>(hi), 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  auto read_a = [&](int h, int u) {
+    fa[h][u] = frag(pal + (h * HM + u) * 2048, pah + (h * HM + u) * 2048);
+    ca[h][u] = qsa[(h * HM + u) * 64];
+  };
+  auto read_b = [&](int h, int u) {
+    fb[h][u] = frag(pbl + (h * HN + u) * 2048, pbh + (h * HN + u) * 2048);
+    cb[h][u] = qsb[(h * HN + u) * 64];
+  };
+  // the stage of block kb is the one that is read from here on
+  int shift = STAGE;
+  auto turn = [&](int kb) {
+    pal += shift; pah += shift; pbl += shift; pbh += shift;
+    shift = -shift;
+    qsa = psa + (kb & 1) * STAGE + (kb & 3);
+    qsb = psb + (kb & 1) * STAGE + (kb & 3);
+  };
+  // A quarter's products, columns outermost; after(x) follows product x of HM HN
+  auto quarter = [&](int ha, int hb, auto after) {
     if constexpr (WIDE) {
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        bf16x8 wa[4], wb[4];
+      for (int j = 0; j < HN; ++j) {
+        bf16x8 wb[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          wa[i] = widen<FA>(fa[i][2 * s], fa[i][2 * s + 1], __int_as_float(ca[i] << 23));
-          wb[i] = widen<FB>(fb[i][2 * s], fb[i][2 * s + 1], __int_as_float(cb[i] << 23));
+        for (int s = 0; s < 4; ++s) wb[s] = widen<FB>(fb[hb][j][2 * s], fb[hb][j][2 * s + 1], __int_as_float(cb[hb][j] << 23));
+#pragma unroll
+        for (int i = 0; i < HM; ++i) {
+          f32x4& c = acc[ha * HM + i][hb * HN + j];
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+            mfma_wide(c, wb[s], widen<FA>(fa[ha][i][2 * s], fa[ha][i][2 * s + 1], __int_as_float(ca[ha][i] << 23)));
+          after(j * HM + i);
+          __builtin_amdgcn_sched_barrier(0);
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[j], wa[i], acc[i][j], 0, 0, 0);
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int j = 0; j < HN; ++j) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = mfma_block<FB, FA>(fb[j], fa[i], acc[i][j], cb[j], ca[i]);
+        for (int i = 0; i < HM; ++i) {
+          f32x4& c = acc[ha * HM + i][hb * HN + j];
+          mfma_block<FB, FA>(c, fb[hb][j], fa[ha][i], cb[hb][j], ca[ha][i]);
+          after(j * HM + i);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
     }
+  };
+  constexpr int ND = MF + NF, N1 = HM * HN;
+  if (nkb > 0) {
+#pragma unroll
+    for (int q = 0; q < ND; ++q) dma_at(q, 0, 0);
+    dma_scales_at(0, 0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    {
+      const int kb = nkb > 1 ? 1 : 0;
+#pragma unroll
+      for (int q = 0; q < ND; ++q) dma_at(q, 1, kb);
+      dma_scales_at(1, kb);
+    }
+#pragma unroll
+    for (int u = 0; u < HM; ++u) read_a(0, u);
+#pragma unroll
+    for (int u = 0; u < HN; ++u) read_b(0, u);
+    for (int kb = 0; kb < nkb; ++kb) {
+      // behind the last block the DMA and the reads go on with the last block's data: nobody uses it
+      const int ahead = kb + 2 < nkb ? kb + 2 : nkb - 1;
+      quarter(0, 0, [&](int x) {
+#pragma unroll
+        for (int u = x * HN / N1; u < (x + 1) * HN / N1; ++u) read_b(1, u);
+      });
+      quarter(0, 1, [&](int x) {
+#pragma unroll
+        for (int u = x * HM / N1; u < (x + 1) * HM / N1; ++u) read_a(1, u);
+      });
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+      turn(kb + 1);
+      quarter(1, 1, [&](int x) {
+#pragma unroll
+        for (int u = x * HM / N1; u < (x + 1) * HM / N1; ++u) read_a(0, u);
+#pragma unroll
+        for (int q = x * MF / N1; q < (x + 1) * MF / N1; ++q) dma_at(q, kb, ahead);
+        if (x == N1 - 1) dma_scales_at(kb, ahead);
+      });
+      quarter(1, 0, [&](int x) {
+        if (x % HM == HM - 1) read_b(0, x / HM);
+#pragma unroll
+        for (int q = x * NF / N1; q < (x + 1) * NF / N1; ++q) dma_at(MF + q, kb, ahead);
+      });
+    }
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_nop 15\n\ts_nop 15" ::: "memory");   // no DMA outlives the workgroup
+#pragma unroll
+    for (int i = 0; i < MF; ++i) settle(acc[i]);
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t m = m0 + wm + 16 * i + r16;
+  for (int i = 0; i < MF; ++i) {
+    const int64_t m = m0 + wm * 16 * MF + 16 * i + r16;
     if (m >= p.M) continue;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int64_t n = n0 + wn + 16 * j + 4 * g + q;
-        if (n >= p.N) continue;
-        float v = acc[i][j][q] + (p.bias ? p.bias[n] : 0.f);
-        if (p.out_bf16) {
-          static_cast<u16*>(p.out)[m * p.ldo + n] = f2bf(v);
+    for (int j = 0; j < NF; ++j) {
+      const int64_t n = n0 + wn * 16 * NF + 16 * j + 4 * g;
+      if (n >= p.N) continue;
+      f32x4 v = acc[i][j];
+      if (p.vec) {
+        if (p.bias) v += *reinterpret_cast<const f32x4*>(p.bias + n);
+        if constexpr (!WIDE) {
+          *reinterpret_cast<uint2*>(static_cast<u16*>(p.out) + m * p.ldo + n) =
+              make_uint2((uint32_t)f2bf(v[0]) | ((uint32_t)f2bf(v[1]) << 16), (uint32_t)f2bf(v[2]) | ((uint32_t)f2bf(v[3]) << 16));
         } else {
-          float* o = static_cast<float*>(p.out) + m * p.ldo + n;
-          *o = p.accumulate ? *o + v : v;
+          f32x4* const o = reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + m * p.ldo + n);
+          if (p.accumulate) v += *o;
+          *o = v;
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (n + q >= p.N) break;
+          const float s = v[q] + (p.bias ? p.bias[n + q] : 0.f);
+          if constexpr (!WIDE) {
+            static_cast<u16*>(p.out)[m * p.ldo + n + q] = f2bf(s);
+          } else {
+            float* const o = static_cast<float*>(p.out) + m * p.ldo + n + q;
+            *o = p.accumulate ? *o + s : s;
+          }
         }
       }
     }
   }
+}
+
+// hipFuncAttributeMaxDynamicSharedMemorySize is not needed on this device; a launch may ask for up to 160 KB.
+template <int FB, int FA, bool WIDE, int MF, int NF>
+void launch_tile(MmP p, const char* name, double flops, double bytes, hipStream_t st) {
+  p.tiles_m = (int)cdiv64(p.M, 32 * MF);
+  p.tiles_n = (int)cdiv64(p.N, 32 * NF);
+  p.tiles = p.tiles_m * p.tiles_n;
+  constexpr int lds = 2 * (32 * MF + 32 * NF) * 132;
+  TG_LAUNCH(name, flops, bytes, (fp8_tile_kernel<FB, FA, WIDE, MF, NF>), dim3((unsigned)p.tiles), dim3(256), lds, st, p);
+}
+
+template <int FB, int FA, bool WIDE>
+void launch_formats(const MmP& p, const char* name, double flops, double bytes, hipStream_t st) {
+  const int64_t cus = tg_num_cus();
+  if (cdiv64(p.M, 256) * cdiv64(p.N, 256) * 5 >= cus * 4) launch_tile<FB, FA, WIDE, 8, 8>(p, name, flops, bytes, st);
+  else if (cdiv64(p.M, 128) * cdiv64(p.N, 128) * 5 >= cus * 4) launch_tile<FB, FA, WIDE, 4, 4>(p, name, flops, bytes, st);
+  else launch_tile<FB, FA, WIDE, 2, 2>(p, name, flops, bytes, st);
 }
 
 bool al16m(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -166,7 +322,7 @@ extern "C" int tg_fp8_matmul(const tg_fp8_matmul_desc* d, const void* a, const v
                              const float* bias, void* out, void* stream) {
   TG_CHECK_ARG(d != nullptr, "null descriptor");
   TG_CHECK_ARG(d->M >= 0 && d->N >= 0 && d->M < ((int64_t)1 << 31) && d->N < ((int64_t)1 << 31), "M and N must lie in [0, 2^31)");
-  TG_CHECK_ARG(d->K >= 0 && d->K % 128 == 0 && d->K <= (1 << 24), "K must be a multiple of 128 in [0, 2^24] (rows padded with zeros)");
+  TG_CHECK_ARG(d->K >= 0 && d->K % 128 == 0 && d->K <= (1 << 22), "K must be a multiple of 128 in [0, 2^22] (rows padded with zeros)");
   TG_CHECK_ARG(fmt_ok(d->a_fmt) && fmt_ok(d->b_fmt), "bad 8-bit type");
   TG_CHECK_ARG(d->out_dtype == TG_F32 || d->out_dtype == TG_BF16, "bad output type");
   TG_CHECK_ARG(!d->accumulate || d->out_dtype == TG_F32, "accumulation needs an f32 output");
@@ -187,16 +343,16 @@ extern "C" int tg_fp8_matmul(const tg_fp8_matmul_desc* d, const void* a, const v
   p.accumulate = d->accumulate;
   const char* const name = "fp8_matmul";
   const double flops = 2.0 * d->M * d->N * d->K, bytes = (double)d->M * d->K + (double)d->N * d->K + (double)d->M * d->N * (p.out_bf16 ? 2 : 4);
-  const int64_t blocks = cdiv64(d->M, 128) * cdiv64(d->N, 128);
-  TG_CHECK_ARG(blocks < ((int64_t)1 << 31), "too many output tiles");
-  const dim3 grid((unsigned)blocks), block(256);
+  TG_CHECK_ARG(cdiv64(d->M, 64) * cdiv64(d->N, 64) < ((int64_t)1 << 27), "too many output tiles");
+  const int oe = p.out_bf16 ? 2 : 4;
+  p.vec = d->N % 4 == 0 && ((uintptr_t)out & (4 * oe - 1)) == 0 && d->ldo % 4 == 0 && al16m(bias);
   const int fa = d->a_fmt == TG_FP8_E5M2, fb = d->b_fmt == TG_FP8_E5M2;
-#define MM_PICK(WIDEV)                                                                                                   \
-  do {                                                                                                                   \
-    if (fa && fb) TG_LAUNCH(name, flops, bytes, (fp8_matmul_kernel<1, 1, WIDEV>), grid, block, 0, ST(stream), p);        \
-    else if (fa) TG_LAUNCH(name, flops, bytes, (fp8_matmul_kernel<0, 1, WIDEV>), grid, block, 0, ST(stream), p);         \
-    else if (fb) TG_LAUNCH(name, flops, bytes, (fp8_matmul_kernel<1, 0, WIDEV>), grid, block, 0, ST(stream), p);         \
-    else TG_LAUNCH(name, flops, bytes, (fp8_matmul_kernel<0, 0, WIDEV>), grid, block, 0, ST(stream), p);                 \
+#define MM_PICK(WIDEV)                                                                     \
+  do {                                                                                     \
+    if (fa && fb) launch_formats<1, 1, WIDEV>(p, name, flops, bytes, ST(stream));          \
+    else if (fa) launch_formats<0, 1, WIDEV>(p, name, flops, bytes, ST(stream));           \
+    else if (fb) launch_formats<1, 0, WIDEV>(p, name, flops, bytes, ST(stream));           \
+    else launch_formats<0, 0, WIDEV>(p, name, flops, bytes, ST(stream));                   \
   } while (0)
   if (p.out_bf16) MM_PICK(false);
   else MM_PICK(true);
@@ -212,7 +368,7 @@ int64_t linear_ws(int64_t M, int64_t K) {
 
 extern "C" int tg_fp8_linear_ws(int64_t M, int64_t N, int64_t K, int64_t* bytes) {
   TG_CHECK_ARG(bytes != nullptr, "null pointer");
-  TG_CHECK_ARG(M >= 0 && N >= 0 && K >= 1 && M < ((int64_t)1 << 31) && N < ((int64_t)1 << 31) && K <= (1 << 24), "M, N in [0, 2^31) and K in [1, 2^24] are wanted");
+  TG_CHECK_ARG(M >= 0 && N >= 0 && K >= 1 && M < ((int64_t)1 << 31) && N < ((int64_t)1 << 31) && K <= (1 << 22), "M, N in [0, 2^31) and K in [1, 2^22] are wanted");
   *bytes = linear_ws(M, K);
   return TG_OK;
 }
@@ -220,7 +376,7 @@ extern "C" int tg_fp8_linear_ws(int64_t M, int64_t N, int64_t K, int64_t* bytes)
 extern "C" int tg_fp8_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* w, const void* scale_w, int64_t N,
                              int w_fmt, const float* bias, void* out, int out_dtype, int64_t ldo, void* ws, int64_t ws_bytes,
                              void* stream) {
-  TG_CHECK_ARG(M >= 0 && N >= 0 && K >= 1 && M < ((int64_t)1 << 31) && N < ((int64_t)1 << 31) && K <= (1 << 24), "M, N in [0, 2^31) and K in [1, 2^24] are wanted");
+  TG_CHECK_ARG(M >= 0 && N >= 0 && K >= 1 && M < ((int64_t)1 << 31) && N < ((int64_t)1 << 31) && K <= (1 << 22), "M, N in [0, 2^31) and K in [1, 2^22] are wanted");
   if (M == 0 || N == 0) return TG_OK;
   TG_CHECK_ARG(ws != nullptr && al16m(ws) && ws_bytes >= linear_ws(M, K), "a workspace of tg_fp8_linear_ws() bytes is missing");
   const int64_t kb = cdiv64(K, 128);
