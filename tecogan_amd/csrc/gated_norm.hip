@@ -28,8 +28,8 @@ __device__ __forceinline__ void load8(const T* __restrict__ row, int c, int C, f
         bf8_unpack(*reinterpret_cast<const uint4*>(row + c), f);
       } else {
         const f4v a = *reinterpret_cast<const f4v*>(row + c), b = *reinterpret_cast<const f4v*>(row + c + 4);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) { f[k] = a[k]; f[4 + k] = b[k]; }
+        f[0] = a[0]; f[1] = a[1]; f[2] = a[2]; f[3] = a[3];
+        f[4] = b[0]; f[5] = b[1]; f[6] = b[2]; f[7] = b[3];
       }
     } else {
 #pragma unroll
@@ -40,6 +40,24 @@ __device__ __forceinline__ void load8(const T* __restrict__ row, int c, int C, f
     for (int k = 0; k < 8; ++k) f[k] = c + k < C ? Elem<T>::ld(row + c + k) : 0.f;
   }
 }
+
+// The same 8 values as they lie in memory: what is fetched a row ahead
+template <typename T, bool VEC> struct Raw8 {
+  float f[8];
+  __device__ __forceinline__ void load(const T* __restrict__ row, int c, int C) { load8<T, VEC>(row, c, C, f); }
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = f[k];
+  }
+};
+template <> struct Raw8<u16, true> {
+  uint4 w;
+  __device__ __forceinline__ void load(const u16* __restrict__ row, int c, int C) {
+    w = make_uint4(0, 0, 0, 0);
+    if (c < C) w = *reinterpret_cast<const uint4*>(row + c);
+  }
+  __device__ __forceinline__ void values(float (&v)[8]) const { bf8_unpack(w, v); }
+};
 
 template <typename T, bool VEC>
 __device__ __forceinline__ void store8(T* __restrict__ row, int c, int C, const float (&f)[8]) {
@@ -61,12 +79,26 @@ __device__ __forceinline__ void store8(T* __restrict__ row, int c, int C, const 
 // fp32 parameter vector (nullable): its 8 values, or `other`
 template <bool VEC>
 __device__ __forceinline__ void param8(const float* __restrict__ p, int c, int C, float other, float (&f)[8]) {
+  f4v a = {other, other, other, other}, b = a;
   if (p) {
-    load8<float, VEC>(p, c, C, f);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = other;
+    if constexpr (VEC) {
+      if (c < C) {
+        a = *reinterpret_cast<const f4v*>(p + c);
+        b = *reinterpret_cast<const f4v*>(p + c + 4);
+      }
+    } else {
+      if (c + 0 < C) a[0] = p[c + 0];
+      if (c + 1 < C) a[1] = p[c + 1];
+      if (c + 2 < C) a[2] = p[c + 2];
+      if (c + 3 < C) a[3] = p[c + 3];
+      if (c + 4 < C) b[0] = p[c + 4];
+      if (c + 5 < C) b[1] = p[c + 5];
+      if (c + 6 < C) b[2] = p[c + 6];
+      if (c + 7 < C) b[3] = p[c + 7];
+    }
   }
+  f[0] = a[0]; f[1] = a[1]; f[2] = a[2]; f[3] = a[3];
+  f[4] = b[0]; f[5] = b[1]; f[6] = b[2]; f[7] = b[3];
 }
 
 __device__ __forceinline__ float gate_value(float g, int act) {
@@ -101,15 +133,53 @@ __device__ __forceinline__ float gate_slope(float g, int act, float* value) {
 
 constexpr int GN_MAX_LPR = 512;
 
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float plus_row16(float v) {           // + the other row of 16 lanes
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float plus_half32(float v) {          // + the other half of the wave
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// Sums over the lanes whose numbers differ in the bits from `from` up to below `to` (powers of two up to 64), by lane exchanges inside
+// the vector unit; every lane gets its sum, all lanes of a group the same bits.
+template <int N>
+__device__ __forceinline__ void lane_sums(float (&v)[N], int from, int to) {
+  if (from < 2 && to >= 2) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += dpp<0xB1>(v[i]);         // lane ^ 1
+  }
+  if (from < 4 && to >= 4) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += dpp<0x4E>(v[i]);         // lane ^ 2
+  }
+  if (from < 8 && to >= 8) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += from == 1 ? dpp<0x141>(v[i]) : __shfl_xor(v[i], 4, 64);   // 7 - lane serves where four agree
+  }
+  if (from < 16 && to >= 16) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += dpp<0x128>(v[i]);        // lane ^ 8
+  }
+  if (from < 32 && to >= 32) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = plus_row16(v[i]);
+  }
+  if (from < 64 && to >= 64) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = plus_half32(v[i]);
+  }
+}
+
 // Sums v[0..N) over the lanes of this lane's row.  Rows wider than a wave meet in `red` (two buffers used in turn: a buffer is
 // written again two calls later, behind the other buffer's barrier).
 template <int N>
 __device__ __forceinline__ void row_sums(float (&v)[N], int lpr, float* red, int& turn) {
-  const int w = lpr < 64 ? lpr : 64;
-  for (int o = w >> 1; o > 0; o >>= 1) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o, 64);
-  }
+  lane_sums(v, 1, lpr < 64 ? lpr : 64);
   if (lpr > 64) {
     const int wave = threadIdx.x >> 6, wpr = lpr >> 6, w0 = wave & ~(wpr - 1);
     float* buf = red + turn * (8 * 4);
@@ -141,29 +211,69 @@ struct GnP {
   float inv_c;
 };
 
+// Parameters stay in registers over a workgroup's rows where they fit (one or two vectors a lane), and the next row's tensors are on
+// their way while a row's sums are made.
 template <typename TO, typename TX, int NV, bool VEC>
 __global__ __launch_bounds__(512) void gated_norm_fwd_kernel(GnP p) {
   __shared__ float red[2 * 8 * 4];
+  constexpr bool KEEP = NV <= 2;                                  // wider rows: no registers for the parameters or a second row
   const tg_gated_norm_desc& d = p.d;
   const int lpr = 1 << p.lpr_log2, lane = threadIdx.x & (lpr - 1), sub = threadIdx.x >> p.lpr_log2, rpb = blockDim.x >> p.lpr_log2;
   const int C = d.C;
-  int turn = 0;
-  for (int64_t base = (int64_t)blockIdx.x * rpb; base < d.rows; base += (int64_t)gridDim.x * rpb) {
-    const bool on = base + sub < d.rows;
-    const int64_t row = on ? base + sub : d.rows - 1;
-    const int Cr = on ? C : 0;                                   // a row past the end reads and writes nothing
-    float x[NV][8], u[NV][8], g[NV][8];
+  const bool layer_post = d.post == TG_NORM_LAYER, layer_pre = d.pre == TG_NORM_LAYER;
+  float wpo[NV][8], bpo[NV][8], sc[NV][8], wpr[NV][8], bpr[NV][8];
+  auto params = [&]() {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int c = (v * lpr + lane) * 8;
-      load8<TX, VEC>(static_cast<const TX*>(p.x) + row * d.ldx, c, Cr, x[v]);
-      if (p.o) load8<TO, VEC>(static_cast<const TO*>(p.o) + row * d.ldo, c, Cr, u[v]);
-      if (p.gate) load8<TO, VEC>(static_cast<const TO*>(p.gate) + (d.rows_per_gate == 1 ? row : row / d.rows_per_gate) * d.ldg, c, Cr, g[v]);
+      param8<VEC>(p.w_post, c, C, 1.f, wpo[v]);
+      param8<VEC>(p.b_post, c, C, 0.f, bpo[v]);
+      param8<VEC>(p.scale, c, C, 1.f, sc[v]);
+      param8<VEC>(p.w_pre, c, C, 1.f, wpr[v]);
+      param8<VEC>(p.b_pre, c, C, 0.f, bpr[v]);
     }
+  };
+  Raw8<TX, VEC> rx[NV];
+  Raw8<TO, VEC> ro[NV], rg[NV];
+  auto fetch = [&](int64_t row) {                                 // a row past the end reads nothing
+    const int Cr = row < d.rows ? C : 0;
+    const int64_t r = row < d.rows ? row : 0;
+    const TX* px = static_cast<const TX*>(p.x) + r * d.ldx;
+    const TO* po = static_cast<const TO*>(p.o) + r * d.ldo;
+    const TO* pg = static_cast<const TO*>(p.gate) + (d.rows_per_gate == 1 ? r : r / d.rows_per_gate) * d.ldg;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * lpr + lane) * 8;
+      rx[v].load(px, c, Cr);
+      if (p.o) ro[v].load(po, c, Cr);
+      if (p.gate) rg[v].load(pg, c, Cr);
+    }
+  };
+  int turn = 0;
+  const int64_t step = (int64_t)gridDim.x * rpb;
+  if constexpr (KEEP) {
+    fetch((int64_t)blockIdx.x * rpb + sub);
+    params();
+  }
+  for (int64_t base = (int64_t)blockIdx.x * rpb; base < d.rows; base += step) {
+    const int64_t row = base + sub;
+    const int Cr = row < d.rows ? C : 0;
+    if constexpr (!KEEP) {
+      fetch(row);
+      params();
+    }
+    float x[NV][8], u[NV][8], g[NV][8];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      rx[v].values(x[v]);
+      if (p.o) ro[v].values(u[v]);
+      if (p.gate) rg[v].values(g[v]);
+    }
+    if (KEEP && base + step < d.rows) fetch(row + step);
     if (p.o) {
       if (d.post != TG_NORM_NONE) {
         float mu = 0.f;
-        if (d.post == TG_NORM_LAYER) {
+        if (layer_post) {
           float s[1] = {0.f};
 #pragma unroll
           for (int v = 0; v < NV; ++v)
@@ -185,31 +295,23 @@ __global__ __launch_bounds__(512) void gated_norm_fwd_kernel(GnP p) {
         row_sums(s, lpr, red, turn);
         const float r = rsqrtf(s[0] * p.inv_c + d.eps);
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-          const int c = (v * lpr + lane) * 8;
-          float w[8], b[8];
-          param8<VEC>(p.w_post, c, C, 1.f, w);
-          param8<VEC>(p.b_post, c, C, 0.f, b);
+        for (int v = 0; v < NV; ++v)
 #pragma unroll
-          for (int k = 0; k < 8; ++k) u[v][k] = u[v][k] * r * w[k] + b[k];
-        }
+          for (int k = 0; k < 8; ++k) u[v][k] = u[v][k] * r * wpo[v][k] + bpo[v][k];
       }
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        const int c = (v * lpr + lane) * 8;
-        float sc[8];
-        param8<VEC>(p.scale, c, C, 1.f, sc);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const float a = p.gate ? gate_value(g[v][k], d.gate_act) : 1.f;
-          x[v][k] += d.alpha * sc[k] * a * u[v][k];
+          x[v][k] += d.alpha * sc[v][k] * a * u[v][k];
         }
-        store8<TX, VEC>(static_cast<TX*>(p.out_y) + row * d.ldy, c, Cr, x[v]);
+        store8<TX, VEC>(static_cast<TX*>(p.out_y) + row * d.ldy, (v * lpr + lane) * 8, Cr, x[v]);
       }
     }
     if (d.pre != TG_NORM_NONE) {
       float mu = 0.f;
-      if (d.pre == TG_NORM_LAYER) {
+      if (layer_pre) {
         float s[1] = {0.f};
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
@@ -234,13 +336,9 @@ __global__ __launch_bounds__(512) void gated_norm_fwd_kernel(GnP p) {
       const float r = rsqrtf(s[0] * p.inv_c + d.eps);
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        const int c = (v * lpr + lane) * 8;
-        float w[8], b[8];
-        param8<VEC>(p.w_pre, c, C, 1.f, w);
-        param8<VEC>(p.b_pre, c, C, 0.f, b);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[v][k] = x[v][k] * r * w[k] + b[k];
-        store8<TO, VEC>(static_cast<TO*>(p.out_h) + row * d.ldh, c, Cr, x[v]);
+        for (int k = 0; k < 8; ++k) x[v][k] = x[v][k] * r * wpr[v][k] + bpr[v][k];
+        store8<TO, VEC>(static_cast<TO*>(p.out_h) + row * d.ldh, (v * lpr + lane) * 8, Cr, x[v]);
       }
     }
   }
@@ -268,21 +366,54 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
   end = item < p.items ? (end < d.rows ? end : d.rows) : start;
   const bool layer = d.pre == TG_NORM_LAYER || d.post == TG_NORM_LAYER;
   float acc[5][NV][8] = {}, dga[NV][8] = {};                        // w_post, b_post, scale, w_pre, b_pre; the gate row
+  Raw8<TX, VEC> ry[NV], rdy[NV];
+  Raw8<TO, VEC> rdh[NV], ro[NV], rg[NV];
+  auto fetch = [&](int64_t row) {
+    const int Cr = row < end ? C : 0;
+    const int64_t r = row < end ? row : 0;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * lpr + lane) * 8;
+      ry[v].load(static_cast<const TX*>(p.y) + r * d.ldy, c, Cr);
+      if (p.d_h) rdh[v].load(static_cast<const TO*>(p.d_h) + r * d.ldh, c, Cr);
+      if (p.d_y) rdy[v].load(static_cast<const TX*>(p.d_y) + r * d.ld_dy, c, Cr);
+      if (p.o) ro[v].load(static_cast<const TO*>(p.o) + r * d.ldo, c, Cr);
+      if (p.gate) rg[v].load(static_cast<const TO*>(p.gate) + (d.rows_per_gate == 1 ? r : r / d.rows_per_gate) * d.ldg, c, Cr);
+    }
+  };
+  float wpre[NV][8], wpost[NV][8], bpost[NV][8], sc[NV][8];
+  auto params = [&]() {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * lpr + lane) * 8;
+      param8<VEC>(p.w_pre, c, C, 1.f, wpre[v]);
+      param8<VEC>(p.w_post, c, C, 1.f, wpost[v]);
+      param8<VEC>(p.b_post, c, C, 0.f, bpost[v]);
+      param8<VEC>(p.scale, c, C, 1.f, sc[v]);
+    }
+  };
   int turn = 0;
+  if constexpr (NV == 1) {                                          // wider rows: no registers for the parameters or a second row
+    fetch(start);
+    params();
+  }
   for (int j = 0; j < p.item_rows; ++j) {
     const bool on = start + j < end;
     const int64_t row = on ? start + j : 0;
     const int Cr = on ? C : 0;
     const int64_t grow = d.rows_per_gate == 1 ? row : row / d.rows_per_gate;
+    if constexpr (NV > 1) {
+      fetch(start + j);
+      params();
+    }
     float y[NV][8], o[NV][8], g[NV][8], dh[NV][8], G[NV][8];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = (v * lpr + lane) * 8;
-      load8<TX, VEC>(static_cast<const TX*>(p.y) + row * d.ldy, c, Cr, y[v]);
-      if (p.d_h) load8<TO, VEC>(static_cast<const TO*>(p.d_h) + row * d.ldh, c, Cr, dh[v]);
-      if (p.d_y) load8<TX, VEC>(static_cast<const TX*>(p.d_y) + row * d.ld_dy, c, Cr, G[v]);
-      if (p.o) load8<TO, VEC>(static_cast<const TO*>(p.o) + row * d.ldo, c, Cr, o[v]);
-      if (p.gate) load8<TO, VEC>(static_cast<const TO*>(p.gate) + grow * d.ldg, c, Cr, g[v]);
+      ry[v].values(y[v]);
+      rdh[v].values(dh[v]);
+      rdy[v].values(G[v]);
+      ro[v].values(o[v]);
+      rg[v].values(g[v]);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         if (!p.d_h) dh[v][k] = 0.f;
@@ -290,6 +421,7 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
         if (!p.o) o[v][k] = 0.f;
       }
     }
+    if (NV == 1 && j + 1 < p.item_rows) fetch(start + j + 1);
     float mu_y = 0.f, mu_o = 0.f;
     if (layer) {
       float s[2] = {0.f, 0.f};
@@ -305,14 +437,12 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int c = (v * lpr + lane) * 8;
-      float w[8];
-      param8<VEC>(p.w_pre, c, C, 1.f, w);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const bool in = c + k < Cr;
         y[v][k] = in ? y[v][k] - mu_y : 0.f;
         if (d.post != TG_NORM_NONE) o[v][k] = in ? o[v][k] - mu_o : 0.f;
-        const float t = dh[v][k] * w[k];
+        const float t = dh[v][k] * wpre[v][k];
         s[0] += y[v][k] * y[v][k];
         s[1] += t * y[v][k];
         s[2] += t;
@@ -326,11 +456,6 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int c = (v * lpr + lane) * 8;
-      float wpre[8], wpost[8], bpost[8], sc[8];
-      param8<VEC>(p.w_pre, c, C, 1.f, wpre);
-      param8<VEC>(p.w_post, c, C, 1.f, wpost);
-      param8<VEC>(p.b_post, c, C, 0.f, bpost);
-      param8<VEC>(p.scale, c, C, 1.f, sc);
       float dg[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -338,7 +463,7 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
           const float n = y[v][k] * r_y;
           acc[3][v][k] += dh[v][k] * n;
           acc[4][v][k] += dh[v][k];
-          if (p.d_h) G[v][k] += r_y * (dh[v][k] * wpre[k] - n * m1 - m2);
+          if (p.d_h) G[v][k] += r_y * (dh[v][k] * wpre[v][k] - n * m1 - m2);
         }
       }
       if (p.d_x) store8<TX, VEC>(static_cast<TX*>(p.d_x) + row * d.ldx, c, Cr, G[v]);
@@ -346,17 +471,17 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const float n = o[v][k] * r_o;
-          const float u = d.post != TG_NORM_NONE ? n * wpost[k] + bpost[k] : o[v][k];
+          const float u = d.post != TG_NORM_NONE ? n * wpost[v][k] + bpost[v][k] : o[v][k];
           float a = 1.f, da = 0.f;
           if (p.gate) da = gate_slope(g[v][k], d.gate_act, &a);
           const float D = c + k < Cr ? d.alpha * G[v][k] : 0.f;
           acc[2][v][k] += D * a * u;
-          dg[k] = D * sc[k] * u * da;
-          const float du = D * sc[k] * a;
+          dg[k] = D * sc[v][k] * u * da;
+          const float du = D * sc[v][k] * a;
           acc[0][v][k] += du * n;
           acc[1][v][k] += du;
           o[v][k] = n;
-          G[v][k] = du * wpost[k];
+          G[v][k] = du * wpost[v][k];
           q[0] += G[v][k] * n;
           q[1] += G[v][k];
         }
@@ -398,6 +523,7 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) store8<float, VEC>(p.gate_part + item * C, (v * lpr + lane) * 8, C, dga[v]);
   }
+  // the workgroup's parameter sums: over the rows of a wave by lane exchange, then over the waves through LDS
 #pragma unroll
   for (int q = 0; q < 5; ++q) {
     if (!(p.want >> q & 1)) continue;
@@ -406,17 +532,20 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
     for (int v = 0; v < NV; ++v) {
       const int c = (v * lpr + lane) * 8;
       if (rpb > 1) {                                                // NV == 1 here: several rows only where a row is narrow
+        if (lpr < 64) lane_sums(acc[q][v], lpr, 64);
+        const int held = lpr < 64 ? blockDim.x >> 6 : rpb;          // sums left per column
+        const bool mine = lpr < 64 ? (threadIdx.x & 63) < lpr : true;
+        const int slot = lpr < 64 ? threadIdx.x >> 6 : sub;
         __syncthreads();
+        if (mine) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) join[(sub * lpr + lane) * 8 + k] = acc[q][v][k];
+          for (int k = 0; k < 8; ++k) join[(slot * lpr + lane) * 8 + k] = acc[q][v][k];
+        }
         __syncthreads();
-        if (sub == 0) {
-          float t[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-          for (int s = 0; s < rpb; ++s) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) t[k] += join[(s * lpr + lane) * 8 + k];
-          }
-          store8<float, VEC>(out, c, C, t);
+        for (int e = threadIdx.x; e < lpr * 8 && e < C; e += blockDim.x) {
+          float t = 0.f;
+          for (int s = 0; s < held; ++s) t += join[s * lpr * 8 + e];
+          out[e] = t;
         }
       } else {
         store8<float, VEC>(out, c, C, acc[q][v]);
@@ -468,22 +597,22 @@ struct Geo {
   int64_t items;
 };
 
-void row_geometry(int C, Geo* g) {
+void row_geometry(int C, int block, Geo* g) {
   const int oct = (C + 7) / 8;
   int l = 0;
   while ((1 << l) < oct && (1 << l) < GN_MAX_LPR) ++l;
   g->lpr_log2 = l;
   g->lpr = 1 << l;
   g->nv = oct <= g->lpr ? 1 : (oct <= 2 * g->lpr ? 2 : 4);
-  g->block = g->lpr < 256 ? 256 : g->lpr;
+  g->block = g->lpr < block ? block : g->lpr;
   g->rpb = g->block / g->lpr;
 }
 
-// The backward pass's split of the rows.  About 512 workgroups (two per compute unit), at least 4 rows per sub-row: every workgroup
-// writes 5 C partial values, a row of the operands is 5 - 8 times C values.
+// The backward pass's split of the rows: workgroups of 512 lanes, about one per compute unit (their registers leave room for one or
+// two), at least 4 rows per sub-row: every workgroup writes up to 5 C partial values, a row of the operands is 5 - 8 times C values.
 void item_geometry(int64_t rows, int C, int64_t k, Geo* g) {
-  row_geometry(C, g);
-  int64_t m = cdiv64(rows, (int64_t)512 * g->rpb);
+  row_geometry(C, 512, g);
+  int64_t m = cdiv64(rows, (int64_t)256 * g->rpb);
   if (m < 4) m = 4;
   g->pieces = 0;
   if (k > 1 && k <= m) {
@@ -549,7 +678,7 @@ extern "C" int tg_gated_norm_forward(const tg_gated_norm_desc* d, const void* x,
   const int C = d->C;
   TG_CHECK_ARG(d->ldx >= C && (!o || (d->ldo >= C && d->ldy >= C)) && (!gate || d->ldg >= C) && (!h || d->ldh >= C), "a row stride below C");
   Geo g;
-  row_geometry(C, &g);
+  row_geometry(C, 256, &g);
   GnP p = {};
   p.d = *d;
   p.x = x; p.o = o; p.gate = gate;
@@ -563,7 +692,8 @@ extern "C" int tg_gated_norm_forward(const tg_gated_norm_desc* d, const void* x,
   const char* const name = "gated_norm_fwd";
   const double n = (double)d->rows * C, flops = 14 * n, ex = d->res_dtype == TG_F32 ? 4 : 2, eo = d->dtype == TG_F32 ? 4 : 2;
   const double bytes = n * (ex + (o ? ex + eo : 0) + (gate && d->rows_per_gate == 1 ? eo : 0) + (h ? eo : 0));
-  const dim3 grid((unsigned)(cdiv64(d->rows, g.rpb) < 4096 ? cdiv64(d->rows, g.rpb) : 4096)), block(g.block);
+  const int64_t resident = (int64_t)tg_num_cus() * (1024 / g.block);  // workgroups that stay on the device and walk over the rows
+  const dim3 grid((unsigned)(cdiv64(d->rows, g.rpb) < resident ? cdiv64(d->rows, g.rpb) : resident)), block(g.block);
   if (vec) GN_PICK(gated_norm_fwd_kernel, true, grid, block, 0, ST(stream), p);
   else GN_PICK(gated_norm_fwd_kernel, false, grid, block, 0, ST(stream), p);
   TG_CHECK_LAUNCH();
