@@ -101,34 +101,64 @@ __device__ __forceinline__ void param8(const float* __restrict__ p, int c, int C
   f[4] = b[0]; f[5] = b[1]; f[6] = b[2]; f[7] = b[3];
 }
 
+// sigmoid(v) and sigmoid(-v) without a difference: e = exp(-|v|), 1 / (1 + e) and e / (1 + e)
+__device__ __forceinline__ void sigmoids(float v, float& up, float& down) {
+  const float e = __expf(-fabsf(v)), r = __builtin_amdgcn_rcpf(1.f + e), q = e * r;
+  up = v >= 0.f ? r : (v != v ? v : q);
+  down = v >= 0.f ? q : r;
+}
+// tanh(v) = sign(v) (1 - e) / (1 + e) with e = exp(-2 |v|); below 0.3, where 1 - e cancels, its power series to v^9 (the next term is
+// 9e-3 v^10 = 5e-8 of the value)
+__device__ __forceinline__ float tanh_of(float v, float e, float r) {
+  const float s = v * v;
+  const float small = v + v * s * (-0.333333333f + s * (0.133333333f + s * (-0.0539682540f + s * 0.0218694885f)));
+  return fabsf(v) < 0.3f ? small : copysignf((1.f - e) * r, v);
+}
 __device__ __forceinline__ float gate_value(float g, int act) {
   switch (act) {
-    case TG_ACT_SIGMOID: return 1.f / (1.f + __expf(-g));
-    case TG_ACT_TANH: return tanhf(g);
-    case TG_ACT_SILU: return g / (1.f + __expf(-g));
+    case TG_ACT_SIGMOID:
+    case TG_ACT_SILU: {
+      float up, down;
+      sigmoids(g, up, down);
+      return act == TG_ACT_SILU ? g * up : up;
+    }
+    case TG_ACT_TANH: {
+      const float e = __expf(-2.f * fabsf(g));
+      return tanh_of(g, e, __builtin_amdgcn_rcpf(1.f + e));
+    }
     default: return g;
   }
 }
 // value and derivative
 __device__ __forceinline__ float gate_slope(float g, int act, float* value) {
   switch (act) {
-    case TG_ACT_SIGMOID: {
-      const float p = 1.f / (1.f + __expf(-g));
-      *value = p;
-      return p * (1.f - p);
+    case TG_ACT_SIGMOID:
+    case TG_ACT_SILU: {
+      float up, down;
+      sigmoids(g, up, down);
+      *value = act == TG_ACT_SILU ? g * up : up;
+      return act == TG_ACT_SILU ? up + g * up * down : up * down;
     }
     case TG_ACT_TANH: {
-      const float t = tanhf(g);
-      *value = t;
-      return 1.f - t * t;
-    }
-    case TG_ACT_SILU: {
-      const float p = 1.f / (1.f + __expf(-g));
-      *value = g * p;
-      return p * (1.f + g * (1.f - p));
+      const float e = __expf(-2.f * fabsf(g)), r = __builtin_amdgcn_rcpf(1.f + e);
+      *value = tanh_of(g, e, r);
+      return 4.f * e * r * r;                                       // 1 - tanh^2
     }
     default: *value = g; return 1.f;
   }
+}
+
+// row / rows_per_gate by a multiplication: n < 2^31, q = (mulhi(n, magic) + n) >> shift
+struct Divide {
+  uint32_t magic;
+  int shift;
+  __device__ __forceinline__ uint32_t of(uint32_t n) const { return shift == 0 ? n : (__umulhi(n, magic) + n) >> shift; }
+};
+Divide divide_by(uint32_t d) {
+  Divide r = {0, 0};
+  while (r.shift < 32 && ((uint64_t)1 << r.shift) < d) ++r.shift;
+  r.magic = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << r.shift) - d)) / d + 1);
+  return r;
 }
 
 constexpr int GN_MAX_LPR = 512;
@@ -204,6 +234,7 @@ struct GnP {
   const float *w_post, *b_post, *scale, *w_pre, *b_pre;
   void *out_y, *out_h, *d_x, *d_o, *d_gate;
   float *part, *gate_part;                   // [blocks][5][C], [items][C]
+  Divide gate_of;
   int lpr_log2;
   int item_rows, pieces;                     // rows of an item; > 0: pieces of a gate row's rows (an item is one piece)
   int64_t items;
@@ -240,7 +271,7 @@ __global__ __launch_bounds__(512) void gated_norm_fwd_kernel(GnP p) {
     const int64_t r = row < d.rows ? row : 0;
     const TX* px = static_cast<const TX*>(p.x) + r * d.ldx;
     const TO* po = static_cast<const TO*>(p.o) + r * d.ldo;
-    const TO* pg = static_cast<const TO*>(p.gate) + (d.rows_per_gate == 1 ? r : r / d.rows_per_gate) * d.ldg;
+    const TO* pg = static_cast<const TO*>(p.gate) + (int64_t)p.gate_of.of((uint32_t)r) * d.ldg;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int c = (v * lpr + lane) * 8;
@@ -286,9 +317,10 @@ __global__ __launch_bounds__(512) void gated_norm_fwd_kernel(GnP p) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
           const int c = (v * lpr + lane) * 8;
+          const float mv = c < Cr ? mu : 0.f;                       // values past the end are 0 and stay 0
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            u[v][k] = c + k < Cr ? u[v][k] - mu : 0.f;
+            u[v][k] -= VEC || c + k < Cr ? mv : 0.f;
             s[0] += u[v][k] * u[v][k];
           }
         }
@@ -317,7 +349,7 @@ __global__ __launch_bounds__(512) void gated_norm_fwd_kernel(GnP p) {
         for (int v = 0; v < NV; ++v) {
           const int c = (v * lpr + lane) * 8;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) s[0] += c + k < Cr ? x[v][k] : 0.f;
+          for (int k = 0; k < 8; ++k) s[0] += (VEC ? c < Cr : c + k < Cr) ? x[v][k] : 0.f;
         }
         row_sums(s, lpr, red, turn);
         mu = s[0] * p.inv_c;
@@ -326,9 +358,10 @@ __global__ __launch_bounds__(512) void gated_norm_fwd_kernel(GnP p) {
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         const int c = (v * lpr + lane) * 8;
+        const bool in = c < Cr;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          x[v][k] = c + k < Cr ? x[v][k] - mu : 0.f;
+          x[v][k] = (VEC ? in : c + k < Cr) ? x[v][k] - mu : 0.f;
           s[0] += x[v][k] * x[v][k];
         }
       }
@@ -378,9 +411,15 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
       if (p.d_h) rdh[v].load(static_cast<const TO*>(p.d_h) + r * d.ldh, c, Cr);
       if (p.d_y) rdy[v].load(static_cast<const TX*>(p.d_y) + r * d.ld_dy, c, Cr);
       if (p.o) ro[v].load(static_cast<const TO*>(p.o) + r * d.ldo, c, Cr);
-      if (p.gate) rg[v].load(static_cast<const TO*>(p.gate) + (d.rows_per_gate == 1 ? r : r / d.rows_per_gate) * d.ldg, c, Cr);
+      if (p.gate) rg[v].load(static_cast<const TO*>(p.gate) + (int64_t)p.gate_of.of((uint32_t)r) * d.ldg, c, Cr);
     }
   };
+  float ga[NV][8], gs[NV][8];                                       // the gate's activation and its derivative
+  int64_t gate_row = 0;
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) { ga[v][k] = 1.f; gs[v][k] = 0.f; }
   float wpre[NV][8], wpost[NV][8], bpost[NV][8], sc[NV][8];
   auto params = [&]() {
 #pragma unroll
@@ -401,24 +440,33 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
     const bool on = start + j < end;
     const int64_t row = on ? start + j : 0;
     const int Cr = on ? C : 0;
-    const int64_t grow = d.rows_per_gate == 1 ? row : row / d.rows_per_gate;
+    const int64_t grow = p.gate_of.of((uint32_t)row);
     if constexpr (NV > 1) {
       fetch(start + j);
       params();
     }
-    float y[NV][8], o[NV][8], g[NV][8], dh[NV][8], G[NV][8];
+    float y[NV][8], o[NV][8], dh[NV][8], G[NV][8];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       ry[v].values(y[v]);
       rdh[v].values(dh[v]);
       rdy[v].values(G[v]);
       ro[v].values(o[v]);
-      rg[v].values(g[v]);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         if (!p.d_h) dh[v][k] = 0.f;
         if (!p.d_y) G[v][k] = 0.f;
         if (!p.o) o[v][k] = 0.f;
+      }
+    }
+    if (p.gate && (j == 0 || grow != gate_row)) {                   // a shared gate row: its activation once
+      gate_row = grow;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        float g[8];
+        rg[v].values(g);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) gs[v][k] = gate_slope(g[k], d.gate_act, &ga[v][k]);
       }
     }
     if (NV == 1 && j + 1 < p.item_rows) fetch(start + j + 1);
@@ -437,11 +485,11 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int c = (v * lpr + lane) * 8;
+      const float my = c < Cr ? mu_y : 0.f, mo = c < Cr ? mu_o : 0.f;   // values past the end are 0 and stay 0
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const bool in = c + k < Cr;
-        y[v][k] = in ? y[v][k] - mu_y : 0.f;
-        if (d.post != TG_NORM_NONE) o[v][k] = in ? o[v][k] - mu_o : 0.f;
+        y[v][k] -= VEC || c + k < Cr ? my : 0.f;
+        o[v][k] -= VEC || c + k < Cr ? mo : 0.f;
         const float t = dh[v][k] * wpre[v][k];
         s[0] += y[v][k] * y[v][k];
         s[1] += t * y[v][k];
@@ -457,13 +505,14 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
     for (int v = 0; v < NV; ++v) {
       const int c = (v * lpr + lane) * 8;
       float dg[8];
+      const float mp = c < Cr ? m2 : 0.f;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         if (d.pre != TG_NORM_NONE) {
           const float n = y[v][k] * r_y;
           acc[3][v][k] += dh[v][k] * n;
           acc[4][v][k] += dh[v][k];
-          if (p.d_h) G[v][k] += r_y * (dh[v][k] * wpre[v][k] - n * m1 - m2);
+          G[v][k] += r_y * (dh[v][k] * wpre[v][k] - n * m1 - (VEC || c + k < Cr ? mp : 0.f));
         }
       }
       if (p.d_x) store8<TX, VEC>(static_cast<TX*>(p.d_x) + row * d.ldx, c, Cr, G[v]);
@@ -472,11 +521,9 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
         for (int k = 0; k < 8; ++k) {
           const float n = o[v][k] * r_o;
           const float u = d.post != TG_NORM_NONE ? n * wpost[v][k] + bpost[v][k] : o[v][k];
-          float a = 1.f, da = 0.f;
-          if (p.gate) da = gate_slope(g[v][k], d.gate_act, &a);
-          const float D = c + k < Cr ? d.alpha * G[v][k] : 0.f;
+          const float a = ga[v][k], D = d.alpha * G[v][k];
           acc[2][v][k] += D * a * u;
-          dg[k] = D * sc[v][k] * u * da;
+          dg[k] = D * sc[v][k] * u * gs[v][k];
           const float du = D * sc[v][k] * a;
           acc[0][v][k] += du * n;
           acc[1][v][k] += du;
@@ -490,7 +537,7 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
             store8<TO, VEC>(static_cast<TO*>(p.d_gate) + row * d.ld_dg, c, Cr, dg);
           } else {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) dga[v][k] += on ? dg[k] : 0.f;
+            for (int k = 0; k < 8; ++k) dga[v][k] += dg[k];
           }
         }
       }
@@ -686,6 +733,7 @@ extern "C" int tg_gated_norm_forward(const tg_gated_norm_desc* d, const void* x,
   p.out_y = y; p.out_h = h;
   p.lpr_log2 = g.lpr_log2;
   p.inv_c = 1.f / (float)C;
+  p.gate_of = divide_by((uint32_t)d->rows_per_gate);
   const bool vec = C % 8 == 0 && al16(x) && al16(o) && al16(gate) && al16(y) && al16(h) && al16(w_post) && al16(b_post) && al16(scale) &&
                    al16(w_pre) && al16(b_pre) && d->ldx % 8 == 0 && (!o || (d->ldo % 8 == 0 && d->ldy % 8 == 0)) &&
                    (!gate || d->ldg % 8 == 0) && (!h || d->ldh % 8 == 0);
@@ -744,6 +792,7 @@ extern "C" int tg_gated_norm_backward(const tg_gated_norm_desc* d, const void* d
     p.item_rows = g.item_rows; p.pieces = g.pieces; p.items = g.items;
     p.want = want;
     p.inv_c = 1.f / (float)C;
+  p.gate_of = divide_by((uint32_t)d->rows_per_gate);
     const bool vec = C % 8 == 0 && al16(d_y) && al16(d_h) && al16(y) && al16(o) && al16(gate) && al16(w_post) && al16(b_post) &&
                      al16(scale) && al16(w_pre) && al16(d_x) && al16(d_o) && al16(d_gate) && (!d_y || d->ld_dy % 8 == 0) &&
                      (!d_h || d->ldh % 8 == 0) && d->ldy % 8 == 0 && (!o || d->ldo % 8 == 0) && (!gate || d->ldg % 8 == 0) &&
