@@ -114,37 +114,47 @@ __device__ __forceinline__ float tanh_of(float v, float e, float r) {
   const float small = v + v * s * (-0.333333333f + s * (0.133333333f + s * (-0.0539682540f + s * 0.0218694885f)));
   return fabsf(v) < 0.3f ? small : copysignf((1.f - e) * r, v);
 }
-__device__ __forceinline__ float gate_value(float g, int act) {
-  switch (act) {
-    case TG_ACT_SIGMOID:
-    case TG_ACT_SILU: {
-      float up, down;
-      sigmoids(g, up, down);
-      return act == TG_ACT_SILU ? g * up : up;
+// g = act(g), one choice for the eight
+__device__ __forceinline__ void gate_values(float (&g)[8], int act) {
+  if (act == TG_ACT_SIGMOID || act == TG_ACT_SILU) {
+    const bool silu = act == TG_ACT_SILU;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float up = __builtin_amdgcn_rcpf(1.f + __expf(-g[k]));
+      g[k] = silu ? g[k] * up : up;
     }
-    case TG_ACT_TANH: {
-      const float e = __expf(-2.f * fabsf(g));
-      return tanh_of(g, e, __builtin_amdgcn_rcpf(1.f + e));
+  } else if (act == TG_ACT_TANH) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float e = __expf(-2.f * fabsf(g[k]));
+      g[k] = tanh_of(g[k], e, __builtin_amdgcn_rcpf(1.f + e));
     }
-    default: return g;
   }
 }
-// value and derivative
-__device__ __forceinline__ float gate_slope(float g, int act, float* value) {
-  switch (act) {
-    case TG_ACT_SIGMOID:
-    case TG_ACT_SILU: {
+// value = act(g), slope = act'(g)
+__device__ __forceinline__ void gate_slopes(const float (&g)[8], int act, float (&value)[8], float (&slope)[8]) {
+  if (act == TG_ACT_SIGMOID || act == TG_ACT_SILU) {
+    const bool silu = act == TG_ACT_SILU;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
       float up, down;
-      sigmoids(g, up, down);
-      *value = act == TG_ACT_SILU ? g * up : up;
-      return act == TG_ACT_SILU ? up + g * up * down : up * down;
+      sigmoids(g[k], up, down);
+      value[k] = silu ? g[k] * up : up;
+      slope[k] = silu ? up + g[k] * up * down : up * down;
     }
-    case TG_ACT_TANH: {
-      const float e = __expf(-2.f * fabsf(g)), r = __builtin_amdgcn_rcpf(1.f + e);
-      *value = tanh_of(g, e, r);
-      return 4.f * e * r * r;                                       // 1 - tanh^2
+  } else if (act == TG_ACT_TANH) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float e = __expf(-2.f * fabsf(g[k])), r = __builtin_amdgcn_rcpf(1.f + e);
+      value[k] = tanh_of(g[k], e, r);
+      slope[k] = 4.f * e * r * r;                                   // 1 - tanh^2
     }
-    default: *value = g; return 1.f;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      value[k] = g[k];
+      slope[k] = 1.f;
+    }
   }
 }
 
@@ -209,20 +219,34 @@ __device__ __forceinline__ void lane_sums(float (&v)[N], int from, int to) {
 // written again two calls later, behind the other buffer's barrier).
 template <int N>
 __device__ __forceinline__ void row_sums(float (&v)[N], int lpr, float* red, int& turn) {
-  lane_sums(v, 1, lpr < 64 ? lpr : 64);
+  if (lpr < 64) {
+    lane_sums(v, 1, lpr);
+    return;
+  }
+  lane_sums(v, 1, 64);                                           // constant bounds: six steps without branches
   if (lpr > 64) {
-    const int wave = threadIdx.x >> 6, wpr = lpr >> 6, w0 = wave & ~(wpr - 1);
-    float* buf = red + turn * (8 * 4);
+    const int wave = threadIdx.x >> 6, w0 = wave & ~((lpr >> 6) - 1);
+    float* buf = red + turn * (8 * 4);                           // [value][wave]
     if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) buf[wave * 4 + i] = v[i];
+      for (int i = 0; i < N; ++i) buf[i * 8 + wave] = v[i];
     }
     __syncthreads();
+    if (lpr == 512) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      float s = 0.f;
-      for (int k = 0; k < wpr; ++k) s += buf[(w0 + k) * 4 + i];
-      v[i] = s;
+      for (int i = 0; i < N; ++i) {
+        const f4v a = *reinterpret_cast<const f4v*>(buf + i * 8), b = *reinterpret_cast<const f4v*>(buf + i * 8 + 4);
+        v[i] = ((a[0] + a[1]) + (a[2] + a[3])) + ((b[0] + b[1]) + (b[2] + b[3]));
+      }
+    } else if (lpr == 256) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const f4v a = *reinterpret_cast<const f4v*>(buf + i * 8 + w0);
+        v[i] = (a[0] + a[1]) + (a[2] + a[3]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = buf[i * 8 + w0] + buf[i * 8 + w0 + 1];
     }
     turn ^= 1;
   }
@@ -242,52 +266,62 @@ struct GnP {
   float inv_c;
 };
 
+// MODE: what there is beside x -- 0 nothing, 1 a block's output, 2 that and a gate, 3 asked at run time (the rarer shapes).  A norm
+// that is not wanted is one with mean 0 and deviation 1: no branches around the values.
 // Parameters stay in registers over a workgroup's rows where they fit (one or two vectors a lane), and the next row's tensors are on
 // their way while a row's sums are made.
-template <typename TO, typename TX, int NV, bool VEC>
+template <typename TO, typename TX, int NV, bool VEC, int MODE>
 __global__ __launch_bounds__(512) void gated_norm_fwd_kernel(GnP p) {
-  __shared__ float red[2 * 8 * 4];
+  __shared__ __attribute__((aligned(16))) float red[2 * 8 * 4];
   constexpr bool KEEP = NV <= 2;                                  // wider rows: no registers for the parameters or a second row
+  const bool HO = MODE == 3 ? p.o != nullptr : MODE >= 1, HG = MODE == 3 ? p.gate != nullptr : MODE == 2;
   const tg_gated_norm_desc& d = p.d;
   const int lpr = 1 << p.lpr_log2, lane = threadIdx.x & (lpr - 1), sub = threadIdx.x >> p.lpr_log2, rpb = blockDim.x >> p.lpr_log2;
   const int C = d.C;
-  const bool layer_post = d.post == TG_NORM_LAYER, layer_pre = d.pre == TG_NORM_LAYER;
   float wpo[NV][8], bpo[NV][8], sc[NV][8], wpr[NV][8], bpr[NV][8];
   auto params = [&]() {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int c = (v * lpr + lane) * 8;
-      param8<VEC>(p.w_post, c, C, 1.f, wpo[v]);
-      param8<VEC>(p.b_post, c, C, 0.f, bpo[v]);
-      param8<VEC>(p.scale, c, C, 1.f, sc[v]);
+      if (HO) {
+        param8<VEC>(p.w_post, c, C, 1.f, wpo[v]);
+        param8<VEC>(p.b_post, c, C, 0.f, bpo[v]);
+        param8<VEC>(p.scale, c, C, 1.f, sc[v]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sc[v][k] *= d.alpha;
+      }
       param8<VEC>(p.w_pre, c, C, 1.f, wpr[v]);
       param8<VEC>(p.b_pre, c, C, 0.f, bpr[v]);
     }
   };
+  const int64_t row0 = (int64_t)blockIdx.x * rpb + sub, step = (int64_t)gridDim.x * rpb;
+  const TX* px = static_cast<const TX*>(p.x) + row0 * d.ldx;      // the row that is fetched next
+  const TO* po = static_cast<const TO*>(p.o) + row0 * d.ldo;
+  TX* py = static_cast<TX*>(p.out_y) + row0 * d.ldy;              // the row that is written next
+  TO* ph = static_cast<TO*>(p.out_h) + row0 * d.ldh;
+  const int64_t sx = step * d.ldx, so = step * d.ldo, sy = step * d.ldy, sh = step * d.ldh;
   Raw8<TX, VEC> rx[NV];
   Raw8<TO, VEC> ro[NV], rg[NV];
   auto fetch = [&](int64_t row) {                                 // a row past the end reads nothing
     const int Cr = row < d.rows ? C : 0;
-    const int64_t r = row < d.rows ? row : 0;
-    const TX* px = static_cast<const TX*>(p.x) + r * d.ldx;
-    const TO* po = static_cast<const TO*>(p.o) + r * d.ldo;
-    const TO* pg = static_cast<const TO*>(p.gate) + (int64_t)p.gate_of.of((uint32_t)r) * d.ldg;
+    const TO* pg = static_cast<const TO*>(p.gate) + (int64_t)p.gate_of.of((uint32_t)row) * d.ldg;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int c = (v * lpr + lane) * 8;
       rx[v].load(px, c, Cr);
-      if (p.o) ro[v].load(po, c, Cr);
-      if (p.gate) rg[v].load(pg, c, Cr);
+      if (HO) ro[v].load(po, c, Cr);
+      if (HG) rg[v].load(pg, c, Cr);
     }
+    px += sx;
+    po += so;
   };
   int turn = 0;
-  const int64_t step = (int64_t)gridDim.x * rpb;
+  int64_t row = row0;
   if constexpr (KEEP) {
-    fetch((int64_t)blockIdx.x * rpb + sub);
+    fetch(row);
     params();
   }
-  for (int64_t base = (int64_t)blockIdx.x * rpb; base < d.rows; base += step) {
-    const int64_t row = base + sub;
+  for (int64_t base = (int64_t)blockIdx.x * rpb; base < d.rows; base += step, row += step, py += sy, ph += sh) {
     const int Cr = row < d.rows ? C : 0;
     if constexpr (!KEEP) {
       fetch(row);
@@ -297,22 +331,22 @@ __global__ __launch_bounds__(512) void gated_norm_fwd_kernel(GnP p) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       rx[v].values(x[v]);
-      if (p.o) ro[v].values(u[v]);
-      if (p.gate) rg[v].values(g[v]);
+      if (HO) ro[v].values(u[v]);
+      if (HG) rg[v].values(g[v]);
     }
     if (KEEP && base + step < d.rows) fetch(row + step);
-    if (p.o) {
+    if (HO) {
+      float mu = 0.f, r = 1.f;
+      if (d.post == TG_NORM_LAYER) {
+        float s[1] = {0.f};
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) s[0] += u[v][k];
+        row_sums(s, lpr, red, turn);
+        mu = s[0] * p.inv_c;
+      }
       if (d.post != TG_NORM_NONE) {
-        float mu = 0.f;
-        if (layer_post) {
-          float s[1] = {0.f};
-#pragma unroll
-          for (int v = 0; v < NV; ++v)
-#pragma unroll
-            for (int k = 0; k < 8; ++k) s[0] += u[v][k];
-          row_sums(s, lpr, red, turn);
-          mu = s[0] * p.inv_c;
-        }
         float s[1] = {0.f};
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
@@ -320,36 +354,36 @@ __global__ __launch_bounds__(512) void gated_norm_fwd_kernel(GnP p) {
           const float mv = c < Cr ? mu : 0.f;                       // values past the end are 0 and stay 0
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            u[v][k] -= VEC || c + k < Cr ? mv : 0.f;
-            s[0] += u[v][k] * u[v][k];
+            const float t = u[v][k] - (VEC || c + k < Cr ? mv : 0.f);
+            s[0] += t * t;
           }
         }
         row_sums(s, lpr, red, turn);
-        const float r = rsqrtf(s[0] * p.inv_c + d.eps);
-#pragma unroll
-        for (int v = 0; v < NV; ++v)
-#pragma unroll
-          for (int k = 0; k < 8; ++k) u[v][k] = u[v][k] * r * wpo[v][k] + bpo[v][k];
+        r = rsqrtf(s[0] * p.inv_c + d.eps);
       }
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
+        const int c = (v * lpr + lane) * 8;
+        if (HG) gate_values(g[v], d.gate_act);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const float a = p.gate ? gate_value(g[v][k], d.gate_act) : 1.f;
-          x[v][k] += d.alpha * sc[v][k] * a * u[v][k];
+          const float t = (u[v][k] - mu) * (r * wpo[v][k]) + bpo[v][k];
+          x[v][k] += (HG ? sc[v][k] * g[v][k] : sc[v][k]) * t;
         }
-        store8<TX, VEC>(static_cast<TX*>(p.out_y) + row * d.ldy, (v * lpr + lane) * 8, Cr, x[v]);
+        store8<TX, VEC>(py, c, Cr, x[v]);
       }
     }
     if (d.pre != TG_NORM_NONE) {
       float mu = 0.f;
-      if (layer_pre) {
+      if (d.pre == TG_NORM_LAYER) {
         float s[1] = {0.f};
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
           const int c = (v * lpr + lane) * 8;
+          float t = 0.f;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) s[0] += (VEC ? c < Cr : c + k < Cr) ? x[v][k] : 0.f;
+          for (int k = 0; k < 8; ++k) t += VEC || c + k < Cr ? x[v][k] : 0.f;
+          s[0] += c < Cr ? t : 0.f;
         }
         row_sums(s, lpr, red, turn);
         mu = s[0] * p.inv_c;
@@ -358,29 +392,31 @@ __global__ __launch_bounds__(512) void gated_norm_fwd_kernel(GnP p) {
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         const int c = (v * lpr + lane) * 8;
-        const bool in = c < Cr;
+        float q = 0.f;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          x[v][k] = (VEC ? in : c + k < Cr) ? x[v][k] - mu : 0.f;
-          s[0] += x[v][k] * x[v][k];
+          const float t = x[v][k] - mu;
+          q += VEC || c + k < Cr ? t * t : 0.f;
         }
+        s[0] += c < Cr ? q : 0.f;
       }
       row_sums(s, lpr, red, turn);
       const float r = rsqrtf(s[0] * p.inv_c + d.eps);
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[v][k] = x[v][k] * r * wpr[v][k] + bpr[v][k];
-        store8<TO, VEC>(static_cast<TO*>(p.out_h) + row * d.ldh, (v * lpr + lane) * 8, Cr, x[v]);
+        for (int k = 0; k < 8; ++k) x[v][k] = (x[v][k] - mu) * (r * wpr[v][k]) + bpr[v][k];
+        store8<TO, VEC>(ph, (v * lpr + lane) * 8, Cr, x[v]);
       }
     }
   }
 }
 
 // One item = item_rows consecutive rows of one sub-row of lanes: whole gate rows, or a piece of one (pieces > 0).
-template <typename TO, typename TX, int NV, bool VEC>
+template <typename TO, typename TX, int NV, bool VEC, int MODE>
 __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
-  __shared__ float red[2 * 8 * 4];
+  const bool HO = MODE == 3 ? p.o != nullptr : MODE >= 1, HG = MODE == 3 ? p.gate != nullptr : MODE == 2;
+  __shared__ __attribute__((aligned(16))) float red[2 * 8 * 4];
   extern __shared__ float join[];                                   // [rows of the workgroup][8 lpr]: only where it has several
   const tg_gated_norm_desc& d = p.d;
   const int lpr = 1 << p.lpr_log2, lane = threadIdx.x & (lpr - 1), sub = threadIdx.x >> p.lpr_log2, rpb = blockDim.x >> p.lpr_log2;
@@ -410,8 +446,8 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
       ry[v].load(static_cast<const TX*>(p.y) + r * d.ldy, c, Cr);
       if (p.d_h) rdh[v].load(static_cast<const TO*>(p.d_h) + r * d.ldh, c, Cr);
       if (p.d_y) rdy[v].load(static_cast<const TX*>(p.d_y) + r * d.ld_dy, c, Cr);
-      if (p.o) ro[v].load(static_cast<const TO*>(p.o) + r * d.ldo, c, Cr);
-      if (p.gate) rg[v].load(static_cast<const TO*>(p.gate) + (int64_t)p.gate_of.of((uint32_t)r) * d.ldg, c, Cr);
+      if (HO) ro[v].load(static_cast<const TO*>(p.o) + r * d.ldo, c, Cr);
+      if (HG) rg[v].load(static_cast<const TO*>(p.gate) + (int64_t)p.gate_of.of((uint32_t)r) * d.ldg, c, Cr);
     }
   };
   float ga[NV][8], gs[NV][8];                                       // the gate's activation and its derivative
@@ -451,22 +487,21 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
       ry[v].values(y[v]);
       rdh[v].values(dh[v]);
       rdy[v].values(G[v]);
-      ro[v].values(o[v]);
+      if (HO) ro[v].values(o[v]);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         if (!p.d_h) dh[v][k] = 0.f;
         if (!p.d_y) G[v][k] = 0.f;
-        if (!p.o) o[v][k] = 0.f;
+        if (!HO) o[v][k] = 0.f;
       }
     }
-    if (p.gate && (j == 0 || grow != gate_row)) {                   // a shared gate row: its activation once
+    if (HG && (j == 0 || grow != gate_row)) {                   // a shared gate row: its activation once
       gate_row = grow;
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         float g[8];
         rg[v].values(g);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) gs[v][k] = gate_slope(g[k], d.gate_act, &ga[v][k]);
+        gate_slopes(g, d.gate_act, ga[v], gs[v]);
       }
     }
     if (NV == 1 && j + 1 < p.item_rows) fetch(start + j + 1);
@@ -508,7 +543,7 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
       const float mp = c < Cr ? m2 : 0.f;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        if (d.pre != TG_NORM_NONE) {
+        {                                                            // no pre norm: dh = 0
           const float n = y[v][k] * r_y;
           acc[3][v][k] += dh[v][k] * n;
           acc[4][v][k] += dh[v][k];
@@ -516,11 +551,11 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
         }
       }
       if (p.d_x) store8<TX, VEC>(static_cast<TX*>(p.d_x) + row * d.ldx, c, Cr, G[v]);
-      if (p.o) {
+      if (HO) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const float n = o[v][k] * r_o;
-          const float u = d.post != TG_NORM_NONE ? n * wpost[v][k] + bpost[v][k] : o[v][k];
+          const float n = o[v][k] * r_o;                             // no post norm: deviation 1, weight 1, bias 0
+          const float u = n * wpost[v][k] + bpost[v][k];
           const float a = ga[v][k], D = d.alpha * G[v][k];
           acc[2][v][k] += D * a * u;
           dg[k] = D * sc[v][k] * u * gs[v][k];
@@ -542,7 +577,7 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
         }
       }
     }
-    if (p.o) {
+    if (HO) {
       if (d.post != TG_NORM_NONE) row_sums(q, lpr, red, turn);
       if (p.d_o) {
         const float n1 = d.post != TG_NORM_NONE ? q[0] * p.inv_c : 0.f, n2 = d.post == TG_NORM_LAYER ? q[1] * p.inv_c : 0.f;
@@ -601,41 +636,39 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
   }
 }
 
-struct GnOut {
-  float* p[5];
+// The second launch: sums of partial rows in a fixed order -- the five parameters over the workgroups, then (pieces > 0) every gate
+// row over its pieces.  A workgroup takes 64 columns of one of them: 16 strided sums a column, then a tree over those.
+struct GnSum {
+  float* param[5];
+  const float *part, *gate_part;
+  void* d_gate;
+  int64_t ld;
+  int blocks, pieces, C, ncb;
 };
-// d_param[c] = sum over the workgroups' partials, fixed order: 16 strided sums per column, then a tree over them
-__global__ __launch_bounds__(1024) void gated_norm_params_kernel(const float* __restrict__ part, int blocks, int C, GnOut out) {
+template <typename TO>
+__global__ __launch_bounds__(1024) void gated_norm_sums_kernel(GnSum p) {
   __shared__ float sm[16][64];
-  const int q = blockIdx.y, cl = threadIdx.x & 63, c = blockIdx.x * 64 + cl, w = threadIdx.x >> 6;
-  float* dst = out.p[q];
-  if (!dst) return;
+  const int64_t q = blockIdx.x / p.ncb;
+  const int cl = threadIdx.x & 63, c = (int)(blockIdx.x - q * p.ncb) * 64 + cl, w = threadIdx.x >> 6;
+  if (q < 5 && !p.param[q]) return;
+  const float* src = q < 5 ? p.part + q * p.C : p.gate_part + (q - 5) * p.pieces * p.C;
+  const int64_t stride = q < 5 ? 5 * (int64_t)p.C : p.C;
+  const int n = q < 5 ? p.blocks : p.pieces;
   float s = 0.f;
-  if (c < C) {
-#pragma unroll 4
-    for (int b = w; b < blocks; b += 16) s += part[((int64_t)b * 5 + q) * C + c];
+  if (c < p.C) {
+#pragma unroll 8
+    for (int b = w; b < n; b += 16) s += src[b * stride + c];
   }
   sm[w][cl] = s;
   __syncthreads();
+#pragma unroll
   for (int h = 8; h > 0; h >>= 1) {
     if (w < h) sm[w][cl] += sm[w + h][cl];
     __syncthreads();
   }
-  if (w == 0 && c < C) dst[c] = sm[0][cl];
-}
-
-// d_gate[group][c] = the sum of the pieces of its rows, in order
-template <typename TO>
-__global__ __launch_bounds__(256) void gated_norm_gate_kernel(const float* __restrict__ part, int64_t groups, int pieces, int C,
-                                                              TO* __restrict__ d_gate, int64_t ld) {
-  const int64_t n = groups * C;
-  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n; e += (int64_t)gridDim.x * 256) {
-    const int64_t gi = e / C;
-    const int c = (int)(e - gi * C);
-    float s = 0.f;
-#pragma unroll 4
-    for (int k = 0; k < pieces; ++k) s += part[(gi * pieces + k) * C + c];
-    Elem<TO>::st(d_gate + gi * ld + c, s);
+  if (w == 0 && c < p.C) {
+    if (q < 5) p.param[q][c] = sm[0][cl];
+    else Elem<TO>::st(static_cast<TO*>(p.d_gate) + (q - 5) * p.ld + c, sm[0][cl]);
   }
 }
 
@@ -704,9 +737,16 @@ bool eps_ok(const tg_gated_norm_desc* d) { return d->eps >= 1e-30f && d->eps <= 
   } while (0)
 #define GN_NV(KERN, TO, TX, VECV, ...)                                                                          \
   do {                                                                                                          \
-    if (g.nv == 1) { TG_LAUNCH(name, flops, bytes, (KERN<TO, TX, 1, VECV>), __VA_ARGS__); }                     \
-    else if (g.nv == 2) { TG_LAUNCH(name, flops, bytes, (KERN<TO, TX, 2, VECV>), __VA_ARGS__); }                \
-    else { TG_LAUNCH(name, flops, bytes, (KERN<TO, TX, 4, VECV>), __VA_ARGS__); }                               \
+    if (g.nv == 1) { GN_MODE(KERN, TO, TX, 1, VECV, __VA_ARGS__); }                                             \
+    else if (g.nv == 2) { GN_MODE(KERN, TO, TX, 2, VECV, __VA_ARGS__); }                                        \
+    else { TG_LAUNCH(name, flops, bytes, (KERN<TO, TX, 4, VECV, 3>), __VA_ARGS__); }                            \
+  } while (0)
+#define GN_MODE(KERN, TO, TX, NVV, VECV, ...)                                                                   \
+  do {                                                                                                          \
+    if (!VECV) { TG_LAUNCH(name, flops, bytes, (KERN<TO, TX, NVV, VECV, VECV ? 0 : 3>), __VA_ARGS__); }           \
+    else if (gate) { TG_LAUNCH(name, flops, bytes, (KERN<TO, TX, NVV, VECV, VECV ? 2 : 3>), __VA_ARGS__); }     \
+    else if (o) { TG_LAUNCH(name, flops, bytes, (KERN<TO, TX, NVV, VECV, VECV ? 1 : 3>), __VA_ARGS__); }        \
+    else { TG_LAUNCH(name, flops, bytes, (KERN<TO, TX, NVV, VECV, VECV ? 0 : 3>), __VA_ARGS__); }               \
   } while (0)
 
 extern "C" int tg_gated_norm_forward(const tg_gated_norm_desc* d, const void* x, const void* o, const void* gate, const float* w_post,
@@ -804,18 +844,13 @@ extern "C" int tg_gated_norm_backward(const tg_gated_norm_desc* d, const void* d
     const size_t lds = g.rpb > 1 ? (size_t)g.block * 8 * sizeof(float) : 0;
     if (vec) GN_PICK(gated_norm_bwd_kernel, true, grid, block, lds, ST(stream), p);
     else GN_PICK(gated_norm_bwd_kernel, false, grid, block, lds, ST(stream), p);
-    if (d_gate && g.pieces > 0) {
-      const int64_t groups = cdiv64(d->rows, d->rows_per_gate);
-      const dim3 gg(grid_1d(groups * C, 256));
-      if (d->dtype == TG_F32)
-        hipLaunchKernelGGL((gated_norm_gate_kernel<float>), gg, dim3(256), 0, ST(stream), p.gate_part, groups, g.pieces, C, (float*)d_gate, d->ld_dg);
-      else
-        hipLaunchKernelGGL((gated_norm_gate_kernel<u16>), gg, dim3(256), 0, ST(stream), p.gate_part, groups, g.pieces, C, (u16*)d_gate, d->ld_dg);
-    }
   }
-  if (want) {
-    const GnOut out = {{d_w_post, d_b_post, d_scale, d_w_pre, d_b_pre}};
-    hipLaunchKernelGGL(gated_norm_params_kernel, dim3((C + 63) / 64, 5), dim3(1024), 0, ST(stream), ws, d->rows > 0 ? g.blocks : 0, C, out);
+  const bool gates = d->rows > 0 && d_gate && g.pieces > 0;
+  if (want || gates) {
+    const GnSum q = {{d_w_post, d_b_post, d_scale, d_w_pre, d_b_pre}, ws, ws + pf, d_gate, d->ld_dg, d->rows > 0 ? g.blocks : 0, g.pieces, C, (C + 63) / 64};
+    const dim3 grid((unsigned)(q.ncb * (5 + (gates ? cdiv64(d->rows, d->rows_per_gate) : 0))));
+    if (d->dtype == TG_F32) hipLaunchKernelGGL((gated_norm_sums_kernel<float>), grid, dim3(1024), 0, ST(stream), q);
+    else hipLaunchKernelGGL((gated_norm_sums_kernel<u16>), grid, dim3(1024), 0, ST(stream), q);
   }
   TG_CHECK_LAUNCH();
 }
