@@ -6,11 +6,13 @@
 //
 // A step is an affine map of the state, h -> P h + L, and maps compose: (P2, L2) after (P1, L1) = (P1 P2, P2 L1 + L2).  A sequence
 // is cut into chunks, each chunk into tiles of 8 W steps (W waves, 8 steps each in registers): every wave composes its 8 steps,
-// the maps meet in LDS, every wave enters its steps with the right state and writes them.  Where the channels alone fill the
-// device there is one chunk and x, g are read once; otherwise a first launch composes the chunks, a second one runs over the
-// chunks' maps (few values), a third one writes the outputs.  About 14 / 50 operations a value: bound by HBM.  States, maps and
-// gradient sums are fp32; 1 - f is (1 - floor) sigmoid(-g), not a difference.  The forward pass keeps the state before every
-// tile (fp32, 1 value in 64): the backward pass makes the states of a tile again from it instead of reading rounded ones.
+// the maps meet in LDS, every wave enters its steps with the right state and writes them; the next tile is fetched meanwhile.  Where
+// the channels alone fill the device there is one chunk and x, g are read once; otherwise a first launch composes each chunk's map
+// and the second one's workgroups compose the maps in front of their chunk (behind it, backward) before they begin: x and g are
+// read twice, the second time from the chunk that was read last on, so that the memory-side cache still holds most of them.
+// About 14 / 50 operations a value: bound by HBM.  States, maps and gradient sums are fp32; 1 - f is (1 - floor) sigmoid(-g), not a
+// difference.  The forward pass keeps the state before every tile (fp32, 1 value in 64): the backward pass makes the states of a tile
+// again from it instead of reading rounded ones.
 //
 // A reset (a new sequence begins at step t) drops the state by selection, not by a product with 0: what was in it, NaN included,
 // does not get past.  In a composed map P = -1 says that a reset is inside (P is a product of values in [0, 1] otherwise).
@@ -32,44 +34,56 @@ struct GsP {
   float *hT, *d_h0;
   float *tiles;                              // [B][ntiles][D] state before each tile
   float *agg_p, *agg_l;                      // [B][nc][D] the chunks' maps
-  float *rev_l, *rev_in;                     // [B][nc][D] backward: chunk's part, gradient that enters a chunk from behind
+  float *rev_l;                              // [B][nc][D] backward: what a chunk adds to the gradient that leaves it in front
   float *floor_part;                         // [B * nc][D]
   int ncb, nc, tpc, ntiles, W;               // channel blocks, chunks, tiles of a chunk, tiles, waves
   int keep_tiles;
 };
 
-template <typename T, int V>
-__device__ __forceinline__ void ldv(const T* p, float (&f)[V]) {
-  if constexpr (V == 1) {
-    f[0] = Elem<T>::ld(p);
-  } else if constexpr (sizeof(T) == 2) {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+// V neighbouring channels of one step, as they lie in memory
+template <typename T, int V> struct Raw;
+template <> struct Raw<u16, 1> {
+  u16 w;
+  __device__ __forceinline__ void load(const u16* p) { w = *p; }
+  __device__ __forceinline__ void zero() { w = 0; }
+  __device__ __forceinline__ void values(float (&f)[1]) const { f[0] = bf2f(w); }
+  static __device__ __forceinline__ void store(u16* p, const float (&f)[1]) { *p = f2bf(f[0]); }
+};
+template <> struct Raw<u16, 2> {
+  uint32_t w;
+  __device__ __forceinline__ void load(const u16* p) { w = *reinterpret_cast<const uint32_t*>(p); }
+  __device__ __forceinline__ void zero() { w = 0; }
+  __device__ __forceinline__ void values(float (&f)[2]) const {
     f[0] = __uint_as_float(w << 16);
     f[1] = __uint_as_float(w & 0xffff0000u);
-  } else {
-    const float2 w = *reinterpret_cast<const float2*>(p);
+  }
+  static __device__ __forceinline__ void store(u16* p, const float (&f)[2]) {
+    *reinterpret_cast<uint32_t*>(p) = (uint32_t)f2bf(f[0]) | ((uint32_t)f2bf(f[1]) << 16);
+  }
+};
+template <> struct Raw<float, 1> {
+  float w;
+  __device__ __forceinline__ void load(const float* p) { w = *p; }
+  __device__ __forceinline__ void zero() { w = 0.f; }
+  __device__ __forceinline__ void values(float (&f)[1]) const { f[0] = w; }
+  static __device__ __forceinline__ void store(float* p, const float (&f)[1]) { *p = f[0]; }
+};
+template <> struct Raw<float, 2> {
+  float2 w;
+  __device__ __forceinline__ void load(const float* p) { w = *reinterpret_cast<const float2*>(p); }
+  __device__ __forceinline__ void zero() { w = make_float2(0.f, 0.f); }
+  __device__ __forceinline__ void values(float (&f)[2]) const {
     f[0] = w.x;
     f[1] = w.y;
   }
-}
-template <typename T, int V>
-__device__ __forceinline__ void stv(T* p, const float (&f)[V]) {
-  if constexpr (V == 1) {
-    Elem<T>::st(p, f[0]);
-  } else if constexpr (sizeof(T) == 2) {
-    *reinterpret_cast<uint32_t*>(p) = (uint32_t)f2bf(f[0]) | ((uint32_t)f2bf(f[1]) << 16);
-  } else {
-    *reinterpret_cast<float2*>(p) = make_float2(f[0], f[1]);
-  }
-}
+  static __device__ __forceinline__ void store(float* p, const float (&f)[2]) { *reinterpret_cast<float2*>(p) = make_float2(f[0], f[1]); }
+};
 
-// sigmoid(g) and sigmoid(-g) without a difference: e = exp(-|g|), 1 / (1 + e) and e / (1 + e)
+// sigmoid(g) and sigmoid(-g) without a difference: e = exp(-g), 1 / (1 + e) and e / (1 + e); e past 2^100: 1 (e may be infinite)
 __device__ __forceinline__ void sigmoids(float g, float& up, float& down) {
-  const float e = __expf(-fabsf(g));
-  const float r = __builtin_amdgcn_rcpf(1.f + e), q = e * r;
-  up = g >= 0.f ? r : q;
-  down = g >= 0.f ? q : r;
-  if (g != g) up = down = g;
+  const float e = __expf(-g);
+  up = __builtin_amdgcn_rcpf(1.f + e);
+  down = e > 0x1p100f ? 1.f : e * up;
 }
 
 // state -> P state + L; P = -1: a reset inside
@@ -79,319 +93,406 @@ __device__ __forceinline__ void compose(float& P, float& L, float P2, float L2) 
   P = P < 0.f || P2 < 0.f ? -1.f : P * P2;
 }
 
-struct Steps {                                                     // the 8 steps of a wave: which are live, which begin a sequence
-  int live;
-  unsigned reset;
-};
-__device__ __forceinline__ Steps steps_of(const GsP& p, int b, int64_t t0, int len) {
-  Steps s;
-  const int64_t left = len - t0;
-  s.live = left < 0 ? 0 : (left > GS_L ? GS_L : (int)left);
-  s.reset = 0;
-  if (p.reset) {
-    const int lane = threadIdx.x & 63;
-    const bool r = lane < s.live && p.reset[(int64_t)b * p.d.T + t0 + lane] != 0;
-    s.reset = (unsigned)__ballot(r);
+// What the kernels know of their place: channels, chunk, steps.  Everything but the channel is the same for a whole wave.
+template <int V>
+struct Place {
+  int lane, wave, b, chunk, c, cl, len, ntiles;
+  bool on;
+  int64_t first;
+  __device__ __forceinline__ Place(const GsP& p, int block) {
+    lane = threadIdx.x & 63;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int cb = block % p.ncb, rest = block / p.ncb;
+    chunk = rest % p.nc;
+    b = rest / p.nc;
+    c = (cb * 64 + lane) * V;
+    on = c < p.d.D;
+    cl = on ? c : p.d.D - V;                                       // lanes past the end read the last channels and write nothing
+    len = p.d.T;
+    if (p.lengths) {
+      const int n = p.lengths[b];
+      len = n < 0 ? 0 : (n < p.d.T ? n : p.d.T);
+    }
+    first = (int64_t)chunk * p.tpc;
+    ntiles = (int)(p.ntiles - first < p.tpc ? p.ntiles - first : p.tpc);
   }
-  return s;
+  // of a wave's 8 steps from t0: how many are live, and (a byte a lane, looked at later) which begin a sequence
+  __device__ __forceinline__ int live(int64_t t0) const {
+    const int64_t left = len - t0;
+    return left < 0 ? 0 : (left > GS_L ? GS_L : (int)left);
+  }
+  __device__ __forceinline__ unsigned resets(const GsP& p, int64_t t0, int n) const {
+    return p.reset && lane < n ? p.reset[(int64_t)b * p.d.T + t0 + lane] : 0;
+  }
+};
+
+// 8 steps of one tensor; `base`: its row of the batch (the same for a wave), cl: the lane's channel
+template <typename T, int V>
+__device__ __forceinline__ void fetch(Raw<T, V> (&r)[GS_L], const T* base, int64_t t0, int64_t stride, int cl, int live) {
+  const T* at = base + t0 * stride;
+  if (live == GS_L) {
+#pragma unroll
+    for (int j = 0; j < GS_L; ++j) r[j].load(at + j * stride + cl);
+  } else {
+#pragma unroll
+    for (int j = 0; j < GS_L; ++j) {
+      r[j].zero();
+      if (j < live) r[j].load(at + j * stride + cl);
+    }
+  }
+}
+
+// The state that enters a chunk (or, backward, the gradient): `start` carried over the maps of the chunks from..to (step +1 or -1),
+// each wave a part of them, the parts joined in LDS.  Every wave returns the same values.
+template <int V>
+__device__ __forceinline__ void enter(const GsP& p, const Place<V>& q, const float* mp, const float* ml, int count, int from, int step,
+                                      float (&h)[V], float (*sP)[64 * V], float (*sL)[64 * V]) {
+  const int W = p.W, per = (count + W - 1) / W, i0 = q.wave * per, i1 = i0 + per < count ? i0 + per : count;
+  float P[V], L[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) { P[v] = 1.f; L[v] = 0.f; }
+#pragma unroll 4
+  for (int i = i0; i < i1; ++i) {
+    const int64_t at = ((int64_t)q.b * p.nc + from + i * step) * p.d.D + q.cl;
+#pragma unroll
+    for (int v = 0; v < V; ++v) compose(P[v], L[v], mp[at + v], ml[at + v]);
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) { sP[q.wave][q.lane * V + v] = P[v]; sL[q.wave][q.lane * V + v] = L[v]; }
+  __syncthreads();
+  for (int w = 0; w < W; ++w) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = apply(sP[w][q.lane * V + v], sL[w][q.lane * V + v], h[v]);
+  }
+  __syncthreads();
 }
 
 // Forward.  OUT false: the chunk's map only (each wave a contiguous part of it); true: states and outputs.
 template <typename T, int V, bool OUT>
 __global__ __launch_bounds__(512) void gated_scan_fwd_kernel(GsP p) {
   __shared__ float sP[GS_MAXW][64 * V], sL[GS_MAXW][64 * V];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = p.W;
-  const int cb = blockIdx.x % p.ncb, rest = blockIdx.x / p.ncb, chunk = rest % p.nc, b = rest / p.nc;
-  const int c = (cb * 64 + lane) * V, D = p.d.D, Tn = p.d.T;
-  const bool on = c < D;
-  int len = Tn;
-  if (p.lengths) {
-    const int n = p.lengths[b];
-    len = n < 0 ? 0 : (n < Tn ? n : Tn);
+  const Place<V> q(p, OUT ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x);
+  const int W = p.W, D = p.d.D, lane = q.lane, wave = q.wave;
+  const T* const xr = static_cast<const T*>(p.x) + (int64_t)q.b * p.d.x_b;
+  const T* const gr = static_cast<const T*>(p.g) + (int64_t)q.b * p.d.g_b;
+  T* const yr = static_cast<T*>(p.y) + (int64_t)q.b * p.d.y_b;
+  // OUT: tile i, wave after wave; otherwise this wave's i-th group of 8 steps of its contiguous part of the chunk
+  auto step0 = [&](int i) -> int64_t { return OUT ? ((q.first + i) * W + wave) * GS_L : (q.first * W + (int64_t)wave * q.ntiles + i) * GS_L; };
+  Raw<T, V> rx[GS_L], rg[GS_L];
+  int64_t t0 = step0(0);
+  int live = q.live(t0);
+  fetch<T, V>(rg, gr, t0, p.d.g_t, q.cl, live);
+  fetch<T, V>(rx, xr, t0, p.d.x_t, q.cl, live);
+  unsigned rr = q.resets(p, t0, live);
+  float low[V], k[V], H[V], P[V], L[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    low[v] = p.floor ? p.floor[q.cl + v] : 0.f;
+    k[v] = 1.f - low[v];
+    H[v] = OUT && p.h0 ? p.h0[(int64_t)q.b * D + q.cl + v] : 0.f;
+    P[v] = 1.f;
+    L[v] = 0.f;
   }
-  const T* xr = static_cast<const T*>(p.x) + (int64_t)b * p.d.x_b + c;
-  const T* gr = static_cast<const T*>(p.g) + (int64_t)b * p.d.g_b + c;
-  T* yr = static_cast<T*>(p.y) + (int64_t)b * p.d.y_b + c;
-  float low[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) low[v] = p.floor && on ? p.floor[c + v] : 0.f;
-  const int64_t first = (int64_t)chunk * p.tpc;
-  const int ntiles = (int)(p.ntiles - first < p.tpc ? p.ntiles - first : p.tpc);
-  const int64_t state = ((int64_t)b * p.ntiles + first) * D + c;  // of p.tiles
-
-  float H[V], P[V], L[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) { H[v] = 0.f; P[v] = 1.f; L[v] = 0.f; }
-  if (OUT && on) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) H[v] = p.nc > 1 ? p.tiles[state + v] : (p.h0 ? p.h0[(int64_t)b * D + c + v] : 0.f);
-  }
-  for (int i = 0; i < ntiles; ++i) {
-    // OUT: tile i, wave after wave; otherwise this wave's i-th group of 8 steps of its contiguous part of the chunk
-    const int64_t t0 = OUT ? ((first + i) * W + wave) * GS_L : (first * W + (int64_t)wave * ntiles + i) * GS_L;
-    const Steps st = steps_of(p, b, t0, len);
+  if (OUT && q.chunk > 0) enter<V>(p, q, p.agg_p, p.agg_l, q.chunk, 0, 1, H, sP, sL);
+  for (int i = 0; i < q.ntiles; ++i) {
+    const unsigned fresh = p.reset ? (unsigned)__ballot(rr != 0) : 0;
+    const int now = live;
+    const int64_t tn = t0;
     float f[GS_L][V], a[GS_L][V];
 #pragma unroll
     for (int j = 0; j < GS_L; ++j) {
-      const bool ok = on && j < st.live;
       float g[V], x[V];
-#pragma unroll
-      for (int v = 0; v < V; ++v) { g[v] = 0.f; x[v] = 0.f; }
-      if (ok) {
-        ldv<T, V>(gr + (t0 + j) * p.d.g_t, g);
-        ldv<T, V>(xr + (t0 + j) * p.d.x_t, x);
-      }
+      rg[j].values(g);
+      rx[j].values(x);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         float up, down;
         sigmoids(g[v], up, down);
-        f[j][v] = ok ? low[v] + (1.f - low[v]) * up : 1.f;
-        a[j][v] = ok ? (1.f - low[v]) * down * x[v] : 0.f;
+        f[j][v] = low[v] + k[v] * up;
+        a[j][v] = k[v] * down * x[v];
       }
+    }
+    if (i + 1 < q.ntiles) {
+      t0 = step0(i + 1);
+      live = q.live(t0);
+      fetch<T, V>(rg, gr, t0, p.d.g_t, q.cl, live);
+      fetch<T, V>(rx, xr, t0, p.d.x_t, q.cl, live);
+      rr = q.resets(p, t0, live);
+    }
+    if (now < GS_L) {
+#pragma unroll
+      for (int j = 0; j < GS_L; ++j)
+        if (j >= now) {
+#pragma unroll
+          for (int v = 0; v < V; ++v) { f[j][v] = 1.f; a[j][v] = 0.f; }
+        }
     }
     if (OUT) {
 #pragma unroll
       for (int v = 0; v < V; ++v) { P[v] = 1.f; L[v] = 0.f; }
     }
+    if (fresh == 0) {
+      float Q[V];
 #pragma unroll
-    for (int j = 0; j < GS_L; ++j) {
-      const bool r = st.reset >> j & 1;
+      for (int v = 0; v < V; ++v) Q[v] = 1.f;
 #pragma unroll
-      for (int v = 0; v < V; ++v) compose(P[v], L[v], r ? -1.f : f[j][v], a[j][v]);
-    }
-    if constexpr (OUT) {
-      if (i > 0) __syncthreads();                                  // the last tile's maps have been read
-#pragma unroll
-      for (int v = 0; v < V; ++v) { sP[wave][lane * V + v] = P[v]; sL[wave][lane * V + v] = L[v]; }
-      __syncthreads();
-      float h[V];
-#pragma unroll
-      for (int v = 0; v < V; ++v) h[v] = H[v];
-      if (p.keep_tiles && wave == 0 && on && !(p.nc > 1 && i == 0)) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) p.tiles[state + (int64_t)i * D + v] = H[v];
-      }
-      for (int w = 0; w < W; ++w) {
+      for (int j = 0; j < GS_L; ++j)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          if (w == wave) h[v] = H[v];
-          H[v] = apply(sP[w][lane * V + v], sL[w][lane * V + v], H[v]);
+          L[v] = f[j][v] * L[v] + a[j][v];
+          Q[v] *= f[j][v];
         }
+#pragma unroll
+      for (int v = 0; v < V; ++v) P[v] = P[v] < 0.f ? -1.f : P[v] * Q[v];
+    } else {
+#pragma unroll
+      for (int j = 0; j < GS_L; ++j)
+#pragma unroll
+        for (int v = 0; v < V; ++v) compose(P[v], L[v], fresh >> j & 1 ? -1.f : f[j][v], a[j][v]);
+    }
+    if constexpr (OUT) {
+      float h[V];
+      if (W > 1) {
+        if (i > 0) __syncthreads();                                // the last tile's maps have been read
+#pragma unroll
+        for (int v = 0; v < V; ++v) { sP[wave][lane * V + v] = P[v]; sL[wave][lane * V + v] = L[v]; }
+        __syncthreads();
       }
 #pragma unroll
+      for (int v = 0; v < V; ++v) h[v] = H[v];
+      if (p.keep_tiles && wave == 0 && q.on) {
+        float* const st = p.tiles + ((int64_t)q.b * p.ntiles + q.first + i) * D + q.c;
+#pragma unroll
+        for (int v = 0; v < V; ++v) st[v] = H[v];
+      }
+      if (W > 1) {
+        for (int w = 0; w < W; ++w) {
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            if (w == wave) h[v] = H[v];
+            H[v] = apply(sP[w][lane * V + v], sL[w][lane * V + v], H[v]);
+          }
+        }
+      }
+      T* const out = yr + tn * p.d.y_t;
+#pragma unroll
       for (int j = 0; j < GS_L; ++j) {
-        const bool r = st.reset >> j & 1;
         float o[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          h[v] = (r ? 0.f : f[j][v] * h[v]) + a[j][v];
-          o[v] = j < st.live ? h[v] : 0.f;
+          h[v] = (fresh >> j & 1 ? 0.f : f[j][v] * h[v]) + a[j][v];
+          o[v] = j < now ? h[v] : 0.f;
         }
-        if (on && t0 + j < Tn) stv<T, V>(yr + (t0 + j) * p.d.y_t, o);
+        if (tn + j < p.d.T && q.on) Raw<T, V>::store(out + j * p.d.y_t + q.c, o);
+      }
+      if (W == 1) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) H[v] = h[v];
       }
     }
   }
   if constexpr (OUT) {
-    if (p.hT && chunk == p.nc - 1 && wave == 0 && on) {
+    if (p.hT && q.chunk == p.nc - 1 && wave == 0 && q.on) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) p.hT[(int64_t)b * D + c + v] = H[v];
+      for (int v = 0; v < V; ++v) p.hT[(int64_t)q.b * D + q.c + v] = H[v];
     }
   } else {
 #pragma unroll
     for (int v = 0; v < V; ++v) { sP[wave][lane * V + v] = P[v]; sL[wave][lane * V + v] = L[v]; }
     __syncthreads();
-    if (wave == 0 && on) {
+    if (wave == 0 && q.on) {
       for (int w = 1; w < W; ++w) {
 #pragma unroll
         for (int v = 0; v < V; ++v) compose(P[v], L[v], sP[w][lane * V + v], sL[w][lane * V + v]);
       }
+      const int64_t at = ((int64_t)q.b * p.nc + q.chunk) * D + q.c;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const int64_t at = ((int64_t)b * p.nc + chunk) * D + c + v;
-        p.agg_p[at] = P[v];
-        p.agg_l[at] = L[v];
+        p.agg_p[at + v] = P[v];
+        p.agg_l[at + v] = L[v];
       }
     }
   }
-}
-
-// The states before the chunks, from h0 over the chunks' maps; written where the outputs' launch looks for them.
-__global__ __launch_bounds__(64) void gated_scan_carry_kernel(GsP p) {
-  const int64_t e = (int64_t)blockIdx.x * 64 + threadIdx.x;
-  const int D = p.d.D;
-  if (e >= (int64_t)p.d.B * D) return;
-  const int64_t b = e / D, c = e - b * D;
-  float H = p.h0 ? p.h0[e] : 0.f;
-#pragma unroll 8
-  for (int k = 0; k < p.nc; ++k) {
-    const int64_t at = (b * p.nc + k) * D + c;
-    p.tiles[(b * p.ntiles + (int64_t)k * p.tpc) * D + c] = H;
-    H = apply(p.agg_p[at], p.agg_l[at], H);
-  }
-}
-
-// The gradient that enters each chunk from behind, and what is left of it before the first step.
-__global__ __launch_bounds__(64) void gated_scan_rcarry_kernel(GsP p) {
-  const int64_t e = (int64_t)blockIdx.x * 64 + threadIdx.x;
-  const int D = p.d.D;
-  if (e >= (int64_t)p.d.B * D) return;
-  const int64_t b = e / D, c = e - b * D;
-  float R = p.d_hT ? p.d_hT[e] : 0.f;
-#pragma unroll 8
-  for (int k = p.nc - 1; k >= 0; --k) {
-    const int64_t at = (b * p.nc + k) * D + c;
-    p.rev_in[at] = R;
-    R = apply(p.agg_p[at], p.rev_l[at], R);
-  }
-  if (p.d_h0) p.d_h0[e] = R;
 }
 
 // Backward.  OUT false: what a chunk adds to the gradient that leaves it in front; true: the gradients.
 template <typename T, int V, bool OUT>
 __global__ __launch_bounds__(512) void gated_scan_bwd_kernel(GsP p) {
   __shared__ float sP[GS_MAXW][64 * V], sL[GS_MAXW][64 * V], sR[GS_MAXW][64 * V];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = p.W;
-  const int cb = blockIdx.x % p.ncb, rest = blockIdx.x / p.ncb, chunk = rest % p.nc, b = rest / p.nc;
-  const int c = (cb * 64 + lane) * V, D = p.d.D, Tn = p.d.T;
-  const bool on = c < D;
-  int len = Tn;
-  if (p.lengths) {
-    const int n = p.lengths[b];
-    len = n < 0 ? 0 : (n < Tn ? n : Tn);
+  const Place<V> q(p, OUT ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x);
+  const int W = p.W, D = p.d.D, lane = q.lane, wave = q.wave;
+  const T* const xr = static_cast<const T*>(p.x) + (int64_t)q.b * p.d.x_b;
+  const T* const gr = static_cast<const T*>(p.g) + (int64_t)q.b * p.d.g_b;
+  const T* const er = static_cast<const T*>(p.d_y) + (int64_t)q.b * p.d.dy_b;
+  T* const dxr = static_cast<T*>(p.d_x) + (int64_t)q.b * p.d.dx_b;
+  T* const dgr = static_cast<T*>(p.d_g) + (int64_t)q.b * p.d.dg_b;
+  auto step0 = [&](int i) -> int64_t { return OUT ? ((q.first + i) * W + wave) * GS_L : (q.first * W + (int64_t)wave * q.ntiles + i) * GS_L; };
+  Raw<T, V> rx[GS_L], rg[GS_L], re[GS_L];
+  float rH[V];
+  auto fetch_all = [&](int i, int64_t t0, int live) {
+    fetch<T, V>(rg, gr, t0, p.d.g_t, q.cl, live);
+    fetch<T, V>(re, er, t0, p.d.dy_t, q.cl, p.d_y ? live : 0);
+    if (OUT) {
+      fetch<T, V>(rx, xr, t0, p.d.x_t, q.cl, live);
+      const float* const st = p.tiles + ((int64_t)q.b * p.ntiles + q.first + i) * D + q.cl;
+#pragma unroll
+      for (int v = 0; v < V; ++v) rH[v] = st[v];
+    }
+  };
+  int64_t t0 = step0(q.ntiles - 1);
+  int live = q.live(t0);
+  fetch_all(q.ntiles - 1, t0, live);
+  unsigned rr = q.resets(p, t0, live);
+  float low[V], k[V], R[V], dlow[V], P[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    low[v] = p.floor ? p.floor[q.cl + v] : 0.f;
+    k[v] = 1.f - low[v];
+    R[v] = OUT && p.d_hT ? p.d_hT[(int64_t)q.b * D + q.cl + v] : 0.f;
+    dlow[v] = 0.f;
+    P[v] = 1.f;
   }
-  const T* xr = static_cast<const T*>(p.x) + (int64_t)b * p.d.x_b + c;
-  const T* gr = static_cast<const T*>(p.g) + (int64_t)b * p.d.g_b + c;
-  const T* er = static_cast<const T*>(p.d_y) + (int64_t)b * p.d.dy_b + c;
-  T* dxr = static_cast<T*>(p.d_x) + (int64_t)b * p.d.dx_b + c;
-  T* dgr = static_cast<T*>(p.d_g) + (int64_t)b * p.d.dg_b + c;
-  float low[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) low[v] = p.floor && on ? p.floor[c + v] : 0.f;
-  const int64_t first = (int64_t)chunk * p.tpc;
-  const int ntiles = (int)(p.ntiles - first < p.tpc ? p.ntiles - first : p.tpc);
-  const int64_t chunk_at = ((int64_t)b * p.nc + chunk) * D + c;
-
-  float R[V], dlow[V], P[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) { R[v] = 0.f; dlow[v] = 0.f; P[v] = 1.f; }
-  if (OUT && on) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) R[v] = p.nc > 1 ? p.rev_in[chunk_at + v] : (p.d_hT ? p.d_hT[(int64_t)b * D + c + v] : 0.f);
-  }
-  for (int i = ntiles - 1; i >= 0; --i) {
-    const int64_t t0 = OUT ? ((first + i) * W + wave) * GS_L : (first * W + (int64_t)wave * ntiles + i) * GS_L;
-    const Steps st = steps_of(p, b, t0, len);
-    float up[GS_L][V], down[GS_L][V], x[GS_L][V], e[GS_L][V];
+  if (OUT && q.chunk < p.nc - 1) enter<V>(p, q, p.agg_p, p.rev_l, p.nc - 1 - q.chunk, p.nc - 1, -1, R, sP, sL);
+  for (int i = q.ntiles - 1; i >= 0; --i) {
+    const unsigned fresh = p.reset ? (unsigned)__ballot(rr != 0) : 0;
+    const int now = live;
+    const int64_t tn = t0;
+    float up[GS_L][V], down[GS_L][V], x[GS_L][V], e[GS_L][V], H[V];
 #pragma unroll
     for (int j = 0; j < GS_L; ++j) {
-      const bool ok = on && j < st.live;
       float g[V];
-#pragma unroll
-      for (int v = 0; v < V; ++v) { g[v] = 0.f; x[j][v] = 0.f; e[j][v] = 0.f; }
-      if (ok) {
-        ldv<T, V>(gr + (t0 + j) * p.d.g_t, g);
-        if (p.d_y) ldv<T, V>(er + (t0 + j) * p.d.dy_t, e[j]);
-        if (OUT) ldv<T, V>(xr + (t0 + j) * p.d.x_t, x[j]);
-      }
+      rg[j].values(g);
+      re[j].values(e[j]);
+      if (OUT) rx[j].values(x[j]);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         sigmoids(g[v], up[j][v], down[j][v]);
-        if (!OUT) x[j][v] = ok ? low[v] + (1.f - low[v]) * up[j][v] : 1.f;            // f: x is not needed
+        H[v] = rH[v];
       }
+    }
+    if (i > 0) {
+      t0 = step0(i - 1);
+      live = q.live(t0);
+      fetch_all(i - 1, t0, live);
+      rr = q.resets(p, t0, live);
     }
     if constexpr (!OUT) {
 #pragma unroll
       for (int j = GS_L - 1; j >= 0; --j) {
-        const bool r = st.reset >> j & 1;
+        if (j < now) {
+          const bool r = fresh >> j & 1;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          R[v] = r ? 0.f : x[j][v] * (e[j][v] + R[v]);
-          P[v] = r || P[v] < 0.f ? -1.f : P[v] * x[j][v];
+          for (int v = 0; v < V; ++v) {
+            const float f = low[v] + k[v] * up[j][v];
+            R[v] = r ? 0.f : f * (e[j][v] + R[v]);
+            P[v] = r || P[v] < 0.f ? -1.f : P[v] * f;
+          }
         }
       }
     } else {
-      float h[GS_L][V], Lf[V], Lr[V];
+      float Lf[V], Lr[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) { P[v] = 1.f; Lf[v] = 0.f; Lr[v] = 0.f; }
+      if (now == GS_L && fresh == 0) {
 #pragma unroll
-      for (int j = 0; j < GS_L; ++j) {
-        const bool r = st.reset >> j & 1, ok = j < st.live;
+        for (int j = 0; j < GS_L; ++j)
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float f = ok ? low[v] + (1.f - low[v]) * up[j][v] : 1.f;
-          const float a = ok ? (1.f - low[v]) * down[j][v] * x[j][v] : 0.f;
-          compose(P[v], Lf[v], r ? -1.f : f, a);
-        }
-      }
+          for (int v = 0; v < V; ++v) {
+            const float f = low[v] + k[v] * up[j][v];
+            Lf[v] = f * Lf[v] + k[v] * down[j][v] * x[j][v];
+            P[v] *= f;
+          }
 #pragma unroll
-      for (int j = GS_L - 1; j >= 0; --j) {
-        const bool r = st.reset >> j & 1, ok = j < st.live;
+        for (int j = GS_L - 1; j >= 0; --j)
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float f = ok ? low[v] + (1.f - low[v]) * up[j][v] : 1.f;
-          Lr[v] = r ? 0.f : f * (e[j][v] + Lr[v]);
-        }
-      }
-      if (i < ntiles - 1) __syncthreads();
+          for (int v = 0; v < V; ++v) Lr[v] = (low[v] + k[v] * up[j][v]) * (e[j][v] + Lr[v]);
+      } else {
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        sP[wave][lane * V + v] = P[v];
-        sL[wave][lane * V + v] = Lf[v];
-        sR[wave][lane * V + v] = Lr[v];
-      }
-      float H[V];
+        for (int j = 0; j < GS_L; ++j)
+          if (j < now) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) H[v] = on ? p.tiles[((int64_t)b * p.ntiles + first + i) * D + c + v] : 0.f;
-      __syncthreads();
-      for (int w = 0; w < wave; ++w) {
+            for (int v = 0; v < V; ++v) compose(P[v], Lf[v], fresh >> j & 1 ? -1.f : low[v] + k[v] * up[j][v], k[v] * down[j][v] * x[j][v]);
+          }
 #pragma unroll
-        for (int v = 0; v < V; ++v) H[v] = apply(sP[w][lane * V + v], sL[w][lane * V + v], H[v]);
+        for (int j = GS_L - 1; j >= 0; --j)
+          if (j < now) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) Lr[v] = fresh >> j & 1 ? 0.f : (low[v] + k[v] * up[j][v]) * (e[j][v] + Lr[v]);
+          }
       }
       float Rw[V];
-#pragma unroll
-      for (int v = 0; v < V; ++v) Rw[v] = R[v];
-      for (int w = W - 1; w >= 0; --w) {
+      if (W > 1) {
+        if (i < q.ntiles - 1) __syncthreads();                     // the last tile's maps have been read
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          if (w == wave) Rw[v] = R[v];
-          R[v] = apply(sP[w][lane * V + v], sR[w][lane * V + v], R[v]);
+          sP[wave][lane * V + v] = P[v];
+          sL[wave][lane * V + v] = Lf[v];
+          sR[wave][lane * V + v] = Lr[v];
         }
+        __syncthreads();
+        for (int w = 0; w < wave; ++w) {
+#pragma unroll
+          for (int v = 0; v < V; ++v) H[v] = apply(sP[w][lane * V + v], sL[w][lane * V + v], H[v]);
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) Rw[v] = R[v];
+        for (int w = W - 1; w >= 0; --w) {
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            if (w == wave) Rw[v] = R[v];
+            R[v] = apply(sP[w][lane * V + v], sR[w][lane * V + v], R[v]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) Rw[v] = R[v];
       }
+      float h[GS_L][V];
 #pragma unroll
       for (int j = 0; j < GS_L; ++j) {                              // the state before each step
-        const bool r = st.reset >> j & 1, ok = j < st.live;
+        const bool r = fresh >> j & 1;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           h[j][v] = r ? 0.f : H[v];
-          if (ok) H[v] = (low[v] + (1.f - low[v]) * up[j][v]) * h[j][v] + (1.f - low[v]) * down[j][v] * x[j][v];
+          H[v] = (low[v] + k[v] * up[j][v]) * h[j][v] + k[v] * down[j][v] * x[j][v];   // behind the live steps nobody looks at it
         }
       }
+      T* const ox = dxr + tn * p.d.dx_t;
+      T* const og = dgr + tn * p.d.dg_t;
 #pragma unroll
       for (int j = GS_L - 1; j >= 0; --j) {
-        const bool r = st.reset >> j & 1, ok = j < st.live;
-        float ox[V], og[V];
+        float vx[V], vg[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float k = 1.f - low[v], Dt = e[j][v] + Rw[v], df = Dt * (h[j][v] - x[j][v]);
-          ox[v] = ok ? k * down[j][v] * Dt : 0.f;
-          og[v] = ok ? df * k * up[j][v] * down[j][v] : 0.f;
-          if (ok) {
-            dlow[v] += df * down[j][v];
-            Rw[v] = r ? 0.f : (low[v] + k * up[j][v]) * Dt;
+        for (int v = 0; v < V; ++v) { vx[v] = 0.f; vg[v] = 0.f; }
+        if (j < now) {
+          const bool r = fresh >> j & 1;
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            const float Dt = e[j][v] + Rw[v], df = Dt * (h[j][v] - x[j][v]) * down[j][v];
+            vx[v] = k[v] * down[j][v] * Dt;
+            vg[v] = k[v] * df * up[j][v];
+            dlow[v] += df;
+            Rw[v] = r ? 0.f : (low[v] + k[v] * up[j][v]) * Dt;
           }
         }
-        if (on && t0 + j < Tn) {
-          stv<T, V>(dxr + (t0 + j) * p.d.dx_t, ox);
-          stv<T, V>(dgr + (t0 + j) * p.d.dg_t, og);
+        if (tn + j < p.d.T && q.on) {
+          Raw<T, V>::store(ox + j * p.d.dx_t + q.c, vx);
+          Raw<T, V>::store(og + j * p.d.dg_t + q.c, vg);
         }
+      }
+      if (W == 1) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) R[v] = Rw[v];
       }
     }
   }
+  const int64_t chunk_at = ((int64_t)q.b * p.nc + q.chunk) * D + q.c;
   if constexpr (!OUT) {
 #pragma unroll
     for (int v = 0; v < V; ++v) { sP[wave][lane * V + v] = P[v]; sR[wave][lane * V + v] = R[v]; }
     __syncthreads();
-    if (wave == 0 && on) {
+    (void)sL;
+    if (wave == 0 && q.on) {
       float t[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) t[v] = 0.f;
@@ -403,16 +504,16 @@ __global__ __launch_bounds__(512) void gated_scan_bwd_kernel(GsP p) {
       for (int v = 0; v < V; ++v) p.rev_l[chunk_at + v] = t[v];
     }
   } else {
-    if (p.d_h0 && p.nc == 1 && wave == 0 && on) {
+    if (p.d_h0 && q.chunk == 0 && wave == 0 && q.on) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) p.d_h0[(int64_t)b * D + c + v] = R[v];
+      for (int v = 0; v < V; ++v) p.d_h0[(int64_t)q.b * D + q.c + v] = R[v];
     }
     if (p.floor_part) {
       __syncthreads();
 #pragma unroll
       for (int v = 0; v < V; ++v) sP[wave][lane * V + v] = dlow[v];
       __syncthreads();
-      if (wave == 0 && on) {
+      if (wave == 0 && q.on) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           float s = 0.f;
@@ -479,7 +580,7 @@ extern "C" int tg_gated_scan_sizes(int B, int T, int D, int64_t* carry_floats, i
   TG_CHECK_ARG(sizes_ok(B, T, D), "B >= 0, T >= 1, D >= 0 and B * ceil(D / 64) < 2^20 are wanted");
   const Plan pl = plan_of(B, T, D);
   *carry_floats = tile_floats(pl, B, D) + (pl.nc > 1 ? 2 * chunk_floats(pl, B, D) : 0);
-  *ws_floats = chunk_floats(pl, B, D) * (pl.nc > 1 ? 3 : 1);
+  *ws_floats = chunk_floats(pl, B, D) * (pl.nc > 1 ? 2 : 1);
   return TG_OK;
 }
 
@@ -529,7 +630,7 @@ extern "C" int tg_gated_scan_forward(const tg_gated_scan_desc* d, const void* x,
   GsP p = {};
   p.d = *d;
   p.x = x; p.g = g; p.h0 = h0; p.floor = floor; p.lengths = lengths; p.reset = reset; p.y = y; p.hT = hT;
-  p.keep_tiles = keep;
+  p.keep_tiles = keep != 0;
   set_plan(&p, pl, V, carry);
   const double n = (double)d->B * d->T * d->D;
   const int64_t blocks = (int64_t)p.ncb * p.nc * d->B;
@@ -537,7 +638,6 @@ extern "C" int tg_gated_scan_forward(const tg_gated_scan_desc* d, const void* x,
     const char* const name = "gated_scan_fwd<map>";
     const double flops = 10 * n, bytes = 2 * es * n;
     GS_PICK(gated_scan_fwd_kernel, false, (unsigned)blocks);
-    hipLaunchKernelGGL(gated_scan_carry_kernel, dim3((unsigned)cdiv64((int64_t)d->B * d->D, 64)), dim3(64), 0, ST(stream), p);
   }
   const char* const name = "gated_scan_fwd";
   const double flops = 14 * n, bytes = 3 * es * n;
@@ -560,7 +660,7 @@ extern "C" int tg_gated_scan_backward(const tg_gated_scan_desc* d, const void* x
     TG_CHECK_ARG(d->x_t >= d->D && d->g_t >= d->D && d->dx_t >= d->D && d->dg_t >= d->D && (!d_y || d->dy_t >= d->D), "a step stride below D");
     const int64_t need = tile_floats(pl, d->B, d->D) + (pl.nc > 1 ? 2 * chunk_floats(pl, d->B, d->D) : 0);
     TG_CHECK_ARG(carry != nullptr && carry_floats >= need && al(carry, 16), "the carry of the forward pass is missing");
-    const int64_t cf = chunk_floats(pl, d->B, d->D), want = cf * (pl.nc > 1 ? 3 : 1);
+    const int64_t cf = chunk_floats(pl, d->B, d->D), want = cf * (pl.nc > 1 ? 2 : 1);
     TG_CHECK_ARG((pl.nc == 1 && !d_floor) || (ws != nullptr && ws_floats >= want && al(ws, 16)), "a workspace of tg_gated_scan_sizes() floats is missing");
     const int es = d->dtype == TG_F32 ? 4 : 2;
     const bool even = d->D % 2 == 0 && al(x, 2 * es) && al(g, 2 * es) && al(d_y, 2 * es) && al(d_x, 2 * es) && al(d_g, 2 * es) &&
@@ -573,17 +673,13 @@ extern "C" int tg_gated_scan_backward(const tg_gated_scan_desc* d, const void* x
     p.d_x = d_x; p.d_g = d_g; p.d_h0 = d_h0;
     set_plan(&p, pl, V, const_cast<float*>(carry));                // only read by this pass
     p.floor_part = d_floor ? ws : nullptr;
-    if (pl.nc > 1) {
-      p.rev_l = ws + cf;
-      p.rev_in = ws + 2 * cf;
-    }
+    if (pl.nc > 1) p.rev_l = ws + cf;
     const double n = (double)d->B * d->T * d->D;
     const int64_t blocks = (int64_t)p.ncb * p.nc * d->B;
     if (pl.nc > 1) {
       const char* const name = "gated_scan_bwd<map>";
       const double flops = 12 * n, bytes = 2 * es * n;
       GS_PICK(gated_scan_bwd_kernel, false, (unsigned)blocks);
-      hipLaunchKernelGGL(gated_scan_rcarry_kernel, dim3((unsigned)cdiv64((int64_t)d->B * d->D, 64)), dim3(64), 0, ST(stream), p);
     }
     const char* const name = "gated_scan_bwd";
     const double flops = 40 * n, bytes = 5 * es * n;
