@@ -11,7 +11,7 @@
 // and the second one's workgroups compose the maps in front of their chunk (behind it, backward) before they begin: x and g are
 // read twice, the second time from the chunk that was read last on, so that the memory-side cache still holds most of them.
 // About 14 / 50 operations a value: bound by HBM.  States, maps and gradient sums are fp32; 1 - f is (1 - floor) sigmoid(-g), not a
-// difference.  The forward pass keeps the state before every tile (fp32, 1 value in 64): the backward pass makes the states of a tile
+// difference.  The forward pass keeps the state before every tile (fp32, 1 value in 32): the backward pass makes the states of a tile
 // again from it instead of reading rounded ones.
 //
 // A reset (a new sequence begins at step t) drops the state by selection, not by a product with 0: what was in it, NaN included,
@@ -22,7 +22,8 @@
 namespace {
 
 constexpr int GS_L = 8;                                            // steps of a wave in a tile
-constexpr int GS_MAXW = 8;
+constexpr int GS_MAXW = 4;                                         // waves of a workgroup: two small ones on a unit cover each other's
+                                                                   // barriers (backward pass 128 us with 8 waves, 109 us with 4)
 
 struct GsP {
   tg_gated_scan_desc d;
@@ -92,6 +93,34 @@ __device__ __forceinline__ void compose(float& P, float& L, float P2, float L2) 
   L = apply(P2, L2, L);
   P = P < 0.f || P2 < 0.f ? -1.f : P * P2;
 }
+
+// The waves' maps of a tile, read at once (the chain over them waits for LDS one time); where there are fewer than 4 waves the others'
+// places hold the identity.
+template <int V>
+struct Maps {
+  float P[GS_MAXW][V], L[GS_MAXW][V];
+  __device__ __forceinline__ void read(float (*sP)[64 * V], float (*sL)[64 * V], int lane, int W) {
+#pragma unroll
+    for (int w = 0; w < GS_MAXW; ++w)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        P[w][v] = sP[w < W ? w : 0][lane * V + v];
+        L[w][v] = sL[w < W ? w : 0][lane * V + v];
+      }
+#pragma unroll
+    for (int w = 1; w < GS_MAXW; ++w)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if (w >= W) { P[w][v] = 1.f; L[w][v] = 0.f; }
+      }
+  }
+  __device__ __forceinline__ void read_l(float (*sL)[64 * V], int lane, int W) {
+#pragma unroll
+    for (int w = 0; w < GS_MAXW; ++w)
+#pragma unroll
+      for (int v = 0; v < V; ++v) L[w][v] = w < W ? sL[w < W ? w : 0][lane * V + v] : 0.f;
+  }
+};
 
 // What the kernels know of their place: channels, chunk, steps.  Everything but the channel is the same for a whole wave.
 template <int V>
@@ -169,7 +198,7 @@ __device__ __forceinline__ void enter(const GsP& p, const Place<V>& q, const flo
 
 // Forward.  OUT false: the chunk's map only (each wave a contiguous part of it); true: states and outputs.
 template <typename T, int V, bool OUT>
-__global__ __launch_bounds__(512) void gated_scan_fwd_kernel(GsP p) {
+__global__ __launch_bounds__(256) void gated_scan_fwd_kernel(GsP p) {
   __shared__ float sP[GS_MAXW][64 * V], sL[GS_MAXW][64 * V];
   const Place<V> q(p, OUT ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x);
   const int W = p.W, D = p.d.D, lane = q.lane, wave = q.wave;
@@ -266,13 +295,15 @@ __global__ __launch_bounds__(512) void gated_scan_fwd_kernel(GsP p) {
         for (int v = 0; v < V; ++v) st[v] = H[v];
       }
       if (W > 1) {
-        for (int w = 0; w < W; ++w) {
+        Maps<V> m;
+        m.read(sP, sL, lane, W);
+#pragma unroll
+        for (int w = 0; w < GS_MAXW; ++w)
 #pragma unroll
           for (int v = 0; v < V; ++v) {
             if (w == wave) h[v] = H[v];
-            H[v] = apply(sP[w][lane * V + v], sL[w][lane * V + v], H[v]);
+            H[v] = apply(m.P[w][v], m.L[w][v], H[v]);
           }
-        }
       }
       T* const out = yr + tn * p.d.y_t;
 #pragma unroll
@@ -317,7 +348,7 @@ __global__ __launch_bounds__(512) void gated_scan_fwd_kernel(GsP p) {
 
 // Backward.  OUT false: what a chunk adds to the gradient that leaves it in front; true: the gradients.
 template <typename T, int V, bool OUT>
-__global__ __launch_bounds__(512) void gated_scan_bwd_kernel(GsP p) {
+__global__ __launch_bounds__(256) void gated_scan_bwd_kernel(GsP p) {
   __shared__ float sP[GS_MAXW][64 * V], sL[GS_MAXW][64 * V], sR[GS_MAXW][64 * V];
   const Place<V> q(p, OUT ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x);
   const int W = p.W, D = p.d.D, lane = q.lane, wave = q.wave;
@@ -430,19 +461,23 @@ __global__ __launch_bounds__(512) void gated_scan_bwd_kernel(GsP p) {
           sR[wave][lane * V + v] = Lr[v];
         }
         __syncthreads();
-        for (int w = 0; w < wave; ++w) {
+        Maps<V> m;
+        m.read(sP, sL, lane, W);
 #pragma unroll
-          for (int v = 0; v < V; ++v) H[v] = apply(sP[w][lane * V + v], sL[w][lane * V + v], H[v]);
-        }
+        for (int w = 0; w < GS_MAXW; ++w)
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+            if (w < wave) H[v] = apply(m.P[w][v], m.L[w][v], H[v]);
+        m.read_l(sR, lane, W);
 #pragma unroll
         for (int v = 0; v < V; ++v) Rw[v] = R[v];
-        for (int w = W - 1; w >= 0; --w) {
+#pragma unroll
+        for (int w = GS_MAXW - 1; w >= 0; --w)
 #pragma unroll
           for (int v = 0; v < V; ++v) {
             if (w == wave) Rw[v] = R[v];
-            R[v] = apply(sP[w][lane * V + v], sR[w][lane * V + v], R[v]);
+            R[v] = apply(m.P[w][v], m.L[w][v], R[v]);
           }
-        }
       } else {
 #pragma unroll
         for (int v = 0; v < V; ++v) Rw[v] = R[v];
@@ -546,18 +581,31 @@ __global__ __launch_bounds__(1024) void gated_scan_floor_kernel(const float* __r
 struct Plan {
   int W, tile, ntiles, nc, tpc;
 };
-// Waves of a tile by the sequence's length; chunks by how many workgroups the channels alone give (128 channels each): about 1024
-// workgroups fill the device.
+// Waves of a tile by the sequence's length.  Chunks: the time goes as tiles of a chunk x rounds of 512 workgroups (two a compute unit:
+// 128 channels x one chunk each; fewer than four a unit reach about 1 / 1.3 of the bandwidth) x bytes a value (3 tensors in one pass,
+// 5 in two), and the second launch of a chunked pass costs about as much as 13 of these units (measured: a tile and a round about
+// 0.8 us, a launch with its gap 4 us).  The fewest chunks at the least of it.
 Plan plan_of(int64_t B, int64_t T, int64_t D) {
   Plan p;
-  p.W = T <= 8 ? 1 : (T <= 16 ? 2 : (T <= 32 ? 4 : 8));
+  p.W = T <= 8 ? 1 : (T <= 16 ? 2 : 4);
   p.tile = p.W * GS_L;
   p.ntiles = (int)cdiv64(T, p.tile);
   const int64_t units = B * cdiv64(D, 128);
-  int64_t nc = units >= 1024 || units == 0 ? 1 : cdiv64(1024, units);
-  if (nc > p.ntiles) nc = p.ntiles;
-  p.tpc = (int)cdiv64(p.ntiles, nc);
-  p.nc = (int)cdiv64(p.ntiles, p.tpc);
+  double best = 0.0;
+  p.nc = p.tpc = 0;
+  for (int64_t n = 1; n <= p.ntiles; ++n) {
+    const int64_t tpc = cdiv64(p.ntiles, n), blocks = units * n;
+    if (n > 1 && (blocks > 4096 || cdiv64(p.ntiles, tpc) != n)) {  // enough workgroups, or the same split as a smaller n
+      if (blocks > 4096) break;
+      continue;
+    }
+    const double cost = (double)tpc * cdiv64(blocks, 512) * (blocks < 1024 ? 1.3 : 1.0) * (n == 1 ? 3 : 5) + (n == 1 ? 0 : 13);
+    if (p.nc == 0 || cost < best) {
+      best = cost;
+      p.nc = (int)n;
+      p.tpc = (int)tpc;
+    }
+  }
   return p;
 }
 

@@ -559,7 +559,6 @@ def frame_to_u8(frame, out, bgr=False):
 # ---- sequence-block operators: gated residual norm, block-scaled fp8 product, gated linear recurrence ------------------------------
 # Beside the functions above: rows may have a stride, shapes and types are checked here (TecoHipError), and a call belongs to the
 # current device: tensors of another one are refused.
-_FLOATS = {torch.float32: TG_F32, torch.bfloat16: TG_BF16}
 _FP8 = {torch.float8_e4m3fn: TG_FP8_E4M3, torch.float8_e5m2: TG_FP8_E5M2}
 FP8_DTYPES = {"e4m3": torch.float8_e4m3fn, "e5m2": torch.float8_e5m2}
 
@@ -571,12 +570,17 @@ def _need(ok, what):
 
 def _on_device(*ts):
     """Every tensor on the current device (None: not given); the raw handle of its current stream."""
-    dev = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    dev = -1
     for t in ts:
         if t is not None:
-            _need(t.is_cuda, "tensor is not on the GPU: tecogan_amd has no CPU path")
-            _need(t.get_device() == dev, "tensor is on another device than the current one")
-    return torch.cuda.current_stream().cuda_stream
+            d = t.get_device()
+            if d < 0:
+                raise L.TecoHipError("tensor is not on the GPU: tecogan_amd has no CPU path")
+            if dev < 0:
+                dev = torch.cuda.current_device()
+            if d != dev:
+                raise L.TecoHipError("tensor is on another device than the current one")
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _at(t):
@@ -587,13 +591,14 @@ def _rows(t, rows, C, dtype, what):
     """Pointer and row stride of `t`, [..., C] with `rows` rows: contiguous channels, one stride between its rows."""
     if t is None:
         return None, 0
-    _need(t.dtype == dtype, "%s: %s expected, got %s" % (what, dtype, t.dtype))
-    _need(t.dim() >= 1 and t.shape[-1] == C and t.numel() == rows * C, "%s: %d rows of %d expected, got %s" % (what, rows, C, tuple(t.shape)))
-    if t.is_contiguous():
+    shape = t.shape
+    if t.dtype is dtype and t.is_contiguous() and shape and shape[-1] == C and t.numel() == rows * C:
         return t.data_ptr(), C
+    _need(t.dtype == dtype, "%s: %s expected, got %s" % (what, dtype, t.dtype))
+    _need(t.dim() >= 1 and shape[-1] == C and t.numel() == rows * C, "%s: %d rows of %d expected, got %s" % (what, rows, C, tuple(shape)))
     _need(t.stride(-1) == 1 or C == 1, "%s: the last dimension must be contiguous" % what)
     ld, n = None, 1                                        # innermost row dimension outwards
-    for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+    for size, stride in zip(reversed(shape[:-1]), reversed(t.stride()[:-1])):
         if size == 1:
             continue
         _need(ld is None or stride == ld * n, "%s: its rows have no common stride" % what)
@@ -607,17 +612,9 @@ def _rows(t, rows, C, dtype, what):
 def _vector(t, n, what, dtype=torch.float32):
     if t is None:
         return None
-    _need(t.dtype == dtype and t.numel() == n and t.is_contiguous(), "%s: %d contiguous values of %s expected" % (what, n, dtype))
+    if t.dtype is not dtype or t.numel() != n or not t.is_contiguous():
+        raise L.TecoHipError("%s: %d contiguous values of %s expected" % (what, n, dtype))
     return t.data_ptr()
-
-
-def _norm_desc(x, o, gate, rows, Cn, post, pre, alpha, gate_act, rows_per_gate, eps):
-    rdt = _FLOATS.get(x.dtype)
-    _need(rdt is not None, "unsupported dtype %s" % x.dtype)
-    d = L.GatedNormDesc()
-    d.rows, d.rows_per_gate, d.C, d.res_dtype, d.post, d.pre = rows, rows_per_gate, Cn, rdt, post, pre
-    d.gate_act, d.alpha, d.eps = gate_act, alpha, eps
-    return d
 
 
 def _gate_rows(rows, rows_per_gate):
@@ -638,13 +635,13 @@ def gated_norm_forward(x, o, gate, y, h, post=NORM_NONE, pre=NORM_RMS, w_post=No
     rows = x.numel() // Cn
     like = o if o is not None else h
     _need(like is not None, "nothing to do: neither a block output nor a pre norm")
-    d = _norm_desc(x, o, gate, rows, Cn, post, pre, alpha, gate_act, rows_per_gate, eps)
-    d.dtype = dt(like)
-    px, d.ldx = _rows(x, rows, Cn, x.dtype, "x")
-    po, d.ldo = _rows(o, rows, Cn, like.dtype, "o")
-    pg, d.ldg = _rows(gate, _gate_rows(rows, rows_per_gate), Cn, like.dtype, "gate")
-    py, d.ldy = _rows(y, rows, Cn, x.dtype, "y")
-    ph, d.ldh = _rows(h, rows, Cn, like.dtype, "h")
+    dtx, dto = x.dtype, like.dtype
+    px, ldx = _rows(x, rows, Cn, dtx, "x")
+    po, ldo = _rows(o, rows, Cn, dto, "o")
+    pg, ldg = _rows(gate, _gate_rows(rows, rows_per_gate), Cn, dto, "gate")
+    py, ldy = _rows(y, rows, Cn, dtx, "y")
+    ph, ldh = _rows(h, rows, Cn, dto, "h")
+    d = L.GatedNormDesc(rows, rows_per_gate, ldx, ldo, ldg, ldy, ldh, 0, 0, 0, Cn, dt(like), dt(x), post, pre, gate_act, alpha, eps)
     check(lib().tg_gated_norm_forward(C.byref(d), px, po, pg, _vector(w_post, Cn, "w_post"), _vector(b_post, Cn, "b_post"),
                                       _vector(scale, Cn, "scale"), _vector(w_pre, Cn, "w_pre"), _vector(b_pre, Cn, "b_pre"), py, ph, stream),
           "tg_gated_norm_forward")
@@ -669,17 +666,17 @@ def gated_norm_backward(d_y, d_h, y, o, gate, d_x, d_o, d_gate, ws, post=NORM_NO
     _need(Cn >= 1, "y: [..., C] with C >= 1 expected")
     rows = y.numel() // Cn
     like = o if o is not None else (d_h if d_h is not None else y)
-    d = _norm_desc(y, o, gate, rows, Cn, post, pre, alpha, gate_act, rows_per_gate, eps)
-    d.dtype = dt(like)
+    dtx, dto = y.dtype, like.dtype
     groups = _gate_rows(rows, rows_per_gate)
-    pdy, d.ld_dy = _rows(d_y, rows, Cn, y.dtype, "d_y")
-    pdh, d.ldh = _rows(d_h, rows, Cn, like.dtype, "d_h")
-    py, d.ldy = _rows(y, rows, Cn, y.dtype, "y")
-    po, d.ldo = _rows(o, rows, Cn, like.dtype, "o")
-    pg, d.ldg = _rows(gate, groups, Cn, like.dtype, "gate")
-    pdx, d.ldx = _rows(d_x, rows, Cn, y.dtype, "d_x")
-    pdo, d.ld_do = _rows(d_o, rows, Cn, like.dtype, "d_o")
-    pdg, d.ld_dg = _rows(d_gate, groups, Cn, like.dtype, "d_gate")
+    pdy, ld_dy = _rows(d_y, rows, Cn, dtx, "d_y")
+    pdh, ldh = _rows(d_h, rows, Cn, dto, "d_h")
+    py, ldy = _rows(y, rows, Cn, dtx, "y")
+    po, ldo = _rows(o, rows, Cn, dto, "o")
+    pg, ldg = _rows(gate, groups, Cn, dto, "gate")
+    pdx, ldx = _rows(d_x, rows, Cn, dtx, "d_x")
+    pdo, ld_do = _rows(d_o, rows, Cn, dto, "d_o")
+    pdg, ld_dg = _rows(d_gate, groups, Cn, dto, "d_gate")
+    d = L.GatedNormDesc(rows, rows_per_gate, ldx, ldo, ldg, ldy, ldh, ld_dy, ld_do, ld_dg, Cn, dt(like), dt(y), post, pre, gate_act, alpha, eps)
     _need(ws is not None and ws.dtype == torch.float32 and ws.is_contiguous(), "ws: contiguous fp32 values expected")
     v = _vector
     check(lib().tg_gated_norm_backward(C.byref(d), pdy, pdh, py, po, pg, v(w_post, Cn, "w_post"), v(b_post, Cn, "b_post"),
@@ -708,12 +705,14 @@ def fp8_alloc(rows, cols, device, fmt="e4m3", tile=False, transposed=False):
 def _fp8_operand(q, s, what):
     """(format, rows, padded columns, scales per tile) of an operand, checked."""
     fmt = _FP8.get(q.dtype)
-    _need(fmt is not None, "%s: float8_e4m3fn or float8_e5m2 expected, got %s" % (what, q.dtype))
-    _need(q.dim() == 2 and q.is_contiguous() and q.shape[1] % 128 == 0, "%s: contiguous [rows, columns padded to 128] expected" % what)
+    if fmt is None:
+        raise L.TecoHipError("%s: float8_e4m3fn or float8_e5m2 expected, got %s" % (what, q.dtype))
+    if q.dim() != 2 or not q.is_contiguous() or q.shape[1] % 128:
+        raise L.TecoHipError("%s: contiguous [rows, columns padded to 128] expected" % what)
     rows, cols = q.shape
-    pitch = -(-(cols // 128) // 4) * 4
-    _need(s.dtype == torch.uint8 and s.is_contiguous() and s.dim() == 2 and s.shape[1] == pitch and s.shape[0] in (rows, -(-rows // 128)),
-          "%s: its scales must be contiguous uint8 [%d or %d, %d], got %s" % (what, rows, -(-rows // 128), pitch, tuple(s.shape)))
+    pitch, tiles = -(-cols // 512) * 4, -(-rows // 128)
+    if s.dtype is not torch.uint8 or not s.is_contiguous() or s.dim() != 2 or s.shape[1] != pitch or s.shape[0] not in (rows, tiles):
+        raise L.TecoHipError("%s: its scales must be contiguous uint8 [%d or %d, %d], got %s" % (what, rows, tiles, pitch, tuple(s.shape)))
     return fmt, rows, cols, int(s.shape[0] != rows)
 
 
@@ -744,13 +743,12 @@ def fp8_matmul(a, scale_a, b, scale_b, out, bias=None, accumulate=False):
     """out [M, N] (bf16 / f32) = a [M, K] b [N, K]^T (+ bias fp32 [N]) (+ out): operands and scales as fp8_quantize writes them, the
     scales of each per row or per tile (by their shape).  fp32 sums; accumulate: f32 outputs only."""
     stream = _on_device(a, scale_a, b, scale_b, out, bias)
-    d = L.Fp8MatmulDesc()
-    d.a_fmt, M, K, d.a_tile = _fp8_operand(a, scale_a, "a")
-    d.b_fmt, N, Kb, d.b_tile = _fp8_operand(b, scale_b, "b")
-    _need(K == Kb, "a and b differ in their padded columns: %d and %d" % (K, Kb))
-    d.M, d.N, d.K = M, N, K
-    po, d.ldo = _rows(out, M, N, out.dtype, "out")
-    d.out_dtype, d.accumulate = dt(out), int(bool(accumulate))
+    a_fmt, M, K, a_tile = _fp8_operand(a, scale_a, "a")
+    b_fmt, N, Kb, b_tile = _fp8_operand(b, scale_b, "b")
+    if K != Kb:
+        raise L.TecoHipError("a and b differ in their padded columns: %d and %d" % (K, Kb))
+    po, ldo = _rows(out, M, N, out.dtype, "out")
+    d = L.Fp8MatmulDesc(M, N, K, ldo, a_fmt, b_fmt, a_tile, b_tile, dt(out), int(bool(accumulate)))
     check(lib().tg_fp8_matmul(C.byref(d), a.data_ptr(), scale_a.data_ptr(), b.data_ptr(), scale_b.data_ptr(), _vector(bias, N, "bias"), po,
                               stream), "tg_fp8_matmul")
     return out
@@ -801,7 +799,8 @@ def _steps(t, shape, dtype, what):
     """Pointer and strides (step, batch row) of a [B, T, D] tensor with contiguous channels."""
     if t is None:
         return None, 0, 0
-    _need(tuple(t.shape) == shape and t.dtype == dtype, "%s: %s of %s expected, got %s of %s" % (what, shape, dtype, tuple(t.shape), t.dtype))
+    if t.shape != shape or t.dtype is not dtype:
+        raise L.TecoHipError("%s: %s of %s expected, got %s of %s" % (what, shape, dtype, tuple(t.shape), t.dtype))
     B, T, D = shape
     sb, st, sd = t.stride()
     _need(sd == 1 or D == 1, "%s: channels must be contiguous" % what)
@@ -829,11 +828,10 @@ def gated_scan_forward(x, g, y, hT, carry, h0=None, floor=None, lengths=None, re
     _need(x.dim() == 3 and x.shape[1] >= 1, "x: [B, T, D] with T >= 1 expected")
     shape = tuple(x.shape)
     B, T, D = shape
-    d = L.GatedScanDesc()
-    d.B, d.T, d.D, d.dtype = B, T, D, dt(x)
-    px, d.x_t, d.x_b = _steps(x, shape, x.dtype, "x")
-    pg, d.g_t, d.g_b = _steps(g, shape, x.dtype, "g")
-    py, d.y_t, d.y_b = _steps(y, shape, x.dtype, "y")
+    px, x_t, x_b = _steps(x, shape, x.dtype, "x")
+    pg, g_t, g_b = _steps(g, shape, x.dtype, "g")
+    py, y_t, y_b = _steps(y, shape, x.dtype, "y")
+    d = L.GatedScanDesc(x_t, x_b, g_t, g_b, y_t, y_b, 0, 0, 0, 0, 0, 0, B, T, D, dt(x))
     pl, pr = _scan_masks(B, T, lengths, reset)
     n = 0 if carry is None else carry.numel()
     check(lib().tg_gated_scan_forward(C.byref(d), px, pg, _vector(h0, B * D, "h0"), _vector(floor, D, "floor"), pl, pr, py,
@@ -850,13 +848,12 @@ def gated_scan_backward(x, g, d_y, d_hT, carry, d_x, d_g, ws, h0=None, floor=Non
     _need(d_h0 is None or h0 is not None, "d_h0 without h0")
     shape = tuple(x.shape)
     B, T, D = shape
-    d = L.GatedScanDesc()
-    d.B, d.T, d.D, d.dtype = B, T, D, dt(x)
-    px, d.x_t, d.x_b = _steps(x, shape, x.dtype, "x")
-    pg, d.g_t, d.g_b = _steps(g, shape, x.dtype, "g")
-    pe, d.dy_t, d.dy_b = _steps(d_y, shape, x.dtype, "d_y")
-    pdx, d.dx_t, d.dx_b = _steps(d_x, shape, x.dtype, "d_x")
-    pdg, d.dg_t, d.dg_b = _steps(d_g, shape, x.dtype, "d_g")
+    px, x_t, x_b = _steps(x, shape, x.dtype, "x")
+    pg, g_t, g_b = _steps(g, shape, x.dtype, "g")
+    pe, dy_t, dy_b = _steps(d_y, shape, x.dtype, "d_y")
+    pdx, dx_t, dx_b = _steps(d_x, shape, x.dtype, "d_x")
+    pdg, dg_t, dg_b = _steps(d_g, shape, x.dtype, "d_g")
+    d = L.GatedScanDesc(x_t, x_b, g_t, g_b, 0, 0, dy_t, dy_b, dx_t, dx_b, dg_t, dg_b, B, T, D, dt(x))
     pl, pr = _scan_masks(B, T, lengths, reset)
     _need(carry is not None, "the carry of the forward pass is missing")
     n, m = carry.numel(), 0 if ws is None else ws.numel()

@@ -102,11 +102,11 @@ def test_gated_scan_refuses():
     big = 1 << 30
     for kw, word in ((dict(T=0), "T >= 1"), (dict(B=-1), "B >= 0"), (dict(dtype=2), "dtype"), (dict(x_t=63), "stride"), (dict(y_t=0), "stride")):
         refused(f(C.byref(desc(**kw)), P, P, None, None, None, None, P, None, P, big, 1, None), word)
-    refused(f(C.byref(desc()), P, P, None, None, None, None, P, None, None, 0, 0, None), "carry")
+    refused(f(C.byref(desc(T=1 << 20)), P, P, None, None, None, None, P, None, None, 0, 0, None), "carry")
     refused(f(C.byref(desc(T=3)), P, P, None, None, None, None, P, None, None, 0, 1, None), "carry")
     refused(f(C.byref(desc()), P, None, None, None, None, None, P, None, P, big, 1, None), "missing")
     refused(b(C.byref(desc()), P, P, None, None, None, P, None, None, big, P, P, None, None, P, big, None), "carry")
-    refused(b(C.byref(desc()), P, P, None, None, None, P, None, P, big, P, P, None, None, P, 8, None), "workspace")
+    refused(b(C.byref(desc(T=1 << 20)), P, P, None, None, None, P, None, P, big, P, P, None, None, P, 8, None), "workspace")
     refused(b(C.byref(desc()), P, P, None, None, None, P, None, P, big, P, P, None, P, P, big, None), "floor")
     refused(b(C.byref(desc(dx_t=1)), P, P, None, None, None, P, None, P, big, P, P, None, None, P, big, None), "stride")
 
