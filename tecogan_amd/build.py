@@ -23,7 +23,7 @@ def _newer(a, b):
 
 def build(force=False, verbose=True):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    deps = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "handoff.h"), os.path.join(HERE, "..", "include", "tecogan_hip.h")]
+    deps = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "handoff.h"), os.path.join(CSRC, "fp8.h"), os.path.join(HERE, "..", "include", "tecogan_hip.h")]
     objs, procs = [], []
     for src in SOURCES:
         s = os.path.join(CSRC, src)

@@ -15,7 +15,7 @@
 //     promises (a weight gradient that is accumulated).
 //
 // The instruction's rows are n and its columns m: a lane holds four neighbouring n of one m.
-#include "common.h"
+#include "fp8.h"
 #include <type_traits>
 
 namespace {
@@ -311,6 +311,126 @@ void launch_formats(const MmP& p, const char* name, double flops, double bytes, 
   else launch_tile<FB, FA, WIDE, 2, 2>(p, name, flops, bytes, st);
 }
 
+// Few rows of a: 16 columns n of the output for a workgroup, all M (at most 16 MF) rows.  Here the weight's bytes count: every wave
+// streams its blocks of K (wave w those with kb % 8 = w: the waves of a workgroup read 1 KB of a row together) from memory straight
+// into the operand's registers, four blocks in flight, and the waves' sums meet in LDS in a fixed order.  Both operands are widened to
+// bf16 (there is time: fp32 sums for either output type).
+// SRC: where a comes from -- 0, 1: 8-bit e4m3 / e5m2; 2, 3: bf16 / f32 values that are quantised here, as tg_fp8_quantize does it (at
+// most 16 rows: one launch instead of two).
+template <int SRC> struct SkinnyA { static constexpr int FMT = SRC == 1 ? 1 : 0; };
+
+struct SkP {
+  MmP m;
+  const void* x;
+  int64_t ldx;
+  int cols, xvec;                                                     // columns of x before padding
+};
+
+constexpr int SK_WAVES = 8, SK_AHEAD = 4;
+
+template <int FB, int SRC, int MF>
+__global__ __launch_bounds__(64 * SK_WAVES) void fp8_skinny_kernel(SkP s) {
+  const MmP& p = s.m;
+  __shared__ float join[SK_WAVES][MF][256];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g = lane >> 4;
+  const int64_t n0 = (int64_t)blockIdx.x * 16, n = n0 + r16 < p.N ? n0 + r16 : p.N - 1;
+  const int nkb = p.K >> 7;
+  const unsigned char* const pb = p.b + n * p.K + g * 16;
+  const unsigned char* const qb = p.sb + (n >> p.sh_b) * p.sp;
+  f32x4 acc[MF];
+#pragma unroll
+  for (int i = 0; i < MF; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int k0 = wave; k0 < nkb; k0 += SK_WAVES * SK_AHEAD) {
+    i32x4m wl[SK_AHEAD], wh[SK_AHEAD];
+    int ws[SK_AHEAD];
+#pragma unroll
+    for (int u = 0; u < SK_AHEAD; ++u) {
+      const int kb = k0 + u * SK_WAVES < nkb ? k0 + u * SK_WAVES : k0;   // past the end: loaded again, not used
+      wl[u] = *reinterpret_cast<const i32x4m*>(pb + kb * 128);
+      wh[u] = *reinterpret_cast<const i32x4m*>(pb + kb * 128 + 64);
+      ws[u] = qb[kb];
+    }
+#pragma unroll
+    for (int u = 0; u < SK_AHEAD; ++u) {
+      const int kb = k0 + u * SK_WAVES;
+      if (kb >= nkb) break;
+      const float sb = __int_as_float(ws[u] << 23);
+      bf16x8 b[4];
+      b[0] = widen<FB>(wl[u][0], wl[u][1], sb);
+      b[1] = widen<FB>(wl[u][2], wl[u][3], sb);
+      b[2] = widen<FB>(wh[u][0], wh[u][1], sb);
+      b[3] = widen<FB>(wh[u][2], wh[u][3], sb);
+#pragma unroll
+      for (int i = 0; i < MF; ++i) {
+        const int64_t m = 16 * i + r16 < p.M ? 16 * i + r16 : p.M - 1;
+        i32x4m lo, hi;
+        float sa;
+        if constexpr (SRC < 2) {
+          const unsigned char* const pa = p.a + m * p.K + kb * 128 + g * 16;
+          lo = *reinterpret_cast<const i32x4m*>(pa);
+          hi = *reinterpret_cast<const i32x4m*>(pa + 64);
+          sa = __int_as_float(p.sa[(m >> p.sh_a) * p.sp + kb] << 23);
+        } else {
+          using T = std::conditional_t<SRC == 2, u16, float>;
+          const T* const row = static_cast<const T*>(s.x) + m * s.ldx;
+          typename Fp8In<T>::type f[4];                                // chunks g and g + 4 of the block: 2 x 16 values
+          uint32_t most = 0;
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            const int c = kb * 128 + (h >> 1) * 64 + g * 16 + (h & 1) * 8, have = s.cols - c;
+            f[h].load(row + c, have < 0 ? 0 : (have > 8 ? 8 : have), s.xvec != 0);
+            most = max(most, f[h].most(false));
+          }
+          const bool bad = __any(most >= FP8_INF);
+          if (bad) most = max(max(f[0].most(true), f[1].most(true)), max(f[2].most(true), f[3].most(true)));
+          most = max(most, (uint32_t)__shfl_xor((int)most, 16, 64));    // the four lanes of a row
+          most = max(most, (uint32_t)__shfl_xor((int)most, 32, 64));
+          const uint32_t code = fp8_scale_code<TG_FP8_E4M3>(most);
+          sa = __uint_as_float(code << 23);
+          const uint2 w0 = f[0].template pack<TG_FP8_E4M3>(code, bad), w1 = f[1].template pack<TG_FP8_E4M3>(code, bad);
+          const uint2 w2 = f[2].template pack<TG_FP8_E4M3>(code, bad), w3 = f[3].template pack<TG_FP8_E4M3>(code, bad);
+          lo = i32x4m{(int)w0.x, (int)w0.y, (int)w1.x, (int)w1.y};
+          hi = i32x4m{(int)w2.x, (int)w2.y, (int)w3.x, (int)w3.y};
+        }
+        constexpr int FA = SkinnyA<SRC>::FMT;
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[0], widen<FA>(lo[0], lo[1], sa), acc[i], 0, 0, 0);
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[1], widen<FA>(lo[2], lo[3], sa), acc[i], 0, 0, 0);
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[2], widen<FA>(hi[0], hi[1], sa), acc[i], 0, 0, 0);
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[3], widen<FA>(hi[2], hi[3], sa), acc[i], 0, 0, 0);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < MF; ++i) *reinterpret_cast<f32x4*>(&join[wave][i][r16 * 16 + 4 * g]) = acc[i];   // [m][n]
+  __syncthreads();
+  for (int e = tid; e < MF * 256; e += 64 * SK_WAVES) {
+    const int64_t m = e >> 4, no = n0 + (e & 15);
+    if (m >= p.M || no >= p.N) continue;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < SK_WAVES; ++w) v += join[w][e >> 8][e & 255];
+    if (p.bias) v += p.bias[no];
+    if (p.out_bf16) {
+      static_cast<u16*>(p.out)[m * p.ldo + no] = f2bf(v);
+    } else {
+      float* const o = static_cast<float*>(p.out) + m * p.ldo + no;
+      *o = p.accumulate ? *o + v : v;
+    }
+  }
+}
+
+template <int FB, int SRC>
+void launch_skinny(const SkP& s, const char* name, double flops, double bytes, hipStream_t st) {
+  const dim3 grid((unsigned)cdiv64(s.m.N, 16)), block(64 * SK_WAVES);
+  const int mf = (int)cdiv64(s.m.M, 16);
+  if (mf <= 1) TG_LAUNCH(name, flops, bytes, (fp8_skinny_kernel<FB, SRC, 1>), grid, block, 0, st, s);
+  if constexpr (SRC < 2) {
+    if (mf == 2) TG_LAUNCH(name, flops, bytes, (fp8_skinny_kernel<FB, SRC, 2>), grid, block, 0, st, s);
+    if (mf > 2) TG_LAUNCH(name, flops, bytes, (fp8_skinny_kernel<FB, SRC, 4>), grid, block, 0, st, s);
+  }
+}
+constexpr int SK_ROWS = 64, SK_FUSED = 16;
+
 bool al16m(const void* p) { return ((uintptr_t)p & 15) == 0; }
 bool fmt_ok(int f) { return f == TG_FP8_E4M3 || f == TG_FP8_E5M2; }
 
@@ -347,6 +467,15 @@ extern "C" int tg_fp8_matmul(const tg_fp8_matmul_desc* d, const void* a, const v
   const int oe = p.out_bf16 ? 2 : 4;
   p.vec = d->N % 4 == 0 && ((uintptr_t)out & (4 * oe - 1)) == 0 && d->ldo % 4 == 0 && al16m(bias);
   const int fa = d->a_fmt == TG_FP8_E5M2, fb = d->b_fmt == TG_FP8_E5M2;
+  if (d->M <= SK_ROWS) {
+    SkP k = {};
+    k.m = p;
+    if (fa && fb) launch_skinny<1, 1>(k, "fp8_skinny", flops, bytes, ST(stream));
+    else if (fa) launch_skinny<0, 1>(k, "fp8_skinny", flops, bytes, ST(stream));
+    else if (fb) launch_skinny<1, 0>(k, "fp8_skinny", flops, bytes, ST(stream));
+    else launch_skinny<0, 0>(k, "fp8_skinny", flops, bytes, ST(stream));
+    TG_CHECK_LAUNCH();
+  }
 #define MM_PICK(WIDEV)                                                                     \
   do {                                                                                     \
     if (fa && fb) launch_formats<1, 1, WIDEV>(p, name, flops, bytes, ST(stream));          \
@@ -388,6 +517,31 @@ extern "C" int tg_fp8_linear(const void* x, int dtype, int64_t M, int64_t K, int
   d.a_fmt = TG_FP8_E4M3; d.b_fmt = w_fmt; d.b_tile = 1; d.out_dtype = out_dtype;
   TG_CHECK_ARG(fmt_ok(w_fmt) && w && scale_w && out && al16m(w) && ((uintptr_t)scale_w & 3) == 0 && ldo >= N &&
                    (out_dtype == TG_F32 || out_dtype == TG_BF16), "bad weight or output");
+  if (M <= SK_FUSED) {
+    TG_CHECK_ARG(x != nullptr && ldx >= K && (dtype == TG_F32 || dtype == TG_BF16), "x is missing, its type unknown or its row stride below K");
+    SkP k = {};
+    k.m.b = static_cast<const unsigned char*>(w); k.m.sb = static_cast<const unsigned char*>(scale_w);
+    k.m.bias = bias; k.m.out = out;
+    k.m.M = M; k.m.N = N; k.m.ldo = ldo;
+    k.m.K = (int)(kb * 128);
+    k.m.sp = (int)cdiv64(kb, 4) * 4;
+    k.m.sh_b = 7;
+    k.m.out_bf16 = out_dtype == TG_BF16;
+    k.x = x;
+    k.ldx = ldx;
+    k.cols = (int)K;
+    k.xvec = al16m(x) && (ldx * (dtype == TG_F32 ? 4 : 2)) % 16 == 0;
+    const double flops = 2.0 * M * N * K, bytes = (double)N * K + (double)M * K * (dtype == TG_F32 ? 4 : 2) + (double)M * N * (k.m.out_bf16 ? 2 : 4);
+    const char* const name = "fp8_skinny<quantise>";
+    if (dtype == TG_BF16) {
+      if (w_fmt == TG_FP8_E5M2) launch_skinny<1, 2>(k, name, flops, bytes, ST(stream));
+      else launch_skinny<0, 2>(k, name, flops, bytes, ST(stream));
+    } else {
+      if (w_fmt == TG_FP8_E5M2) launch_skinny<1, 3>(k, name, flops, bytes, ST(stream));
+      else launch_skinny<0, 3>(k, name, flops, bytes, ST(stream));
+    }
+    TG_CHECK_LAUNCH();
+  }
   const int rc = tg_fp8_quantize(x, dtype, M, K, ldx, TG_FP8_E4M3, 0, q, s, nullptr, nullptr, stream);
   if (rc != TG_OK) return rc;
   return tg_fp8_matmul(&d, q, s, w, scale_w, bias, out, stream);

@@ -9,63 +9,11 @@
 // One workgroup takes a 128 x 128 tile, 64 values a thread in registers: the matrix is read once for both orders that a training
 // step needs (blocks along the columns for y and dx, along the rows for dW), 2 + 1 + 1 bytes a value: bound by HBM.  The transposed
 // copy goes through LDS as bytes (rows of 144 bytes), so both copies are written as whole 128-byte lines.
-#include "common.h"
+#include "fp8.h"
 
 namespace {
 
 constexpr int FQ_PITCH = 144;
-
-template <typename T>
-__device__ __forceinline__ void load8q(const T* __restrict__ p, int have, bool vec, float (&f)[8]) {
-  if (vec && have >= 8) {
-    if constexpr (sizeof(T) == 2) {
-      bf8_unpack(*reinterpret_cast<const uint4*>(p), f);
-    } else {
-      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-      f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-      f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = k < have ? Elem<T>::ld(p + k) : 0.f;
-  }
-}
-
-__device__ __forceinline__ float finite_abs(float v) {
-  const float a = fabsf(v);
-  return a < __builtin_inff() ? a : 0.f;
-}
-
-// biased exponent of a block's scale
-template <int FMT>
-__device__ __forceinline__ uint32_t scale_code(float amax) {
-  const uint32_t b = __float_as_uint(amax);
-  if (b == 0) return 127;
-  const int e = (int)(b >> 23) - 127 - (FMT == TG_FP8_E4M3 ? 8 : 15) + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
-  return (uint32_t)((e < -126 ? -126 : e) + 127);
-}
-__device__ __forceinline__ float inverse_scale(uint32_t code) { return __uint_as_float((254u - code) << 23); }
-
-// four values -> four bytes; |v| <= largest(type) but for NaN and infinity
-template <int FMT>
-__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
-  int w = 0;
-  if constexpr (FMT == TG_FP8_E4M3) {
-    w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, w, false);
-    w = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
-  } else {
-    w = __builtin_amdgcn_cvt_pk_bf8_f32(a, b, w, false);
-    w = __builtin_amdgcn_cvt_pk_bf8_f32(c, d, w, true);
-  }
-  return (uint32_t)w;
-}
-
-// infinities of e4m3 become NaN before the conversion, so that nothing depends on its overflow mode
-template <int FMT>
-__device__ __forceinline__ float storable(float v) {
-  if (FMT == TG_FP8_E4M3 && fabsf(v) == __builtin_inff()) return __builtin_nanf("");
-  return v;
-}
 
 struct FqP {
   const void* x;
@@ -77,28 +25,41 @@ struct FqP {
 template <typename T, int FMT>
 __global__ __launch_bounds__(256) void fp8_quantize_kernel(FqP p) {
   __shared__ __attribute__((aligned(16))) unsigned char sh[128 * FQ_PITCH];
-  __shared__ float smax[4][128];
+  __shared__ uint32_t smax[4][128];
+  using In = typename Fp8In<T>::type;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, wave = tid >> 6;
   const int64_t tr = blockIdx.x / p.tiles_c, tc = blockIdx.x - tr * p.tiles_c;
   const int64_t r0 = tr * 128 + ty * 8, c0 = tc * 128 + tx * 8;
   const int have = p.cols - c0 >= 8 ? 8 : (p.cols - c0 > 0 ? (int)(p.cols - c0) : 0);
-  float v[8][8];
+  In v[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    load8q<T>(static_cast<const T*>(p.x) + (r0 + j) * p.ldx + c0, r0 + j < p.rows ? have : 0, p.vec != 0, v[j]);
-
+  for (int j = 0; j < 8; ++j) {
+    if (r0 + j < p.rows && have > 0) v[j].load(static_cast<const T*>(p.x) + (r0 + j) * p.ldx + c0, have, p.vec != 0);
+    else v[j].zero();
+  }
+  uint32_t mr[8], ma = 0;                                               // bits of the largest absolute value: of each row, of all
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    mr[j] = v[j].most(false);
+    ma = ma > mr[j] ? ma : mr[j];
+  }
+  const bool bad = __any(ma >= FP8_INF);
+  if (bad) {
+    ma = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      mr[j] = v[j].most(true);
+      ma = ma > mr[j] ? ma : mr[j];
+    }
+  }
   uint32_t code_tile = 0;
   if (p.tile) {
-    float m = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int k = 0; k < 8; ++k) m = fmaxf(m, finite_abs(v[j][k]));
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    if ((tid & 63) == 0) smax[wave][0] = m;
+    ma = fp8_max16(ma);
+    ma = max(ma, (uint32_t)__shfl_xor((int)ma, 16, 64));
+    ma = max(ma, (uint32_t)__shfl_xor((int)ma, 32, 64));
+    if ((tid & 63) == 0) smax[wave][0] = ma;
     __syncthreads();
-    m = fmaxf(fmaxf(smax[0][0], smax[1][0]), fmaxf(smax[2][0], smax[3][0]));
-    code_tile = scale_code<FMT>(m);
+    code_tile = fp8_scale_code<FMT>(max(max(smax[0][0], smax[1][0]), max(smax[2][0], smax[3][0])));
     if (tid == 0) {
       if (p.q) p.s[tr * p.sp + tc] = (unsigned char)code_tile;
       if (p.qt) p.st[tc * p.stp + tr] = (unsigned char)code_tile;
@@ -107,39 +68,40 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(FqP p) {
   if (p.q) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      uint32_t code = code_tile;
-      if (!p.tile) {
-        float m = 0.f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) m = fmaxf(m, finite_abs(v[j][k]));
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-        code = scale_code<FMT>(m);
-      }
-      const float i = inverse_scale(code);
+      const uint32_t code = p.tile ? code_tile : fp8_scale_code<FMT>(fp8_max16(mr[j]));
       if (r0 + j < p.rows) {
-        uint2 w;
-        w.x = pack4<FMT>(storable<FMT>(v[j][0] * i), storable<FMT>(v[j][1] * i), storable<FMT>(v[j][2] * i), storable<FMT>(v[j][3] * i));
-        w.y = pack4<FMT>(storable<FMT>(v[j][4] * i), storable<FMT>(v[j][5] * i), storable<FMT>(v[j][6] * i), storable<FMT>(v[j][7] * i));
-        *reinterpret_cast<uint2*>(p.q + (r0 + j) * p.cp + c0) = w;
+        *reinterpret_cast<uint2*>(p.q + (r0 + j) * p.cp + c0) = v[j].template pack<FMT>(code, bad);
         if (!p.tile && tx == 0) p.s[(r0 + j) * p.sp + tc] = (unsigned char)code;
       }
     }
   }
   if (p.qt) {
-    float inv[8];
+    uint32_t code[8];
     if (p.tile) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) inv[k] = inverse_scale(code_tile);
+      for (int k = 0; k < 8; ++k) code[k] = code_tile;
     } else {
-      float m[8];
+      uint32_t m[8];                                                    // of the 8 columns, over the wave's 32 rows
+      if constexpr (sizeof(T) == 2) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        m[k] = 0.f;
+        for (int k = 0; k < 4; ++k) {
+          u16x2q a = v[0].abs2(k, bad);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m[k] = fmaxf(m[k], finite_abs(v[j][k]));
-        m[k] = fmaxf(m[k], __shfl_xor(m[k], 16, 64));
-        m[k] = fmaxf(m[k], __shfl_xor(m[k], 32, 64));
+          for (int j = 1; j < 8; ++j) a = __builtin_elementwise_max(a, v[j].abs2(k, bad));
+          a = __builtin_elementwise_max(a, __builtin_bit_cast(u16x2q, __shfl_xor(__builtin_bit_cast(int, a), 16, 64)));
+          a = __builtin_elementwise_max(a, __builtin_bit_cast(u16x2q, __shfl_xor(__builtin_bit_cast(int, a), 32, 64)));
+          m[2 * k] = (uint32_t)a[0] << 16;
+          m[2 * k + 1] = (uint32_t)a[1] << 16;
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          m[k] = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) m[k] = max(m[k], v[j].abs1(k, bad));
+          m[k] = max(m[k], (uint32_t)__shfl_xor((int)m[k], 16, 64));
+          m[k] = max(m[k], (uint32_t)__shfl_xor((int)m[k], 32, 64));
+        }
       }
       if ((tid & 63) < 16) {
 #pragma unroll
@@ -149,16 +111,27 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(FqP p) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const int c = tx * 8 + k;
-        const uint32_t code = scale_code<FMT>(fmaxf(fmaxf(smax[0][c], smax[1][c]), fmaxf(smax[2][c], smax[3][c])));
-        inv[k] = inverse_scale(code);
-        if (ty == 0 && c0 + k < p.cols) p.st[(c0 + k) * p.stp + tr] = (unsigned char)code;
+        code[k] = fp8_scale_code<FMT>(max(max(smax[0][c], smax[1][c]), max(smax[2][c], smax[3][c])));
+        if (ty == 0 && c0 + k < p.cols) p.st[(c0 + k) * p.stp + tr] = (unsigned char)code[k];
       }
     }
+    const bool nan = bad && FMT == TG_FP8_E4M3;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       uint2 w;
-      w.x = pack4<FMT>(storable<FMT>(v[0][k] * inv[k]), storable<FMT>(v[1][k] * inv[k]), storable<FMT>(v[2][k] * inv[k]), storable<FMT>(v[3][k] * inv[k]));
-      w.y = pack4<FMT>(storable<FMT>(v[4][k] * inv[k]), storable<FMT>(v[5][k] * inv[k]), storable<FMT>(v[6][k] * inv[k]), storable<FMT>(v[7][k] * inv[k]));
+      if constexpr (sizeof(T) == 2) {
+        uint32_t d[4];                                                  // column k of rows 2 i, 2 i + 1
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          d[i] = In::storable(__builtin_amdgcn_perm(v[2 * i + 1].word(k >> 1), v[2 * i].word(k >> 1), k & 1 ? 0x07060302u : 0x05040100u), nan);
+        w.x = fp8_pair<FMT, true>(fp8_pair<FMT, false>(0, d[0], code[k]), d[1], code[k]);
+        w.y = fp8_pair<FMT, true>(fp8_pair<FMT, false>(0, d[2], code[k]), d[3], code[k]);
+      } else {
+        w.x = fp8_pair<FMT, true>(fp8_pair<FMT, false>(0, In::storable(v[0].value(k), nan), In::storable(v[1].value(k), nan), code[k]),
+                                  In::storable(v[2].value(k), nan), In::storable(v[3].value(k), nan), code[k]);
+        w.y = fp8_pair<FMT, true>(fp8_pair<FMT, false>(0, In::storable(v[4].value(k), nan), In::storable(v[5].value(k), nan), code[k]),
+                                  In::storable(v[6].value(k), nan), In::storable(v[7].value(k), nan), code[k]);
+      }
       *reinterpret_cast<uint2*>(sh + (tx * 8 + k) * FQ_PITCH + ty * 8) = w;
     }
     __syncthreads();
