@@ -78,6 +78,19 @@ __device__ __forceinline__ uint4 bf8_pack(const float (&f)[8]) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// 16 / 8 / 4 bytes at any element's address: the device loads and stores them in one instruction whatever the alignment (rows of odd
+// lengths, slices), only slower where a cache line is crossed
+struct __attribute__((packed, aligned(2))) Any128 { uint32_t w[4]; };
+struct __attribute__((packed, aligned(2))) Any64 { uint32_t w[2]; };
+struct __attribute__((packed, aligned(2))) Any32 { uint32_t w; };
+__device__ __forceinline__ uint4 ld128_any(const void* p) {
+  const Any128 a = *static_cast<const Any128*>(p);
+  return make_uint4(a.w[0], a.w[1], a.w[2], a.w[3]);
+}
+__device__ __forceinline__ void st128_any(void* p, const uint4& v) {
+  *static_cast<Any128*>(p) = Any128{{v.x, v.y, v.z, v.w}};
+}
+
 template <typename T> struct Elem;
 template <> struct Elem<float> {
   static __device__ __forceinline__ float ld(const float* p) { return *p; }

@@ -39,8 +39,8 @@ struct Fp8In16 {
   uint4 w;
   __device__ __forceinline__ void zero() { w = make_uint4(0, 0, 0, 0); }
   __device__ __forceinline__ void load(const u16* p, int have, bool vec) {
-    if (vec && have >= 8) {
-      w = *reinterpret_cast<const uint4*>(p);
+    if (have >= 8) {
+      w = vec ? *reinterpret_cast<const uint4*>(p) : ld128_any(p);
     } else {
       uint32_t q[4];
 #pragma unroll
@@ -82,9 +82,9 @@ struct Fp8In32 {
   f32x4 a, b;
   __device__ __forceinline__ void zero() { a = b = f32x4{0.f, 0.f, 0.f, 0.f}; }
   __device__ __forceinline__ void load(const float* p, int have, bool vec) {
-    if (vec && have >= 8) {
-      a = *reinterpret_cast<const f32x4*>(p);
-      b = *reinterpret_cast<const f32x4*>(p + 4);
+    if (have >= 8) {
+      a = vec ? *reinterpret_cast<const f32x4*>(p) : __builtin_bit_cast(f32x4, ld128_any(p));
+      b = vec ? *reinterpret_cast<const f32x4*>(p + 4) : __builtin_bit_cast(f32x4, ld128_any(p + 4));
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {

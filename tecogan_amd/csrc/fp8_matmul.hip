@@ -313,12 +313,10 @@ void launch_formats(const MmP& p, const char* name, double flops, double bytes, 
 
 // Few rows of a: 16 columns n of the output for a workgroup, all M (at most 16 MF) rows.  Here the weight's bytes count: every wave
 // streams its blocks of K (wave w those with kb % 8 = w: the waves of a workgroup read 1 KB of a row together) from memory straight
-// into the operand's registers, four blocks in flight, and the waves' sums meet in LDS in a fixed order.  Both operands are widened to
+// into the operand's registers, two or four blocks in flight, and the waves' sums meet in LDS in a fixed order.  Both operands are widened to
 // bf16 (there is time: fp32 sums for either output type).
 // SRC: where a comes from -- 0, 1: 8-bit e4m3 / e5m2; 2, 3: bf16 / f32 values that are quantised here, as tg_fp8_quantize does it (at
 // most 16 rows: one launch instead of two).
-template <int SRC> struct SkinnyA { static constexpr int FMT = SRC == 1 ? 1 : 0; };
-
 struct SkP {
   MmP m;
   const void* x;
@@ -326,10 +324,13 @@ struct SkP {
   int cols, xvec;                                                     // columns of x before padding
 };
 
-constexpr int SK_WAVES = 8, SK_AHEAD = 4;
+constexpr int SK_WAVES = 8;
 
 template <int FB, int SRC, int MF>
 __global__ __launch_bounds__(64 * SK_WAVES) void fp8_skinny_kernel(SkP s) {
+  constexpr int AHEAD = MF == 4 ? 2 : 4;                                // blocks of K in flight
+  using T = std::conditional_t<SRC == 3, float, u16>;
+  using In = typename Fp8In<T>::type;
   const MmP& p = s.m;
   __shared__ float join[SK_WAVES][MF][256];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g = lane >> 4;
@@ -337,62 +338,67 @@ __global__ __launch_bounds__(64 * SK_WAVES) void fp8_skinny_kernel(SkP s) {
   const int nkb = p.K >> 7;
   const unsigned char* const pb = p.b + n * p.K + g * 16;
   const unsigned char* const qb = p.sb + (n >> p.sh_b) * p.sp;
+  int64_t m[MF];
+#pragma unroll
+  for (int i = 0; i < MF; ++i) m[i] = 16 * i + r16 < p.M ? 16 * i + r16 : p.M - 1;
+  const T* const row = static_cast<const T*>(s.x) + (SRC >= 2 ? m[0] * s.ldx : 0);
   f32x4 acc[MF];
 #pragma unroll
   for (int i = 0; i < MF; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int k0 = wave; k0 < nkb; k0 += SK_WAVES * SK_AHEAD) {
-    i32x4m wl[SK_AHEAD], wh[SK_AHEAD];
-    int ws[SK_AHEAD];
+  for (int k0 = wave; k0 < nkb; k0 += SK_WAVES * AHEAD) {
+    i32x4m wl[AHEAD], wh[AHEAD], al[AHEAD][MF], ah[AHEAD][MF];
+    In f[SRC >= 2 ? AHEAD : 1][4];
+    int ws[AHEAD], as[AHEAD][MF];
 #pragma unroll
-    for (int u = 0; u < SK_AHEAD; ++u) {
+    for (int u = 0; u < AHEAD; ++u) {
       const int kb = k0 + u * SK_WAVES < nkb ? k0 + u * SK_WAVES : k0;   // past the end: loaded again, not used
       wl[u] = *reinterpret_cast<const i32x4m*>(pb + kb * 128);
       wh[u] = *reinterpret_cast<const i32x4m*>(pb + kb * 128 + 64);
       ws[u] = qb[kb];
+      if constexpr (SRC >= 2) {
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {                                    // chunks g and g + 4 of the block: 2 x 16 values
+          const int c = kb * 128 + (h >> 1) * 64 + g * 16 + (h & 1) * 8, have = s.cols - c;
+          f[u][h].load(row + c, have < 0 ? 0 : (have > 8 ? 8 : have), s.xvec != 0);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < MF; ++i) {
+          const unsigned char* const pa = p.a + m[i] * p.K + kb * 128 + g * 16;
+          al[u][i] = *reinterpret_cast<const i32x4m*>(pa);
+          ah[u][i] = *reinterpret_cast<const i32x4m*>(pa + 64);
+          as[u][i] = p.sa[(m[i] >> p.sh_a) * p.sp + kb];
+        }
+      }
     }
 #pragma unroll
-    for (int u = 0; u < SK_AHEAD; ++u) {
-      const int kb = k0 + u * SK_WAVES;
-      if (kb >= nkb) break;
+    for (int u = 0; u < AHEAD; ++u) {
+      if (k0 + u * SK_WAVES >= nkb) break;
       const float sb = __int_as_float(ws[u] << 23);
-      bf16x8 b[4];
-      b[0] = widen<FB>(wl[u][0], wl[u][1], sb);
-      b[1] = widen<FB>(wl[u][2], wl[u][3], sb);
-      b[2] = widen<FB>(wh[u][0], wh[u][1], sb);
-      b[3] = widen<FB>(wh[u][2], wh[u][3], sb);
+      const bf16x8 b[4] = {widen<FB>(wl[u][0], wl[u][1], sb), widen<FB>(wl[u][2], wl[u][3], sb), widen<FB>(wh[u][0], wh[u][1], sb),
+                           widen<FB>(wh[u][2], wh[u][3], sb)};
 #pragma unroll
       for (int i = 0; i < MF; ++i) {
-        const int64_t m = 16 * i + r16 < p.M ? 16 * i + r16 : p.M - 1;
         i32x4m lo, hi;
         float sa;
         if constexpr (SRC < 2) {
-          const unsigned char* const pa = p.a + m * p.K + kb * 128 + g * 16;
-          lo = *reinterpret_cast<const i32x4m*>(pa);
-          hi = *reinterpret_cast<const i32x4m*>(pa + 64);
-          sa = __int_as_float(p.sa[(m >> p.sh_a) * p.sp + kb] << 23);
+          lo = al[u][i];
+          hi = ah[u][i];
+          sa = __int_as_float(as[u][i] << 23);
         } else {
-          using T = std::conditional_t<SRC == 2, u16, float>;
-          const T* const row = static_cast<const T*>(s.x) + m * s.ldx;
-          typename Fp8In<T>::type f[4];                                // chunks g and g + 4 of the block: 2 x 16 values
-          uint32_t most = 0;
-#pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            const int c = kb * 128 + (h >> 1) * 64 + g * 16 + (h & 1) * 8, have = s.cols - c;
-            f[h].load(row + c, have < 0 ? 0 : (have > 8 ? 8 : have), s.xvec != 0);
-            most = max(most, f[h].most(false));
-          }
+          uint32_t most = max(max(f[u][0].most(false), f[u][1].most(false)), max(f[u][2].most(false), f[u][3].most(false)));
           const bool bad = __any(most >= FP8_INF);
-          if (bad) most = max(max(f[0].most(true), f[1].most(true)), max(f[2].most(true), f[3].most(true)));
+          if (bad) most = max(max(f[u][0].most(true), f[u][1].most(true)), max(f[u][2].most(true), f[u][3].most(true)));
           most = max(most, (uint32_t)__shfl_xor((int)most, 16, 64));    // the four lanes of a row
           most = max(most, (uint32_t)__shfl_xor((int)most, 32, 64));
           const uint32_t code = fp8_scale_code<TG_FP8_E4M3>(most);
           sa = __uint_as_float(code << 23);
-          const uint2 w0 = f[0].template pack<TG_FP8_E4M3>(code, bad), w1 = f[1].template pack<TG_FP8_E4M3>(code, bad);
-          const uint2 w2 = f[2].template pack<TG_FP8_E4M3>(code, bad), w3 = f[3].template pack<TG_FP8_E4M3>(code, bad);
+          const uint2 w0 = f[u][0].template pack<TG_FP8_E4M3>(code, bad), w1 = f[u][1].template pack<TG_FP8_E4M3>(code, bad);
+          const uint2 w2 = f[u][2].template pack<TG_FP8_E4M3>(code, bad), w3 = f[u][3].template pack<TG_FP8_E4M3>(code, bad);
           lo = i32x4m{(int)w0.x, (int)w0.y, (int)w1.x, (int)w1.y};
           hi = i32x4m{(int)w2.x, (int)w2.y, (int)w3.x, (int)w3.y};
         }
-        constexpr int FA = SkinnyA<SRC>::FMT;
+        constexpr int FA = SRC == 1 ? 1 : 0;
         acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[0], widen<FA>(lo[0], lo[1], sa), acc[i], 0, 0, 0);
         acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[1], widen<FA>(lo[2], lo[3], sa), acc[i], 0, 0, 0);
         acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[2], widen<FA>(hi[0], hi[1], sa), acc[i], 0, 0, 0);

@@ -35,6 +35,14 @@ __device__ __forceinline__ void load8(const T* __restrict__ row, int c, int C, f
 #pragma unroll
       for (int k = 0; k < 8; ++k) f[k] = 0.f;
     }
+  } else if (c + 8 <= C) {                                        // any alignment
+    if constexpr (sizeof(T) == 2) {
+      bf8_unpack(ld128_any(row + c), f);
+    } else {
+      const f4v a = __builtin_bit_cast(f4v, ld128_any(row + c)), b = __builtin_bit_cast(f4v, ld128_any(row + c + 4));
+      f[0] = a[0]; f[1] = a[1]; f[2] = a[2]; f[3] = a[3];
+      f[4] = b[0]; f[5] = b[1]; f[6] = b[2]; f[7] = b[3];
+    }
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k) f[k] = c + k < C ? Elem<T>::ld(row + c + k) : 0.f;
@@ -69,6 +77,13 @@ __device__ __forceinline__ void store8(T* __restrict__ row, int c, int C, const 
       *reinterpret_cast<f4v*>(row + c) = f4v{f[0], f[1], f[2], f[3]};
       *reinterpret_cast<f4v*>(row + c + 4) = f4v{f[4], f[5], f[6], f[7]};
     }
+  } else if (c + 8 <= C) {
+    if constexpr (sizeof(T) == 2) {
+      st128_any(row + c, bf8_pack(f));
+    } else {
+      st128_any(row + c, __builtin_bit_cast(uint4, f4v{f[0], f[1], f[2], f[3]}));
+      st128_any(row + c + 4, __builtin_bit_cast(uint4, f4v{f[4], f[5], f[6], f[7]}));
+    }
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
@@ -86,6 +101,9 @@ __device__ __forceinline__ void param8(const float* __restrict__ p, int c, int C
         a = *reinterpret_cast<const f4v*>(p + c);
         b = *reinterpret_cast<const f4v*>(p + c + 4);
       }
+    } else if (c + 8 <= C) {
+      a = __builtin_bit_cast(f4v, ld128_any(p + c));
+      b = __builtin_bit_cast(f4v, ld128_any(p + c + 4));
     } else {
       if (c + 0 < C) a[0] = p[c + 0];
       if (c + 1 < C) a[1] = p[c + 1];

@@ -52,14 +52,14 @@ template <> struct Raw<u16, 1> {
 };
 template <> struct Raw<u16, 2> {
   uint32_t w;
-  __device__ __forceinline__ void load(const u16* p) { w = *reinterpret_cast<const uint32_t*>(p); }
+  __device__ __forceinline__ void load(const u16* p) { w = reinterpret_cast<const Any32*>(p)->w; }
   __device__ __forceinline__ void zero() { w = 0; }
   __device__ __forceinline__ void values(float (&f)[2]) const {
     f[0] = __uint_as_float(w << 16);
     f[1] = __uint_as_float(w & 0xffff0000u);
   }
   static __device__ __forceinline__ void store(u16* p, const float (&f)[2]) {
-    *reinterpret_cast<uint32_t*>(p) = (uint32_t)f2bf(f[0]) | ((uint32_t)f2bf(f[1]) << 16);
+    reinterpret_cast<Any32*>(p)->w = (uint32_t)f2bf(f[0]) | ((uint32_t)f2bf(f[1]) << 16);
   }
 };
 template <> struct Raw<float, 1> {
@@ -71,13 +71,18 @@ template <> struct Raw<float, 1> {
 };
 template <> struct Raw<float, 2> {
   float2 w;
-  __device__ __forceinline__ void load(const float* p) { w = *reinterpret_cast<const float2*>(p); }
+  __device__ __forceinline__ void load(const float* p) {
+    const Any64 a = *reinterpret_cast<const Any64*>(p);
+    w = make_float2(__uint_as_float(a.w[0]), __uint_as_float(a.w[1]));
+  }
   __device__ __forceinline__ void zero() { w = make_float2(0.f, 0.f); }
   __device__ __forceinline__ void values(float (&f)[2]) const {
     f[0] = w.x;
     f[1] = w.y;
   }
-  static __device__ __forceinline__ void store(float* p, const float (&f)[2]) { *reinterpret_cast<float2*>(p) = make_float2(f[0], f[1]); }
+  static __device__ __forceinline__ void store(float* p, const float (&f)[2]) {
+    *reinterpret_cast<Any64*>(p) = Any64{{__float_as_uint(f[0]), __float_as_uint(f[1])}};
+  }
 };
 
 // sigmoid(g) and sigmoid(-g) without a difference: e = exp(-g), 1 / (1 + e) and e / (1 + e); e past 2^100: 1 (e may be infinite)
@@ -672,9 +677,7 @@ extern "C" int tg_gated_scan_forward(const tg_gated_scan_desc* d, const void* x,
   const int64_t need = tile_floats(pl, d->B, d->D) + (pl.nc > 1 ? 2 * chunk_floats(pl, d->B, d->D) : 0);
   TG_CHECK_ARG((pl.nc == 1 && !keep) || (carry != nullptr && carry_floats >= need && al(carry, 16)), "the carry of tg_gated_scan_sizes() floats is missing");
   const int es = d->dtype == TG_F32 ? 4 : 2;
-  const bool even = d->D % 2 == 0 && al(x, 2 * es) && al(g, 2 * es) && al(y, 2 * es) &&
-                    ((d->x_t | d->x_b | d->g_t | d->g_b | d->y_t | d->y_b) & 1) == 0;
-  const int V = even ? 2 : 1;
+  const int V = d->D % 2 == 0 ? 2 : 1;
   GsP p = {};
   p.d = *d;
   p.x = x; p.g = g; p.h0 = h0; p.floor = floor; p.lengths = lengths; p.reset = reset; p.y = y; p.hT = hT;
@@ -711,10 +714,7 @@ extern "C" int tg_gated_scan_backward(const tg_gated_scan_desc* d, const void* x
     const int64_t cf = chunk_floats(pl, d->B, d->D), want = cf * (pl.nc > 1 ? 2 : 1);
     TG_CHECK_ARG((pl.nc == 1 && !d_floor) || (ws != nullptr && ws_floats >= want && al(ws, 16)), "a workspace of tg_gated_scan_sizes() floats is missing");
     const int es = d->dtype == TG_F32 ? 4 : 2;
-    const bool even = d->D % 2 == 0 && al(x, 2 * es) && al(g, 2 * es) && al(d_y, 2 * es) && al(d_x, 2 * es) && al(d_g, 2 * es) &&
-                      ((d->x_t | d->x_b | d->g_t | d->g_b | d->dx_t | d->dx_b | d->dg_t | d->dg_b) & 1) == 0 &&
-                      (!d_y || ((d->dy_t | d->dy_b) & 1) == 0);
-    const int V = even ? 2 : 1;
+    const int V = d->D % 2 == 0 ? 2 : 1;
     GsP p = {};
     p.d = *d;
     p.x = x; p.g = g; p.floor = floor; p.lengths = lengths; p.reset = reset; p.d_y = d_y; p.d_hT = d_hT;
