@@ -33,11 +33,12 @@ __device__ __forceinline__ uint32_t fp8_pair(uint32_t w, uint32_t ab /*two bf16*
   else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf8_bf16(o, v, s, HI));
 }
 
-// 8 neighbouring values as they lie in memory.  `bad` (the same for a wave): a NaN or an infinity is among the wave's values; they
+// 8 neighbouring values as they lie in memory.  BAD (one choice for a wave): a NaN or an infinity is among the wave's values; they
 // are left out of the largest absolute value, and infinities of e4m3, which has none, become NaN before the conversion.
 struct Fp8In16 {
   uint4 w;
   __device__ __forceinline__ void zero() { w = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void load(const u16* p) { w = *reinterpret_cast<const uint4*>(p); }
   __device__ __forceinline__ void load(const u16* p, int have, bool vec) {
     if (have >= 8) {
       w = vec ? *reinterpret_cast<const uint4*>(p) : ld128_any(p);
@@ -50,37 +51,43 @@ struct Fp8In16 {
   }
   __device__ __forceinline__ uint32_t word(int k) const { return k == 0 ? w.x : k == 1 ? w.y : k == 2 ? w.z : w.w; }
   // |values| of word k, two bf16
-  __device__ __forceinline__ u16x2q abs2(int k, bool bad) const {
+  template <bool BAD>
+  __device__ __forceinline__ u16x2q abs2(int k) const {
     uint32_t a = word(k) & 0x7fff7fffu;
-    if (bad) {
+    if constexpr (BAD) {
       if ((a & 0xffffu) >= 0x7f80u) a &= 0xffff0000u;
       if ((a >> 16) >= 0x7f80u) a &= 0xffffu;
     }
     return __builtin_bit_cast(u16x2q, a);
   }
-  __device__ __forceinline__ uint32_t most(bool bad) const {           // bits of the largest absolute value
-    const u16x2q m = __builtin_elementwise_max(__builtin_elementwise_max(abs2(0, bad), abs2(1, bad)), __builtin_elementwise_max(abs2(2, bad), abs2(3, bad)));
+  template <bool BAD>
+  __device__ __forceinline__ uint32_t most() const {                   // bits of the largest absolute value
+    const u16x2q m = __builtin_elementwise_max(__builtin_elementwise_max(abs2<BAD>(0), abs2<BAD>(1)), __builtin_elementwise_max(abs2<BAD>(2), abs2<BAD>(3)));
     return (uint32_t)(m[0] > m[1] ? m[0] : m[1]) << 16;
   }
-  static __device__ __forceinline__ uint32_t storable(uint32_t ab, bool bad) {
-    if (bad) {
+  template <int FMT, bool BAD>
+  static __device__ __forceinline__ uint32_t storable(uint32_t ab) {
+    if constexpr (BAD && FMT == TG_FP8_E4M3) {
       if ((ab & 0x7fffu) == 0x7f80u) ab |= 0x40u;
       if ((ab & 0x7fff0000u) == 0x7f800000u) ab |= 0x400000u;
     }
     return ab;
   }
-  template <int FMT>
-  __device__ __forceinline__ uint2 pack(uint32_t code, bool bad) const {
-    const bool nan = bad && FMT == TG_FP8_E4M3;
+  template <int FMT, bool BAD>
+  __device__ __forceinline__ uint2 pack(uint32_t code) const {
     uint2 o;
-    o.x = fp8_pair<FMT, true>(fp8_pair<FMT, false>(0, storable(w.x, nan), code), storable(w.y, nan), code);
-    o.y = fp8_pair<FMT, true>(fp8_pair<FMT, false>(0, storable(w.z, nan), code), storable(w.w, nan), code);
+    o.x = fp8_pair<FMT, true>(fp8_pair<FMT, false>(0, storable<FMT, BAD>(w.x), code), storable<FMT, BAD>(w.y), code);
+    o.y = fp8_pair<FMT, true>(fp8_pair<FMT, false>(0, storable<FMT, BAD>(w.z), code), storable<FMT, BAD>(w.w), code);
     return o;
   }
 };
 struct Fp8In32 {
   f32x4 a, b;
   __device__ __forceinline__ void zero() { a = b = f32x4{0.f, 0.f, 0.f, 0.f}; }
+  __device__ __forceinline__ void load(const float* p) {
+    a = *reinterpret_cast<const f32x4*>(p);
+    b = *reinterpret_cast<const f32x4*>(p + 4);
+  }
   __device__ __forceinline__ void load(const float* p, int have, bool vec) {
     if (have >= 8) {
       a = vec ? *reinterpret_cast<const f32x4*>(p) : __builtin_bit_cast(f32x4, ld128_any(p));
@@ -94,28 +101,30 @@ struct Fp8In32 {
     }
   }
   __device__ __forceinline__ float value(int k) const { return k < 4 ? a[k & 3] : b[k & 3]; }
-  __device__ __forceinline__ uint32_t abs1(int k, bool bad) const {
+  template <bool BAD>
+  __device__ __forceinline__ uint32_t abs1(int k) const {
     const uint32_t v = __float_as_uint(value(k)) & 0x7fffffffu;
-    return bad && v >= FP8_INF ? 0u : v;
+    return BAD && v >= FP8_INF ? 0u : v;
   }
-  __device__ __forceinline__ uint32_t most(bool bad) const {
+  template <bool BAD>
+  __device__ __forceinline__ uint32_t most() const {
     uint32_t m = 0;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const uint32_t v = abs1(k, bad);
+      const uint32_t v = abs1<BAD>(k);
       m = m > v ? m : v;
     }
     return m;
   }
-  static __device__ __forceinline__ float storable(float v, bool bad) {
-    return bad && (__float_as_uint(v) & 0x7fffffffu) == FP8_INF ? __builtin_nanf("") : v;
+  template <int FMT, bool BAD>
+  static __device__ __forceinline__ float storable(float v) {
+    return BAD && FMT == TG_FP8_E4M3 && (__float_as_uint(v) & 0x7fffffffu) == FP8_INF ? __builtin_nanf("") : v;
   }
-  template <int FMT>
-  __device__ __forceinline__ uint2 pack(uint32_t code, bool bad) const {
-    const bool nan = bad && FMT == TG_FP8_E4M3;
+  template <int FMT, bool BAD>
+  __device__ __forceinline__ uint2 pack(uint32_t code) const {
     uint2 o;
-    o.x = fp8_pair<FMT, true>(fp8_pair<FMT, false>(0, storable(a[0], nan), storable(a[1], nan), code), storable(a[2], nan), storable(a[3], nan), code);
-    o.y = fp8_pair<FMT, true>(fp8_pair<FMT, false>(0, storable(b[0], nan), storable(b[1], nan), code), storable(b[2], nan), storable(b[3], nan), code);
+    o.x = fp8_pair<FMT, true>(fp8_pair<FMT, false>(0, storable<FMT, BAD>(a[0]), storable<FMT, BAD>(a[1]), code), storable<FMT, BAD>(a[2]), storable<FMT, BAD>(a[3]), code);
+    o.y = fp8_pair<FMT, true>(fp8_pair<FMT, false>(0, storable<FMT, BAD>(b[0]), storable<FMT, BAD>(b[1]), code), storable<FMT, BAD>(b[2]), storable<FMT, BAD>(b[3]), code);
     return o;
   }
 };

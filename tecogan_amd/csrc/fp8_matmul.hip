@@ -82,13 +82,16 @@ __device__ __forceinline__ bf16x8 widen(int lo, int hi, float scale) {
 }
 
 typedef __attribute__((address_space(3))) void lds_void_m;
-// 16 bytes a lane from rsrc[voff + soff] to lds + 16 lane
+// 16 (4) bytes a lane from rsrc[voff + soff] to lds + 16 (4) lane
+__device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t rsrc, unsigned char* lds, int voff, int soff) {   // 4 bytes a lane
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_m*)lds, 4, voff, soff, 0, 0);
+}
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rsrc, unsigned char* lds, int voff, int soff) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_m*)lds, 16, voff, soff, 0, 0);
 }
 
 // 32 MF x 32 NF outputs, four waves of 16 MF x 16 NF.  A stage of LDS holds one block of K of both operands, rows of 128 bytes, filled
-// by 16-byte DMA from global memory, and the scale dwords of its rows; two stages in turn.  The 16-byte chunk c of row r sits at chunk
+// by 16-byte DMA from global memory, and the scale dwords of its rows; S stages in turn.  The 16-byte chunk c of row r sits at chunk
 // c ^ ((r >> 1) & 7) (chosen on the global side): a lane's 32 bytes are chunks g and g + 4 (g = lane / 16) in both operands -- any
 // order of k serves -- and the 16 lanes that a ds_read_b128 serves together cover all 64 banks once.
 //
@@ -96,8 +99,8 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rsrc, unsigned char
 // quarter's products the fragments that the next quarters need are read, each into the registers of the one that has just been used
 // up: b1, a1 of this block, then a0 and -- column by column, as (a1, b0) finishes with them -- b0 of the next.  The one barrier of a
 // block sits in its middle: there every wave has read the last of this stage and its own DMA of the next stage has landed; the DMA
-// of the block after that goes out between the products of the second half.
-template <int FB, int FA, bool WIDE, int MF, int NF>
+// of block kb + S goes out between the products of the second half.
+template <int FB, int FA, bool WIDE, int MF, int NF, int S>
 __global__ __launch_bounds__(256, MF * NF >= 64 ? 1 : 2) void fp8_tile_kernel(MmP p) {
   constexpr int TM = 32 * MF, TN = 32 * NF, STAGE = (TM + TN) * 132, HM = MF / 2, HN = NF / 2;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -127,19 +130,30 @@ __global__ __launch_bounds__(256, MF * NF >= 64 ? 1 : 2) void fp8_tile_kernel(Mm
     const int row = (wave * NF + i) * 8 + (lane >> 3);
     ob[i] = (row < rows_b ? row : rows_b - 1) * p.K + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
   }
-  auto dma_at = [&](int q, int stage, int kb) {                       // instruction q of block kb into stage % 2
-    unsigned char* const st = smem + (stage & 1) * STAGE;
+  auto dma_at = [&](int q, int stage, int kb) {                       // instruction q of block kb into stage % S
+    unsigned char* const st = smem + (stage & (S - 1)) * STAGE;
     if (q < MF) dma16(rsrcA, st + (wave * MF + q) * 1024, oa[q < MF ? q : 0], kb * 128);
     else dma16(rsrcB, st + TM * 128 + (wave * NF + q - MF) * 1024, ob[q < MF ? 0 : q - MF], kb * 128);
   };
-  // scales: a dword DMA takes the four bytes around block kb of 64 rows: wave w those of A's and of B's rows 64 w .. 64 w + 63
+  // scales: a dword DMA takes the four bytes around block kb of 64 rows
   const auto rsrcSA = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.sa + (m0 >> p.sh_a) * p.sp), 0, (((rows_a - 1) >> p.sh_a) + 1) * p.sp, 0x00020000);
   const auto rsrcSB = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.sb + (n0 >> p.sh_b) * p.sp), 0, (((rows_b - 1) >> p.sh_b) + 1) * p.sp, 0x00020000);
-  const int osa = ((tid < rows_a ? tid : rows_a - 1) >> p.sh_a) * p.sp, osb = ((tid < rows_b ? tid : rows_b - 1) >> p.sh_b) * p.sp;
+  constexpr int NCH = (TM + TN) / 64, NS = NCH >= 4 ? NCH / 4 : 1;     // 64 rows each; with fewer than four, waves fetch the same
+  int os[NS];
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    const int ch = (wave + 4 * i) % NCH, row = (ch * 64 < TM ? ch * 64 : ch * 64 - TM) + lane;
+    if (ch * 64 < TM) os[i] = ((row < rows_a ? row : rows_a - 1) >> p.sh_a) * p.sp;
+    else os[i] = ((row < rows_b ? row : rows_b - 1) >> p.sh_b) * p.sp;
+  }
   auto dma_scales_at = [&](int stage, int kb) {
-    unsigned char* const st = smem + (stage & 1) * STAGE + (TM + TN) * 128;
-    if (wave * 64 < TM) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrcSA, (lds_void_m*)(st + wave * 256), 4, osa, kb & ~3, 0, 0);
-    if (wave * 64 < TN) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrcSB, (lds_void_m*)(st + TM * 4 + wave * 256), 4, osb, kb & ~3, 0, 0);
+    unsigned char* const st = smem + (stage & (S - 1)) * STAGE + (TM + TN) * 128;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const int ch = (wave + 4 * i) % NCH;
+      if (ch * 64 < TM) dma4(rsrcSA, st + ch * 256, os[i], kb & ~3);
+      else dma4(rsrcSB, st + ch * 256, os[i], kb & ~3);
+    }
   };
 
   f32x4 acc[MF][NF];
@@ -151,13 +165,13 @@ __global__ __launch_bounds__(256, MF * NF >= 64 ? 1 : 2) void fp8_tile_kernel(Mm
   int ca[2][HM], cb[2][HN];
   // this lane's addresses in the stage that is read: low and high chunks of a fragment, its scale
   const int la = r16 * 128 + ((g ^ (r16 >> 1)) << 4);
-  const unsigned char* pal = smem + wm * 16 * MF * 128 + la;
-  const unsigned char* pah = smem + ((wm * 16 * MF * 128 + la) ^ 64);
-  const unsigned char* pbl = smem + TM * 128 + wn * 16 * NF * 128 + la;
-  const unsigned char* pbh = smem + ((TM * 128 + wn * 16 * NF * 128 + la) ^ 64);
+  const unsigned char* const bal = smem + wm * 16 * MF * 128 + la;
+  const unsigned char* const bah = smem + ((wm * 16 * MF * 128 + la) ^ 64);
+  const unsigned char* const bbl = smem + TM * 128 + wn * 16 * NF * 128 + la;
+  const unsigned char* const bbh = smem + ((TM * 128 + wn * 16 * NF * 128 + la) ^ 64);
   const unsigned char* const psa = smem + (TM + TN) * 128 + (wm * 16 * MF + r16) * 4;
   const unsigned char* const psb = smem + (TM + TN) * 128 + (TM + wn * 16 * NF + r16) * 4;
-  const unsigned char *qsa = psa, *qsb = psb;
+  const unsigned char *pal = bal, *pah = bah, *pbl = bbl, *pbh = bbh, *qsa = psa, *qsb = psb;
   auto frag = [](const unsigned char* lo, const unsigned char* hi) {
     return __builtin_shufflevector(*reinterpret_cast<const i32x4m*>(lo), *reinterpret_cast<const i32x4m*>(hi), 0, 1, 2, 3, 4, 5, 6, 7);
   };
@@ -169,13 +183,18 @@ __global__ __launch_bounds__(256, MF * NF >= 64 ? 1 : 2) void fp8_tile_kernel(Mm
     fb[h][u] = frag(pbl + (h * HN + u) * 2048, pbh + (h * HN + u) * 2048);
     cb[h][u] = qsb[(h * HN + u) * 64];
   };
-  // the stage of block kb is the one that is read from here on
+  // what is read from here on is block kb
   int shift = STAGE;
   auto turn = [&](int kb) {
-    pal += shift; pah += shift; pbl += shift; pbh += shift;
-    shift = -shift;
-    qsa = psa + (kb & 1) * STAGE + (kb & 3);
-    qsb = psb + (kb & 1) * STAGE + (kb & 3);
+    const int st = (kb & (S - 1)) * STAGE;
+    if constexpr (S == 2) {                                           // no second set of addresses: the largest tile has no registers for it
+      pal += shift; pah += shift; pbl += shift; pbh += shift;
+      shift = -shift;
+    } else {
+      pal = bal + st; pah = bah + st; pbl = bbl + st; pbh = bbh + st;
+    }
+    qsa = psa + st + (kb & 3);
+    qsb = psb + st + (kb & 3);
   };
   // A quarter's products, columns outermost; after(x) follows product x of HM HN
   auto quarter = [&](int ha, int hb, auto after) {
@@ -211,23 +230,21 @@ __global__ __launch_bounds__(256, MF * NF >= 64 ? 1 : 2) void fp8_tile_kernel(Mm
   constexpr int ND = MF + NF, N1 = HM * HN;
   if (nkb > 0) {
 #pragma unroll
-    for (int q = 0; q < ND; ++q) dma_at(q, 0, 0);
-    dma_scales_at(0, 0);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    {
-      const int kb = nkb > 1 ? 1 : 0;
+    for (int k = 0; k < S; ++k) {
+      const int kb = k < nkb ? k : nkb - 1;
 #pragma unroll
-      for (int q = 0; q < ND; ++q) dma_at(q, 1, kb);
-      dma_scales_at(1, kb);
+      for (int q = 0; q < ND; ++q) dma_at(q, k, kb);
+      dma_scales_at(k, kb);
     }
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * (ND + NS)) : "memory");   // the first block has landed
+    __builtin_amdgcn_s_barrier();
 #pragma unroll
     for (int u = 0; u < HM; ++u) read_a(0, u);
 #pragma unroll
     for (int u = 0; u < HN; ++u) read_b(0, u);
     for (int kb = 0; kb < nkb; ++kb) {
       // behind the last block the DMA and the reads go on with the last block's data: nobody uses it
-      const int ahead = kb + 2 < nkb ? kb + 2 : nkb - 1;
+      const int ahead = kb + S < nkb ? kb + S : nkb - 1;
       quarter(0, 0, [&](int x) {
 #pragma unroll
         for (int u = x * HN / N1; u < (x + 1) * HN / N1; ++u) read_b(1, u);
@@ -236,7 +253,8 @@ __global__ __launch_bounds__(256, MF * NF >= 64 ? 1 : 2) void fp8_tile_kernel(Mm
 #pragma unroll
         for (int u = x * HM / N1; u < (x + 1) * HM / N1; ++u) read_a(1, u);
       });
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      // this wave's DMA of the next block has landed: at most that of the S - 2 blocks behind it may be under way
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S - 2) * (ND + NS)) : "memory");
       __builtin_amdgcn_s_barrier();
       __builtin_amdgcn_sched_barrier(0);
       turn(kb + 1);
@@ -294,26 +312,26 @@ __global__ __launch_bounds__(256, MF * NF >= 64 ? 1 : 2) void fp8_tile_kernel(Mm
 }
 
 // hipFuncAttributeMaxDynamicSharedMemorySize is not needed on this device; a launch may ask for up to 160 KB.
-template <int FB, int FA, bool WIDE, int MF, int NF>
+template <int FB, int FA, bool WIDE, int MF, int NF, int S>
 void launch_tile(MmP p, const char* name, double flops, double bytes, hipStream_t st) {
   p.tiles_m = (int)cdiv64(p.M, 32 * MF);
   p.tiles_n = (int)cdiv64(p.N, 32 * NF);
   p.tiles = p.tiles_m * p.tiles_n;
-  constexpr int lds = 2 * (32 * MF + 32 * NF) * 132;
-  TG_LAUNCH(name, flops, bytes, (fp8_tile_kernel<FB, FA, WIDE, MF, NF>), dim3((unsigned)p.tiles), dim3(256), lds, st, p);
+  constexpr int lds = S * (32 * MF + 32 * NF) * 132;
+  TG_LAUNCH(name, flops, bytes, (fp8_tile_kernel<FB, FA, WIDE, MF, NF, S>), dim3((unsigned)p.tiles), dim3(256), lds, st, p);
 }
 
 template <int FB, int FA, bool WIDE>
 void launch_formats(const MmP& p, const char* name, double flops, double bytes, hipStream_t st) {
   const int64_t cus = tg_num_cus();
-  if (cdiv64(p.M, 256) * cdiv64(p.N, 256) * 5 >= cus * 4) launch_tile<FB, FA, WIDE, 8, 8>(p, name, flops, bytes, st);
-  else if (cdiv64(p.M, 128) * cdiv64(p.N, 128) * 5 >= cus * 4) launch_tile<FB, FA, WIDE, 4, 4>(p, name, flops, bytes, st);
-  else launch_tile<FB, FA, WIDE, 2, 2>(p, name, flops, bytes, st);
+  if (cdiv64(p.M, 256) * cdiv64(p.N, 256) * 5 >= cus * 4) launch_tile<FB, FA, WIDE, 8, 8, 2>(p, name, flops, bytes, st);
+  else if (cdiv64(p.M, 128) * cdiv64(p.N, 128) * 5 >= cus * 4) launch_tile<FB, FA, WIDE, 4, 4, 2>(p, name, flops, bytes, st);
+  else launch_tile<FB, FA, WIDE, 2, 2, 4>(p, name, flops, bytes, st);
 }
 
 // Few rows of a: 16 columns n of the output for a workgroup, all M (at most 16 MF) rows.  Here the weight's bytes count: every wave
 // streams its blocks of K (wave w those with kb % 8 = w: the waves of a workgroup read 1 KB of a row together) from memory straight
-// into the operand's registers, two or four blocks in flight, and the waves' sums meet in LDS in a fixed order.  Both operands are widened to
+// into the operand's registers, four blocks in flight, and the waves' sums meet in LDS in a fixed order.  Both operands are widened to
 // bf16 (there is time: fp32 sums for either output type).
 // SRC: where a comes from -- 0, 1: 8-bit e4m3 / e5m2; 2, 3: bf16 / f32 values that are quantised here, as tg_fp8_quantize does it (at
 // most 16 rows: one launch instead of two).
@@ -321,14 +339,14 @@ struct SkP {
   MmP m;
   const void* x;
   int64_t ldx;
-  int cols, xvec;                                                     // columns of x before padding
+  int cols, plain;                                                    // columns of x before padding; whole blocks, 16-byte aligned
 };
 
 constexpr int SK_WAVES = 8;
 
 template <int FB, int SRC, int MF>
 __global__ __launch_bounds__(64 * SK_WAVES) void fp8_skinny_kernel(SkP s) {
-  constexpr int AHEAD = MF == 4 ? 2 : 4;                                // blocks of K in flight
+  constexpr int AHEAD = 4;                                              // blocks of K in flight
   using T = std::conditional_t<SRC == 3, float, u16>;
   using In = typename Fp8In<T>::type;
   const MmP& p = s.m;
@@ -356,10 +374,16 @@ __global__ __launch_bounds__(64 * SK_WAVES) void fp8_skinny_kernel(SkP s) {
       wh[u] = *reinterpret_cast<const i32x4m*>(pb + kb * 128 + 64);
       ws[u] = qb[kb];
       if constexpr (SRC >= 2) {
+        const T* const at = row + kb * 128 + g * 16;                     // chunks g and g + 4 of the block: 2 x 16 values
+        if (s.plain) {
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {                                    // chunks g and g + 4 of the block: 2 x 16 values
-          const int c = kb * 128 + (h >> 1) * 64 + g * 16 + (h & 1) * 8, have = s.cols - c;
-          f[u][h].load(row + c, have < 0 ? 0 : (have > 8 ? 8 : have), s.xvec != 0);
+          for (int h = 0; h < 4; ++h) f[u][h].load(at + (h >> 1) * 64 + (h & 1) * 8);
+        } else {
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            const int o = (h >> 1) * 64 + (h & 1) * 8, have = s.cols - (kb * 128 + g * 16 + o);
+            f[u][h].load(at + o, have < 0 ? 0 : (have > 8 ? 8 : have), false);
+          }
         }
       } else {
 #pragma unroll
@@ -386,17 +410,26 @@ __global__ __launch_bounds__(64 * SK_WAVES) void fp8_skinny_kernel(SkP s) {
           hi = ah[u][i];
           sa = __int_as_float(as[u][i] << 23);
         } else {
-          uint32_t most = max(max(f[u][0].most(false), f[u][1].most(false)), max(f[u][2].most(false), f[u][3].most(false)));
+          uint32_t most = max(max(f[u][0].template most<false>(), f[u][1].template most<false>()),
+                              max(f[u][2].template most<false>(), f[u][3].template most<false>()));
           const bool bad = __any(most >= FP8_INF);
-          if (bad) most = max(max(f[u][0].most(true), f[u][1].most(true)), max(f[u][2].most(true), f[u][3].most(true)));
+          if (bad)
+            most = max(max(f[u][0].template most<true>(), f[u][1].template most<true>()),
+                       max(f[u][2].template most<true>(), f[u][3].template most<true>()));
           most = max(most, (uint32_t)__shfl_xor((int)most, 16, 64));    // the four lanes of a row
           most = max(most, (uint32_t)__shfl_xor((int)most, 32, 64));
           const uint32_t code = fp8_scale_code<TG_FP8_E4M3>(most);
           sa = __uint_as_float(code << 23);
-          const uint2 w0 = f[u][0].template pack<TG_FP8_E4M3>(code, bad), w1 = f[u][1].template pack<TG_FP8_E4M3>(code, bad);
-          const uint2 w2 = f[u][2].template pack<TG_FP8_E4M3>(code, bad), w3 = f[u][3].template pack<TG_FP8_E4M3>(code, bad);
-          lo = i32x4m{(int)w0.x, (int)w0.y, (int)w1.x, (int)w1.y};
-          hi = i32x4m{(int)w2.x, (int)w2.y, (int)w3.x, (int)w3.y};
+          uint2 w[4];
+          if (bad) {
+#pragma unroll
+            for (int h = 0; h < 4; ++h) w[h] = f[u][h].template pack<TG_FP8_E4M3, true>(code);
+          } else {
+#pragma unroll
+            for (int h = 0; h < 4; ++h) w[h] = f[u][h].template pack<TG_FP8_E4M3, false>(code);
+          }
+          lo = i32x4m{(int)w[0].x, (int)w[0].y, (int)w[1].x, (int)w[1].y};
+          hi = i32x4m{(int)w[2].x, (int)w[2].y, (int)w[3].x, (int)w[3].y};
         }
         constexpr int FA = SRC == 1 ? 1 : 0;
         acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[0], widen<FA>(lo[0], lo[1], sa), acc[i], 0, 0, 0);
@@ -432,10 +465,15 @@ void launch_skinny(const SkP& s, const char* name, double flops, double bytes, h
   if (mf <= 1) TG_LAUNCH(name, flops, bytes, (fp8_skinny_kernel<FB, SRC, 1>), grid, block, 0, st, s);
   if constexpr (SRC < 2) {
     if (mf == 2) TG_LAUNCH(name, flops, bytes, (fp8_skinny_kernel<FB, SRC, 2>), grid, block, 0, st, s);
-    if (mf > 2) TG_LAUNCH(name, flops, bytes, (fp8_skinny_kernel<FB, SRC, 4>), grid, block, 0, st, s);
   }
 }
-constexpr int SK_ROWS = 64, SK_FUSED = 16;
+// Up to 32 rows (4096 x 4096: 6.5 us with 1, 10 with 32 rows; with 64 the 64 x 64 tiles take 12, this kernel 15).  Quantising on the way
+// costs every workgroup the whole of x again: with 4 blocks of K a wave in one round of workgroups 3.6 us, twice or four times that 8 - 12,
+// against about 4.5 us for a launch of the quantiser.
+constexpr int SK_ROWS = 32, SK_FUSED = 16;
+bool skinny_fuses(int64_t M, int64_t N, int64_t nkb) {
+  return M <= SK_FUSED && cdiv64(cdiv64(N, 16), tg_num_cus()) * cdiv64(nkb, SK_WAVES) <= 4;
+}
 
 bool al16m(const void* p) { return ((uintptr_t)p & 15) == 0; }
 bool fmt_ok(int f) { return f == TG_FP8_E4M3 || f == TG_FP8_E5M2; }
@@ -523,7 +561,7 @@ extern "C" int tg_fp8_linear(const void* x, int dtype, int64_t M, int64_t K, int
   d.a_fmt = TG_FP8_E4M3; d.b_fmt = w_fmt; d.b_tile = 1; d.out_dtype = out_dtype;
   TG_CHECK_ARG(fmt_ok(w_fmt) && w && scale_w && out && al16m(w) && ((uintptr_t)scale_w & 3) == 0 && ldo >= N &&
                    (out_dtype == TG_F32 || out_dtype == TG_BF16), "bad weight or output");
-  if (M <= SK_FUSED) {
+  if (skinny_fuses(M, N, kb)) {
     TG_CHECK_ARG(x != nullptr && ldx >= K && (dtype == TG_F32 || dtype == TG_BF16), "x is missing, its type unknown or its row stride below K");
     SkP k = {};
     k.m.b = static_cast<const unsigned char*>(w); k.m.sb = static_cast<const unsigned char*>(scale_w);
@@ -536,7 +574,7 @@ extern "C" int tg_fp8_linear(const void* x, int dtype, int64_t M, int64_t K, int
     k.x = x;
     k.ldx = ldx;
     k.cols = (int)K;
-    k.xvec = al16m(x) && (ldx * (dtype == TG_F32 ? 4 : 2)) % 16 == 0;
+    k.plain = K % 128 == 0 && al16m(x) && (ldx * (dtype == TG_F32 ? 4 : 2)) % 16 == 0;
     const double flops = 2.0 * M * N * K, bytes = (double)N * K + (double)M * K * (dtype == TG_F32 ? 4 : 2) + (double)M * N * (k.m.out_bf16 ? 2 : 4);
     const char* const name = "fp8_skinny<quantise>";
     if (dtype == TG_BF16) {

@@ -22,6 +22,60 @@ struct FqP {
   int tiles_c, tile, vec;
 };
 
+// bits of the largest absolute values of a thread's 8 columns, over the wave's 32 rows
+template <bool BAD>
+__device__ __forceinline__ void column_most(const Fp8In16 (&v)[8], uint32_t (&m)[8]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    u16x2q a = v[0].abs2<BAD>(k);
+#pragma unroll
+    for (int j = 1; j < 8; ++j) a = __builtin_elementwise_max(a, v[j].abs2<BAD>(k));
+    a = __builtin_elementwise_max(a, __builtin_bit_cast(u16x2q, __shfl_xor(__builtin_bit_cast(int, a), 16, 64)));
+    a = __builtin_elementwise_max(a, __builtin_bit_cast(u16x2q, __shfl_xor(__builtin_bit_cast(int, a), 32, 64)));
+    m[2 * k] = (uint32_t)a[0] << 16;
+    m[2 * k + 1] = (uint32_t)a[1] << 16;
+  }
+}
+template <bool BAD>
+__device__ __forceinline__ void column_most(const Fp8In32 (&v)[8], uint32_t (&m)[8]) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    m[k] = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m[k] = max(m[k], v[j].abs1<BAD>(k));
+    m[k] = max(m[k], (uint32_t)__shfl_xor((int)m[k], 16, 64));
+    m[k] = max(m[k], (uint32_t)__shfl_xor((int)m[k], 32, 64));
+  }
+}
+// a thread's 8 columns of 8 rows as bytes, column by column
+template <int FMT, bool BAD>
+__device__ __forceinline__ void columns_out(const Fp8In16 (&v)[8], const uint32_t (&code)[8], unsigned char* out) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    uint32_t d[4];                                                      // column k of rows 2 i, 2 i + 1
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      d[i] = Fp8In16::storable<FMT, BAD>(__builtin_amdgcn_perm(v[2 * i + 1].word(k >> 1), v[2 * i].word(k >> 1), k & 1 ? 0x07060302u : 0x05040100u));
+    uint2 w;
+    w.x = fp8_pair<FMT, true>(fp8_pair<FMT, false>(0, d[0], code[k]), d[1], code[k]);
+    w.y = fp8_pair<FMT, true>(fp8_pair<FMT, false>(0, d[2], code[k]), d[3], code[k]);
+    *reinterpret_cast<uint2*>(out + k * FQ_PITCH) = w;
+  }
+}
+template <int FMT, bool BAD>
+__device__ __forceinline__ void columns_out(const Fp8In32 (&v)[8], const uint32_t (&code)[8], unsigned char* out) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    float d[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) d[j] = Fp8In32::storable<FMT, BAD>(v[j].value(k));
+    uint2 w;
+    w.x = fp8_pair<FMT, true>(fp8_pair<FMT, false>(0, d[0], d[1], code[k]), d[2], d[3], code[k]);
+    w.y = fp8_pair<FMT, true>(fp8_pair<FMT, false>(0, d[4], d[5], code[k]), d[6], d[7], code[k]);
+    *reinterpret_cast<uint2*>(out + k * FQ_PITCH) = w;
+  }
+}
+
 template <typename T, int FMT>
 __global__ __launch_bounds__(256) void fp8_quantize_kernel(FqP p) {
   __shared__ __attribute__((aligned(16))) unsigned char sh[128 * FQ_PITCH];
@@ -40,7 +94,7 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(FqP p) {
   uint32_t mr[8], ma = 0;                                               // bits of the largest absolute value: of each row, of all
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    mr[j] = v[j].most(false);
+    mr[j] = v[j].template most<false>();
     ma = ma > mr[j] ? ma : mr[j];
   }
   const bool bad = __any(ma >= FP8_INF);
@@ -48,7 +102,7 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(FqP p) {
     ma = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      mr[j] = v[j].most(true);
+      mr[j] = v[j].template most<true>();
       ma = ma > mr[j] ? ma : mr[j];
     }
   }
@@ -70,7 +124,7 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(FqP p) {
     for (int j = 0; j < 8; ++j) {
       const uint32_t code = p.tile ? code_tile : fp8_scale_code<FMT>(fp8_max16(mr[j]));
       if (r0 + j < p.rows) {
-        *reinterpret_cast<uint2*>(p.q + (r0 + j) * p.cp + c0) = v[j].template pack<FMT>(code, bad);
+        *reinterpret_cast<uint2*>(p.q + (r0 + j) * p.cp + c0) = bad ? v[j].template pack<FMT, true>(code) : v[j].template pack<FMT, false>(code);
         if (!p.tile && tx == 0) p.s[(r0 + j) * p.sp + tc] = (unsigned char)code;
       }
     }
@@ -82,27 +136,8 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(FqP p) {
       for (int k = 0; k < 8; ++k) code[k] = code_tile;
     } else {
       uint32_t m[8];                                                    // of the 8 columns, over the wave's 32 rows
-      if constexpr (sizeof(T) == 2) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          u16x2q a = v[0].abs2(k, bad);
-#pragma unroll
-          for (int j = 1; j < 8; ++j) a = __builtin_elementwise_max(a, v[j].abs2(k, bad));
-          a = __builtin_elementwise_max(a, __builtin_bit_cast(u16x2q, __shfl_xor(__builtin_bit_cast(int, a), 16, 64)));
-          a = __builtin_elementwise_max(a, __builtin_bit_cast(u16x2q, __shfl_xor(__builtin_bit_cast(int, a), 32, 64)));
-          m[2 * k] = (uint32_t)a[0] << 16;
-          m[2 * k + 1] = (uint32_t)a[1] << 16;
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          m[k] = 0;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) m[k] = max(m[k], v[j].abs1(k, bad));
-          m[k] = max(m[k], (uint32_t)__shfl_xor((int)m[k], 16, 64));
-          m[k] = max(m[k], (uint32_t)__shfl_xor((int)m[k], 32, 64));
-        }
-      }
+      if (bad) column_most<true>(v, m);
+      else column_most<false>(v, m);
       if ((tid & 63) < 16) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) smax[wave][tx * 8 + k] = m[k];
@@ -115,25 +150,8 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(FqP p) {
         if (ty == 0 && c0 + k < p.cols) p.st[(c0 + k) * p.stp + tr] = (unsigned char)code[k];
       }
     }
-    const bool nan = bad && FMT == TG_FP8_E4M3;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      uint2 w;
-      if constexpr (sizeof(T) == 2) {
-        uint32_t d[4];                                                  // column k of rows 2 i, 2 i + 1
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          d[i] = In::storable(__builtin_amdgcn_perm(v[2 * i + 1].word(k >> 1), v[2 * i].word(k >> 1), k & 1 ? 0x07060302u : 0x05040100u), nan);
-        w.x = fp8_pair<FMT, true>(fp8_pair<FMT, false>(0, d[0], code[k]), d[1], code[k]);
-        w.y = fp8_pair<FMT, true>(fp8_pair<FMT, false>(0, d[2], code[k]), d[3], code[k]);
-      } else {
-        w.x = fp8_pair<FMT, true>(fp8_pair<FMT, false>(0, In::storable(v[0].value(k), nan), In::storable(v[1].value(k), nan), code[k]),
-                                  In::storable(v[2].value(k), nan), In::storable(v[3].value(k), nan), code[k]);
-        w.y = fp8_pair<FMT, true>(fp8_pair<FMT, false>(0, In::storable(v[4].value(k), nan), In::storable(v[5].value(k), nan), code[k]),
-                                  In::storable(v[6].value(k), nan), In::storable(v[7].value(k), nan), code[k]);
-      }
-      *reinterpret_cast<uint2*>(sh + (tx * 8 + k) * FQ_PITCH + ty * 8) = w;
-    }
+    if (bad) columns_out<FMT, true>(v, code, sh + tx * 8 * FQ_PITCH + ty * 8);
+    else columns_out<FMT, false>(v, code, sh + tx * 8 * FQ_PITCH + ty * 8);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
