@@ -78,15 +78,29 @@ __device__ __forceinline__ uint4 bf8_pack(const float (&f)[8]) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// 16 / 8 / 4 bytes at any element's address: the device loads and stores them in one instruction whatever the alignment (rows of odd
-// lengths, slices), only slower where a cache line is crossed
-struct __attribute__((packed, aligned(2))) Any128 { uint32_t w[4]; };
+// 8 / 4 bytes at any element's address (rows of odd lengths, slices): the device takes them in one instruction, only slower
 struct __attribute__((packed, aligned(2))) Any64 { uint32_t w[2]; };
 struct __attribute__((packed, aligned(2))) Any32 { uint32_t w; };
+// 16 bytes at any even address.  A misaligned 16-byte load runs at a fifth of the bandwidth; the two aligned ones that hold its first
+// and its last byte (both in memory that belongs to the tensor: neither touches another 16-byte granule) and a shift do not.
 __device__ __forceinline__ uint4 ld128_any(const void* p) {
-  const Any128 a = *static_cast<const Any128*>(p);
-  return make_uint4(a.w[0], a.w[1], a.w[2], a.w[3]);
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+  const uint4 a = *reinterpret_cast<const uint4*>(at & ~(uintptr_t)15), b = *reinterpret_cast<const uint4*>((at + 15) & ~(uintptr_t)15);
+  const uint32_t s = (uint32_t)at & 15;
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  if (s & 8) {
+#pragma unroll
+    for (int k = 0; k < 6; ++k) w[k] = w[k + 2];
+  }
+  if (s & 4) {
+#pragma unroll
+    for (int k = 0; k < 5; ++k) w[k] = w[k + 1];
+  }
+  const uint32_t r = s & 3;
+  return make_uint4(__builtin_amdgcn_alignbyte(w[1], w[0], r), __builtin_amdgcn_alignbyte(w[2], w[1], r),
+                    __builtin_amdgcn_alignbyte(w[3], w[2], r), __builtin_amdgcn_alignbyte(w[4], w[3], r));
 }
+struct __attribute__((packed, aligned(2))) Any128 { uint32_t w[4]; };
 __device__ __forceinline__ void st128_any(void* p, const uint4& v) {
   *static_cast<Any128*>(p) = Any128{{v.x, v.y, v.z, v.w}};
 }

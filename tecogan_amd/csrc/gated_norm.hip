@@ -435,7 +435,8 @@ template <typename TO, typename TX, int NV, bool VEC, int MODE>
 __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
   const bool HO = MODE == 3 ? p.o != nullptr : MODE >= 1, HG = MODE == 3 ? p.gate != nullptr : MODE == 2;
   __shared__ __attribute__((aligned(16))) float red[2 * 8 * 4];
-  extern __shared__ float join[];                                   // [rows of the workgroup][8 lpr]: only where it has several
+  extern __shared__ __attribute__((aligned(16))) float join[];      // [rows of the workgroup][8 lpr]: only where it has several
+  constexpr bool IN_LDS = NV > 1;                                   // the parameter sums of wide rows: no registers for them
   const tg_gated_norm_desc& d = p.d;
   const int lpr = 1 << p.lpr_log2, lane = threadIdx.x & (lpr - 1), sub = threadIdx.x >> p.lpr_log2, rpb = blockDim.x >> p.lpr_log2;
   const int C = d.C;
@@ -452,7 +453,29 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
   }
   end = item < p.items ? (end < d.rows ? end : d.rows) : start;
   const bool layer = d.pre == TG_NORM_LAYER || d.post == TG_NORM_LAYER;
-  float acc[5][NV][8] = {}, dga[NV][8] = {};                        // w_post, b_post, scale, w_pre, b_pre; the gate row
+  // sums of w_post, b_post, scale, w_pre, b_pre, and of the gate row; in LDS every lane has its own places, 16 bytes apart
+  float acc[IN_LDS ? 1 : 5][IN_LDS ? 1 : NV][8] = {}, dga[NV][8] = {};
+  auto place_of = [&](int q, int v) { return reinterpret_cast<f4v*>(join) + (__popc(p.want & ((1 << q) - 1)) * NV + v) * 2 * GN_MAX_LPR + threadIdx.x; };
+  auto add = [&](int q, int v, const float (&t)[8]) {
+    if constexpr (IN_LDS) {
+      if (p.want >> q & 1) {
+        f4v* const at = place_of(q, v);
+        at[0] += f4v{t[0], t[1], t[2], t[3]};
+        at[GN_MAX_LPR] += f4v{t[4], t[5], t[6], t[7]};
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) acc[q][v][k] += t[k];
+    }
+  };
+  if constexpr (IN_LDS) {
+#pragma unroll
+    for (int q = 0; q < 5; ++q)
+      if (p.want >> q & 1) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) place_of(q, v)[0] = place_of(q, v)[GN_MAX_LPR] = f4v{0.f, 0.f, 0.f, 0.f};
+      }
+  }
   Raw8<TX, VEC> ry[NV], rdy[NV];
   Raw8<TO, VEC> rdh[NV], ro[NV], rg[NV];
   auto fetch = [&](int64_t row) {
@@ -490,7 +513,13 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
     fetch(start);
     params();
   }
-  for (int j = 0; j < p.item_rows; ++j) {
+  // the workgroup's longest item: without pieces its first one
+  int jn = p.item_rows;
+  if (p.pieces == 0) {
+    const int64_t rows = d.rows - (int64_t)blockIdx.x * rpb * p.item_rows;
+    if (rows < jn) jn = (int)rows;
+  }
+  for (int j = 0; j < jn; ++j) {
     const bool on = start + j < end;
     const int64_t row = on ? start + j : 0;
     const int Cr = on ? C : 0;
@@ -522,7 +551,7 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
         gate_slopes(g, d.gate_act, ga[v], gs[v]);
       }
     }
-    if (NV == 1 && j + 1 < p.item_rows) fetch(start + j + 1);
+    if (NV == 1 && j + 1 < jn) fetch(start + j + 1);
     float mu_y = 0.f, mu_o = 0.f;
     if (layer) {
       float s[2] = {0.f, 0.f};
@@ -557,17 +586,16 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int c = (v * lpr + lane) * 8;
-      float dg[8];
+      float dg[8], t0[8], t1[8], t2[8];
       const float mp = c < Cr ? m2 : 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        {                                                            // no pre norm: dh = 0
-          const float n = y[v][k] * r_y;
-          acc[3][v][k] += dh[v][k] * n;
-          acc[4][v][k] += dh[v][k];
-          G[v][k] += r_y * (dh[v][k] * wpre[v][k] - n * m1 - (VEC || c + k < Cr ? mp : 0.f));
-        }
+      for (int k = 0; k < 8; ++k) {                                  // no pre norm: dh = 0
+        const float n = y[v][k] * r_y;
+        t0[k] = dh[v][k] * n;
+        G[v][k] += r_y * (dh[v][k] * wpre[v][k] - n * m1 - (VEC || c + k < Cr ? mp : 0.f));
       }
+      add(3, v, t0);
+      add(4, v, dh[v]);
       if (p.d_x) store8<TX, VEC>(static_cast<TX*>(p.d_x) + row * d.ldx, c, Cr, G[v]);
       if (HO) {
 #pragma unroll
@@ -575,16 +603,18 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
           const float n = o[v][k] * r_o;                             // no post norm: deviation 1, weight 1, bias 0
           const float u = n * wpost[v][k] + bpost[v][k];
           const float a = ga[v][k], D = d.alpha * G[v][k];
-          acc[2][v][k] += D * a * u;
+          t2[k] = D * a * u;
           dg[k] = D * sc[v][k] * u * gs[v][k];
-          const float du = D * sc[v][k] * a;
-          acc[0][v][k] += du * n;
-          acc[1][v][k] += du;
+          t1[k] = D * sc[v][k] * a;
+          t0[k] = t1[k] * n;
           o[v][k] = n;
-          G[v][k] = du * wpost[v][k];
+          G[v][k] = t1[k] * wpost[v][k];
           q[0] += G[v][k] * n;
           q[1] += G[v][k];
         }
+        add(0, v, t0);
+        add(1, v, t1);
+        add(2, v, t2);
         if (p.d_gate) {
           if (d.rows_per_gate == 1) {
             store8<TO, VEC>(static_cast<TO*>(p.d_gate) + row * d.ld_dg, c, Cr, dg);
@@ -631,15 +661,15 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int c = (v * lpr + lane) * 8;
-      if (rpb > 1) {                                                // NV == 1 here: several rows only where a row is narrow
-        if (lpr < 64) lane_sums(acc[q][v], lpr, 64);
+      if (!IN_LDS && rpb > 1) {                                     // several rows only where a row is narrow
+        if (lpr < 64) lane_sums(acc[IN_LDS ? 0 : q][IN_LDS ? 0 : v], lpr, 64);
         const int held = lpr < 64 ? blockDim.x >> 6 : rpb;          // sums left per column
         const bool mine = lpr < 64 ? (threadIdx.x & 63) < lpr : true;
         const int slot = lpr < 64 ? threadIdx.x >> 6 : sub;
         __syncthreads();
         if (mine) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) join[(slot * lpr + lane) * 8 + k] = acc[q][v][k];
+          for (int k = 0; k < 8; ++k) join[(slot * lpr + lane) * 8 + k] = acc[IN_LDS ? 0 : q][IN_LDS ? 0 : v][k];
         }
         __syncthreads();
         for (int e = threadIdx.x; e < lpr * 8 && e < C; e += blockDim.x) {
@@ -647,6 +677,10 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
           for (int s = 0; s < held; ++s) t += join[s * lpr * 8 + e];
           out[e] = t;
         }
+      } else if constexpr (IN_LDS) {
+        const f4v a = place_of(q, v)[0], b = place_of(q, v)[GN_MAX_LPR];
+        const float t[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        store8<float, VEC>(out, c, C, t);
       } else {
         store8<float, VEC>(out, c, C, acc[q][v]);
       }
@@ -859,9 +893,24 @@ extern "C" int tg_gated_norm_backward(const tg_gated_norm_desc* d, const void* d
     const double n = (double)d->rows * C, flops = 40 * n, ex = d->res_dtype == TG_F32 ? 4 : 2, eo = d->dtype == TG_F32 ? 4 : 2;
     const double bytes = n * (ex * (1 + (d_y ? 1 : 0) + (d_x ? 1 : 0)) + eo * ((d_h ? 1 : 0) + (o ? 1 : 0) + (d_o ? 1 : 0)));
     const dim3 grid((unsigned)g.blocks), block(g.block);
-    const size_t lds = g.rpb > 1 ? (size_t)g.block * 8 * sizeof(float) : 0;
-    if (vec) GN_PICK(gated_norm_bwd_kernel, true, grid, block, lds, ST(stream), p);
-    else GN_PICK(gated_norm_bwd_kernel, false, grid, block, lds, ST(stream), p);
+    // Wide rows: as many parameter sums at a time as LDS holds beside the row sums' buffers (4 up to 8192 columns, 2 above); passes
+    // that only sum come first, since the outputs may lie over the inputs.
+    const int room = g.nv > 1 ? (int)(159 * 1024 / ((size_t)g.nv * GN_MAX_LPR * 32)) : 5;
+    int left = want;
+    do {
+      p.want = 0;
+      for (int n = 0; left && n < room; ++n) {
+        const int bit = left & -left;
+        p.want |= bit;
+        left ^= bit;
+      }
+      p.d_x = left ? nullptr : d_x;
+      p.d_o = left ? nullptr : d_o;
+      p.d_gate = left ? nullptr : d_gate;
+      const size_t lds = g.nv > 1 ? (size_t)__builtin_popcount(p.want) * g.nv * GN_MAX_LPR * 32 : (g.rpb > 1 ? (size_t)g.block * 8 * sizeof(float) : 0);
+      if (vec) GN_PICK(gated_norm_bwd_kernel, true, grid, block, lds, ST(stream), p);
+      else GN_PICK(gated_norm_bwd_kernel, false, grid, block, lds, ST(stream), p);
+    } while (left);
   }
   const bool gates = d->rows > 0 && d_gate && g.pieces > 0;
   if (want || gates) {

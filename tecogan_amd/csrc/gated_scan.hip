@@ -604,7 +604,8 @@ Plan plan_of(int64_t B, int64_t T, int64_t D) {
       if (blocks > 4096) break;
       continue;
     }
-    const double cost = (double)tpc * cdiv64(blocks, 512) * (blocks < 1024 ? 1.3 : 1.0) * (n == 1 ? 3 : 5) + (n == 1 ? 0 : 13);
+    const double rounds = (double)cdiv64(blocks, 512);
+    const double cost = tpc * rounds * (blocks < 1024 ? 1.3 : 1.0) * (n == 1 ? 3 : 5) + (n == 1 ? 0 : 13 + 0.08 * n * rounds);
     if (p.nc == 0 || cost < best) {
       best = cost;
       p.nc = (int)n;

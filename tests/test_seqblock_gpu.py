@@ -46,6 +46,9 @@ NORM_CASES = [
     (5, 8193, BF, F32, "layer", "rms", 1, "none", True, 1),          # four vectors a lane, scalar path
     (4, 16384, F32, F32, "rms", "layer", 2, "sigmoid", True, 1),     # the widest row
     (2100, 96, BF, BF, "rms", "rms", 700, "none", True, 1),          # pieces of several gate rows
+    (11, 5000, BF, F32, "layer", "layer", 3, "sigmoid", True, 1),    # more parameter sums than one pass over wide rows holds
+    (40, 1003, BF, BF, "layer", "rms", 1, "tanh", True, 1),          # rows that begin at every alignment
+    (40, 1003, F32, F32, "rms", "layer", 8, "silu", True, 1),
 ]
 
 
@@ -235,6 +238,23 @@ def test_gated_norm_in_place_and_empty():
     K.gated_norm_forward(e, e, None, e, e, post=K.NORM_RMS)
     K.gated_norm_backward(e, e, e, e, None, e, e, None, torch.empty(K.gated_norm_ws(0, 128), device=DEV), post=K.NORM_RMS, d_w_pre=d_w)
     assert (d_w == 0).all()
+
+
+@pytest.mark.parametrize("C", [128, 5000])
+def test_gated_norm_gradients_over_their_inputs(C):
+    """d_x over d_y, d_o over d_h's place would be another row's; d_x = d_y and d_o = o are element for element: same bits as apart."""
+    case = (21, C, BF, BF, "layer", "layer", 1, "silu", True, 1)
+    i, p = norm_inputs(case)
+    d_y, d_h = rnd(21, C, seed=11, dtype=BF), rnd(21, C, seed=12, dtype=BF)
+    ws = torch.empty(K.gated_norm_ws(21, C), device=DEV)
+
+    def run(over):
+        a = dict(d_y=dev(d_y), d_h=dev(d_h), y=dev(i["x"]), o=dev(i["o"]), gate=dev(i["gate"]))
+        d_x, d_o, d_g = (a["d_y"], a["o"], a["gate"]) if over else (torch.empty_like(a[n]) for n in ("d_y", "o", "gate"))
+        params = {n: torch.empty(C, device=DEV) for n in ("d_w_post", "d_b_post", "d_scale", "d_w_pre", "d_b_pre")}
+        K.gated_norm_backward(a["d_y"], a["d_h"], a["y"], a["o"], a["gate"], d_x, d_o, d_g, ws, **norm_how(case, p), **params)
+        return [d_x, d_o, d_g] + list(params.values())
+    assert all(torch.equal(a, b) for a, b in zip(run(False), run(True)))
 
 
 def test_gated_norm_rows_of_zeros_and_of_nan_do_not_touch_their_neighbours():
