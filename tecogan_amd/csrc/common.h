@@ -81,8 +81,8 @@ __device__ __forceinline__ uint4 bf8_pack(const float (&f)[8]) {
 // 8 / 4 bytes at any element's address (rows of odd lengths, slices): the device takes them in one instruction, only slower
 struct __attribute__((packed, aligned(2))) Any64 { uint32_t w[2]; };
 struct __attribute__((packed, aligned(2))) Any32 { uint32_t w; };
-// 16 bytes at any even address.  A misaligned 16-byte load runs at a fifth of the bandwidth; the two aligned ones that hold its first
-// and its last byte (both in memory that belongs to the tensor: neither touches another 16-byte granule) and a shift do not.
+// 16 bytes at any even address: the two aligned pieces that hold the first and the last of them (no other granule of 16 is touched),
+// shifted together (quantiser [1000, 1345]: 7.3 us; values fetched one by one 11.4)
 __device__ __forceinline__ uint4 ld128_any(const void* p) {
   const uintptr_t at = reinterpret_cast<uintptr_t>(p);
   const uint4 a = *reinterpret_cast<const uint4*>(at & ~(uintptr_t)15), b = *reinterpret_cast<const uint4*>((at + 15) & ~(uintptr_t)15);
@@ -99,10 +99,6 @@ __device__ __forceinline__ uint4 ld128_any(const void* p) {
   const uint32_t r = s & 3;
   return make_uint4(__builtin_amdgcn_alignbyte(w[1], w[0], r), __builtin_amdgcn_alignbyte(w[2], w[1], r),
                     __builtin_amdgcn_alignbyte(w[3], w[2], r), __builtin_amdgcn_alignbyte(w[4], w[3], r));
-}
-struct __attribute__((packed, aligned(2))) Any128 { uint32_t w[4]; };
-__device__ __forceinline__ void st128_any(void* p, const uint4& v) {
-  *static_cast<Any128*>(p) = Any128{{v.x, v.y, v.z, v.w}};
 }
 
 template <typename T> struct Elem;

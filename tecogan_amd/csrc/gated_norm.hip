@@ -20,55 +20,60 @@ namespace {
 
 typedef float f4v __attribute__((ext_vector_type(4)));
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* __restrict__ row, int c, int C, float (&f)[8]) {
-  if constexpr (VEC) {
-    if (c < C) {
-      if constexpr (sizeof(T) == 2) {
-        bf8_unpack(*reinterpret_cast<const uint4*>(row + c), f);
-      } else {
-        const f4v a = *reinterpret_cast<const f4v*>(row + c), b = *reinterpret_cast<const f4v*>(row + c + 4);
-        f[0] = a[0]; f[1] = a[1]; f[2] = a[2]; f[3] = a[3];
-        f[4] = b[0]; f[5] = b[1]; f[6] = b[2]; f[7] = b[3];
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] = 0.f;
-    }
-  } else if (c + 8 <= C) {                                        // any alignment
-    if constexpr (sizeof(T) == 2) {
-      bf8_unpack(ld128_any(row + c), f);
-    } else {
-      const f4v a = __builtin_bit_cast(f4v, ld128_any(row + c)), b = __builtin_bit_cast(f4v, ld128_any(row + c + 4));
-      f[0] = a[0]; f[1] = a[1]; f[2] = a[2]; f[3] = a[3];
-      f[4] = b[0]; f[5] = b[1]; f[6] = b[2]; f[7] = b[3];
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = c + k < C ? Elem<T>::ld(row + c + k) : 0.f;
-  }
-}
-
-// The same 8 values as they lie in memory: what is fetched a row ahead
-template <typename T, bool VEC> struct Raw8 {
-  float f[8];
-  __device__ __forceinline__ void load(const T* __restrict__ row, int c, int C) { load8<T, VEC>(row, c, C, f); }
-  __device__ __forceinline__ void values(float (&v)[8]) const {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = f[k];
-  }
+// A lane's 8 values of a vector: neighbours (VEC: 16-byte loads), or, where a row's length, stride or address is no multiple of 8
+// values, every lpr-th: single loads in which a wave still reads one stretch of memory, and no case for a row's end (52600 rows of 775
+// bf16 values: 178 us; 16 bytes at a time from odd addresses 401, and 776 values 83).
+template <bool VEC> struct Cols {
+  static __device__ __forceinline__ int first(int v, int lane, int lpr) { return VEC ? (v * lpr + lane) * 8 : v * lpr * 8 + lane; }
+  static __device__ __forceinline__ int step(int lpr) { return VEC ? 1 : lpr; }
 };
+
+// The 8 values as they lie in memory: what is fetched a row ahead.  C: the row's columns, 0 for a row past the end, which reads nothing;
+// values past them are 0.
+template <typename T, bool VEC> struct Raw8;
 template <> struct Raw8<u16, true> {
   uint4 w;
-  __device__ __forceinline__ void load(const u16* __restrict__ row, int c, int C) {
+  __device__ __forceinline__ void load(const u16* __restrict__ row, int c, int, int C) {
     w = make_uint4(0, 0, 0, 0);
     if (c < C) w = *reinterpret_cast<const uint4*>(row + c);
   }
   __device__ __forceinline__ void values(float (&v)[8]) const { bf8_unpack(w, v); }
 };
+template <> struct Raw8<float, true> {
+  f4v a, b;
+  __device__ __forceinline__ void load(const float* __restrict__ row, int c, int, int C) {
+    a = b = f4v{0.f, 0.f, 0.f, 0.f};
+    if (c < C) {
+      a = *reinterpret_cast<const f4v*>(row + c);
+      b = *reinterpret_cast<const f4v*>(row + c + 4);
+    }
+  }
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+    v[0] = a[0]; v[1] = a[1]; v[2] = a[2]; v[3] = a[3];
+    v[4] = b[0]; v[5] = b[1]; v[6] = b[2]; v[7] = b[3];
+  }
+};
+template <typename T> struct Raw8<T, false> {
+  T w[8];
+  int left, step;
+  __device__ __forceinline__ void load(const T* __restrict__ row, int c, int st, int C) {
+    left = C - c;
+    step = st;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = T(0);
+    if (C > 0) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w[k] = row[min(c + k * st, C - 1)];
+    }
+  }
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = k * step < left ? Elem<T>::ld(&w[k]) : 0.f;
+  }
+};
 
 template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* __restrict__ row, int c, int C, const float (&f)[8]) {
+__device__ __forceinline__ void store8(T* __restrict__ row, int c, int st, int C, const float (&f)[8]) {
   if constexpr (VEC) {
     if (c >= C) return;
     if constexpr (sizeof(T) == 2) {
@@ -77,46 +82,24 @@ __device__ __forceinline__ void store8(T* __restrict__ row, int c, int C, const 
       *reinterpret_cast<f4v*>(row + c) = f4v{f[0], f[1], f[2], f[3]};
       *reinterpret_cast<f4v*>(row + c + 4) = f4v{f[4], f[5], f[6], f[7]};
     }
-  } else if (c + 8 <= C) {
-    if constexpr (sizeof(T) == 2) {
-      st128_any(row + c, bf8_pack(f));
-    } else {
-      st128_any(row + c, __builtin_bit_cast(uint4, f4v{f[0], f[1], f[2], f[3]}));
-      st128_any(row + c + 4, __builtin_bit_cast(uint4, f4v{f[4], f[5], f[6], f[7]}));
-    }
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      if (c + k < C) Elem<T>::st(row + c + k, f[k]);
+      if (c + k * st < C) Elem<T>::st(row + c + k * st, f[k]);
   }
 }
 
 // fp32 parameter vector (nullable): its 8 values, or `other`
 template <bool VEC>
-__device__ __forceinline__ void param8(const float* __restrict__ p, int c, int C, float other, float (&f)[8]) {
-  f4v a = {other, other, other, other}, b = a;
+__device__ __forceinline__ void param8(const float* __restrict__ p, int c, int st, int C, float other, float (&f)[8]) {
   if (p) {
-    if constexpr (VEC) {
-      if (c < C) {
-        a = *reinterpret_cast<const f4v*>(p + c);
-        b = *reinterpret_cast<const f4v*>(p + c + 4);
-      }
-    } else if (c + 8 <= C) {
-      a = __builtin_bit_cast(f4v, ld128_any(p + c));
-      b = __builtin_bit_cast(f4v, ld128_any(p + c + 4));
-    } else {
-      if (c + 0 < C) a[0] = p[c + 0];
-      if (c + 1 < C) a[1] = p[c + 1];
-      if (c + 2 < C) a[2] = p[c + 2];
-      if (c + 3 < C) a[3] = p[c + 3];
-      if (c + 4 < C) b[0] = p[c + 4];
-      if (c + 5 < C) b[1] = p[c + 5];
-      if (c + 6 < C) b[2] = p[c + 6];
-      if (c + 7 < C) b[3] = p[c + 7];
-    }
+    Raw8<float, VEC> raw;
+    raw.load(p, c, st, C);
+    raw.values(f);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = other;
   }
-  f[0] = a[0]; f[1] = a[1]; f[2] = a[2]; f[3] = a[3];
-  f[4] = b[0]; f[5] = b[1]; f[6] = b[2]; f[7] = b[3];
 }
 
 // sigmoid(v) and sigmoid(-v) without a difference: e = exp(-|v|), 1 / (1 + e) and e / (1 + e)
@@ -295,21 +278,21 @@ __global__ __launch_bounds__(512) void gated_norm_fwd_kernel(GnP p) {
   const bool HO = MODE == 3 ? p.o != nullptr : MODE >= 1, HG = MODE == 3 ? p.gate != nullptr : MODE == 2;
   const tg_gated_norm_desc& d = p.d;
   const int lpr = 1 << p.lpr_log2, lane = threadIdx.x & (lpr - 1), sub = threadIdx.x >> p.lpr_log2, rpb = blockDim.x >> p.lpr_log2;
-  const int C = d.C;
+  const int C = d.C, st = Cols<VEC>::step(lpr);
   float wpo[NV][8], bpo[NV][8], sc[NV][8], wpr[NV][8], bpr[NV][8];
   auto params = [&]() {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = (v * lpr + lane) * 8;
+      const int c = Cols<VEC>::first(v, lane, lpr);
       if (HO) {
-        param8<VEC>(p.w_post, c, C, 1.f, wpo[v]);
-        param8<VEC>(p.b_post, c, C, 0.f, bpo[v]);
-        param8<VEC>(p.scale, c, C, 1.f, sc[v]);
+        param8<VEC>(p.w_post, c, st, C, 1.f, wpo[v]);
+        param8<VEC>(p.b_post, c, st, C, 0.f, bpo[v]);
+        param8<VEC>(p.scale, c, st, C, 1.f, sc[v]);
 #pragma unroll
         for (int k = 0; k < 8; ++k) sc[v][k] *= d.alpha;
       }
-      param8<VEC>(p.w_pre, c, C, 1.f, wpr[v]);
-      param8<VEC>(p.b_pre, c, C, 0.f, bpr[v]);
+      param8<VEC>(p.w_pre, c, st, C, 1.f, wpr[v]);
+      param8<VEC>(p.b_pre, c, st, C, 0.f, bpr[v]);
     }
   };
   const int64_t row0 = (int64_t)blockIdx.x * rpb + sub, step = (int64_t)gridDim.x * rpb;
@@ -325,10 +308,10 @@ __global__ __launch_bounds__(512) void gated_norm_fwd_kernel(GnP p) {
     const TO* pg = static_cast<const TO*>(p.gate) + (int64_t)p.gate_of.of((uint32_t)row) * d.ldg;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = (v * lpr + lane) * 8;
-      rx[v].load(px, c, Cr);
-      if (HO) ro[v].load(po, c, Cr);
-      if (HG) rg[v].load(pg, c, Cr);
+      const int c = Cols<VEC>::first(v, lane, lpr);
+      rx[v].load(px, c, st, Cr);
+      if (HO) ro[v].load(po, c, st, Cr);
+      if (HG) rg[v].load(pg, c, st, Cr);
     }
     px += sx;
     po += so;
@@ -368,11 +351,11 @@ __global__ __launch_bounds__(512) void gated_norm_fwd_kernel(GnP p) {
         float s[1] = {0.f};
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-          const int c = (v * lpr + lane) * 8;
+          const int c = Cols<VEC>::first(v, lane, lpr);
           const float mv = c < Cr ? mu : 0.f;                       // values past the end are 0 and stay 0
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const float t = u[v][k] - (VEC || c + k < Cr ? mv : 0.f);
+            const float t = u[v][k] - (VEC || c + k * st < Cr ? mv : 0.f);
             s[0] += t * t;
           }
         }
@@ -381,14 +364,14 @@ __global__ __launch_bounds__(512) void gated_norm_fwd_kernel(GnP p) {
       }
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        const int c = (v * lpr + lane) * 8;
+        const int c = Cols<VEC>::first(v, lane, lpr);
         if (HG) gate_values(g[v], d.gate_act);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const float t = (u[v][k] - mu) * (r * wpo[v][k]) + bpo[v][k];
           x[v][k] += (HG ? sc[v][k] * g[v][k] : sc[v][k]) * t;
         }
-        store8<TX, VEC>(py, c, Cr, x[v]);
+        store8<TX, VEC>(py, c, st, Cr, x[v]);
       }
     }
     if (d.pre != TG_NORM_NONE) {
@@ -397,10 +380,10 @@ __global__ __launch_bounds__(512) void gated_norm_fwd_kernel(GnP p) {
         float s[1] = {0.f};
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-          const int c = (v * lpr + lane) * 8;
+          const int c = Cols<VEC>::first(v, lane, lpr);
           float t = 0.f;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) t += VEC || c + k < Cr ? x[v][k] : 0.f;
+          for (int k = 0; k < 8; ++k) t += VEC || c + k * st < Cr ? x[v][k] : 0.f;
           s[0] += c < Cr ? t : 0.f;
         }
         row_sums(s, lpr, red, turn);
@@ -409,12 +392,12 @@ __global__ __launch_bounds__(512) void gated_norm_fwd_kernel(GnP p) {
       float s[1] = {0.f};
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        const int c = (v * lpr + lane) * 8;
+        const int c = Cols<VEC>::first(v, lane, lpr);
         float q = 0.f;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const float t = x[v][k] - mu;
-          q += VEC || c + k < Cr ? t * t : 0.f;
+          q += VEC || c + k * st < Cr ? t * t : 0.f;
         }
         s[0] += c < Cr ? q : 0.f;
       }
@@ -424,7 +407,7 @@ __global__ __launch_bounds__(512) void gated_norm_fwd_kernel(GnP p) {
       for (int v = 0; v < NV; ++v) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) x[v][k] = (x[v][k] - mu) * (r * wpr[v][k]) + bpr[v][k];
-        store8<TO, VEC>(ph, (v * lpr + lane) * 8, Cr, x[v]);
+        store8<TO, VEC>(ph, Cols<VEC>::first(v, lane, lpr), st, Cr, x[v]);
       }
     }
   }
@@ -439,7 +422,7 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
   constexpr bool IN_LDS = NV > 1;                                   // the parameter sums of wide rows: no registers for them
   const tg_gated_norm_desc& d = p.d;
   const int lpr = 1 << p.lpr_log2, lane = threadIdx.x & (lpr - 1), sub = threadIdx.x >> p.lpr_log2, rpb = blockDim.x >> p.lpr_log2;
-  const int C = d.C;
+  const int C = d.C, st = Cols<VEC>::step(lpr);
   const int64_t item = (int64_t)blockIdx.x * rpb + sub;
   int64_t start, end;
   if (p.pieces > 0) {
@@ -483,12 +466,12 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
     const int64_t r = row < end ? row : 0;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = (v * lpr + lane) * 8;
-      ry[v].load(static_cast<const TX*>(p.y) + r * d.ldy, c, Cr);
-      if (p.d_h) rdh[v].load(static_cast<const TO*>(p.d_h) + r * d.ldh, c, Cr);
-      if (p.d_y) rdy[v].load(static_cast<const TX*>(p.d_y) + r * d.ld_dy, c, Cr);
-      if (HO) ro[v].load(static_cast<const TO*>(p.o) + r * d.ldo, c, Cr);
-      if (HG) rg[v].load(static_cast<const TO*>(p.gate) + (int64_t)p.gate_of.of((uint32_t)r) * d.ldg, c, Cr);
+      const int c = Cols<VEC>::first(v, lane, lpr);
+      ry[v].load(static_cast<const TX*>(p.y) + r * d.ldy, c, st, Cr);
+      if (p.d_h) rdh[v].load(static_cast<const TO*>(p.d_h) + r * d.ldh, c, st, Cr);
+      if (p.d_y) rdy[v].load(static_cast<const TX*>(p.d_y) + r * d.ld_dy, c, st, Cr);
+      if (HO) ro[v].load(static_cast<const TO*>(p.o) + r * d.ldo, c, st, Cr);
+      if (HG) rg[v].load(static_cast<const TO*>(p.gate) + (int64_t)p.gate_of.of((uint32_t)r) * d.ldg, c, st, Cr);
     }
   };
   float ga[NV][8], gs[NV][8];                                       // the gate's activation and its derivative
@@ -501,11 +484,11 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
   auto params = [&]() {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = (v * lpr + lane) * 8;
-      param8<VEC>(p.w_pre, c, C, 1.f, wpre[v]);
-      param8<VEC>(p.w_post, c, C, 1.f, wpost[v]);
-      param8<VEC>(p.b_post, c, C, 0.f, bpost[v]);
-      param8<VEC>(p.scale, c, C, 1.f, sc[v]);
+      const int c = Cols<VEC>::first(v, lane, lpr);
+      param8<VEC>(p.w_pre, c, st, C, 1.f, wpre[v]);
+      param8<VEC>(p.w_post, c, st, C, 1.f, wpost[v]);
+      param8<VEC>(p.b_post, c, st, C, 0.f, bpost[v]);
+      param8<VEC>(p.scale, c, st, C, 1.f, sc[v]);
     }
   };
   int turn = 0;
@@ -566,12 +549,12 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
     float s[4] = {0.f, 0.f, 0.f, 0.f};                              // |y - mu|^2, t (y - mu), t, |o - mu|^2 with t = dh w_pre
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = (v * lpr + lane) * 8;
+      const int c = Cols<VEC>::first(v, lane, lpr);
       const float my = c < Cr ? mu_y : 0.f, mo = c < Cr ? mu_o : 0.f;   // values past the end are 0 and stay 0
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        y[v][k] -= VEC || c + k < Cr ? my : 0.f;
-        o[v][k] -= VEC || c + k < Cr ? mo : 0.f;
+        y[v][k] -= VEC || c + k * st < Cr ? my : 0.f;
+        o[v][k] -= VEC || c + k * st < Cr ? mo : 0.f;
         const float t = dh[v][k] * wpre[v][k];
         s[0] += y[v][k] * y[v][k];
         s[1] += t * y[v][k];
@@ -585,18 +568,18 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
     float q[2] = {0.f, 0.f};                                        // t o^, t with t = du w_post
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = (v * lpr + lane) * 8;
+      const int c = Cols<VEC>::first(v, lane, lpr);
       float dg[8], t0[8], t1[8], t2[8];
       const float mp = c < Cr ? m2 : 0.f;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {                                  // no pre norm: dh = 0
         const float n = y[v][k] * r_y;
         t0[k] = dh[v][k] * n;
-        G[v][k] += r_y * (dh[v][k] * wpre[v][k] - n * m1 - (VEC || c + k < Cr ? mp : 0.f));
+        G[v][k] += r_y * (dh[v][k] * wpre[v][k] - n * m1 - (VEC || c + k * st < Cr ? mp : 0.f));
       }
       add(3, v, t0);
       add(4, v, dh[v]);
-      if (p.d_x) store8<TX, VEC>(static_cast<TX*>(p.d_x) + row * d.ldx, c, Cr, G[v]);
+      if (p.d_x) store8<TX, VEC>(static_cast<TX*>(p.d_x) + row * d.ldx, c, st, Cr, G[v]);
       if (HO) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -617,7 +600,7 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
         add(2, v, t2);
         if (p.d_gate) {
           if (d.rows_per_gate == 1) {
-            store8<TO, VEC>(static_cast<TO*>(p.d_gate) + row * d.ld_dg, c, Cr, dg);
+            store8<TO, VEC>(static_cast<TO*>(p.d_gate) + row * d.ld_dg, c, st, Cr, dg);
           } else {
 #pragma unroll
             for (int k = 0; k < 8; ++k) dga[v][k] += dg[k];
@@ -631,18 +614,18 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
         const float n1 = d.post != TG_NORM_NONE ? q[0] * p.inv_c : 0.f, n2 = d.post == TG_NORM_LAYER ? q[1] * p.inv_c : 0.f;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-          const int c = (v * lpr + lane) * 8;
+          const int c = Cols<VEC>::first(v, lane, lpr);
           float out[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k) out[k] = r_o * (G[v][k] - o[v][k] * n1 - n2);
-          store8<TO, VEC>(static_cast<TO*>(p.d_o) + row * d.ld_do, c, Cr, out);
+          store8<TO, VEC>(static_cast<TO*>(p.d_o) + row * d.ld_do, c, st, Cr, out);
         }
       }
       // the last row of a gate row in this item: its sum is complete (whole gate rows only)
       if (p.d_gate && p.pieces == 0 && d.rows_per_gate > 1 && on && (row + 1 == d.rows || (row + 1) % d.rows_per_gate == 0)) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-          store8<TO, VEC>(static_cast<TO*>(p.d_gate) + grow * d.ld_dg, (v * lpr + lane) * 8, C, dga[v]);
+          store8<TO, VEC>(static_cast<TO*>(p.d_gate) + grow * d.ld_dg, Cols<VEC>::first(v, lane, lpr), st, C, dga[v]);
 #pragma unroll
           for (int k = 0; k < 8; ++k) dga[v][k] = 0.f;
         }
@@ -651,7 +634,7 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
   }
   if (p.pieces > 0 && item < p.items) {
 #pragma unroll
-    for (int v = 0; v < NV; ++v) store8<float, VEC>(p.gate_part + item * C, (v * lpr + lane) * 8, C, dga[v]);
+    for (int v = 0; v < NV; ++v) store8<float, VEC>(p.gate_part + item * C, Cols<VEC>::first(v, lane, lpr), st, C, dga[v]);
   }
   // the workgroup's parameter sums: over the rows of a wave by lane exchange, then over the waves through LDS
 #pragma unroll
@@ -660,7 +643,7 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
     float* out = p.part + ((int64_t)blockIdx.x * 5 + q) * C;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = (v * lpr + lane) * 8;
+      const int c = Cols<VEC>::first(v, lane, lpr);
       if (!IN_LDS && rpb > 1) {                                     // several rows only where a row is narrow
         if (lpr < 64) lane_sums(acc[IN_LDS ? 0 : q][IN_LDS ? 0 : v], lpr, 64);
         const int held = lpr < 64 ? blockDim.x >> 6 : rpb;          // sums left per column
@@ -669,7 +652,7 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
         __syncthreads();
         if (mine) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) join[(slot * lpr + lane) * 8 + k] = acc[IN_LDS ? 0 : q][IN_LDS ? 0 : v][k];
+          for (int k = 0; k < 8; ++k) join[slot * lpr * 8 + Cols<VEC>::first(0, lane, lpr) + k * st] = acc[IN_LDS ? 0 : q][IN_LDS ? 0 : v][k];
         }
         __syncthreads();
         for (int e = threadIdx.x; e < lpr * 8 && e < C; e += blockDim.x) {
@@ -680,9 +663,9 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
       } else if constexpr (IN_LDS) {
         const f4v a = place_of(q, v)[0], b = place_of(q, v)[GN_MAX_LPR];
         const float t[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-        store8<float, VEC>(out, c, C, t);
+        store8<float, VEC>(out, c, st, C, t);
       } else {
-        store8<float, VEC>(out, c, C, acc[q][v]);
+        store8<float, VEC>(out, c, st, C, acc[q][v]);
       }
     }
   }

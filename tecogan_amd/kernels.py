@@ -716,27 +716,37 @@ def _fp8_operand(q, s, what):
     return fmt, rows, cols, int(s.shape[0] != rows)
 
 
+def _fp8_result(q, s, rows, cols, tile, what):
+    """Format of a quantised matrix to be written (None: not wanted), checked."""
+    if (q is None) != (s is None):
+        raise L.TecoHipError("%s goes with its scales" % what)
+    if q is None:
+        return None
+    sq, ss = _fp8_shapes(rows, cols, tile)
+    fmt = _FP8.get(q.dtype)
+    if fmt is None or q.shape != sq or not q.is_contiguous():
+        raise L.TecoHipError("%s: contiguous 8-bit floats %s expected" % (what, sq))
+    if s.dtype is not torch.uint8 or s.shape != ss or not s.is_contiguous():
+        raise L.TecoHipError("%s: contiguous uint8 scales %s expected" % (what, ss))
+    return fmt
+
+
 def fp8_quantize(x, q, scale, qt=None, scale_t=None, tile=False):
     """x [..., cols] (bf16 / f32) as 8-bit floating point with one power-of-two scale for each block of 128: q with its blocks along
     the columns, qt (the transposed copy) with its blocks along the rows; `tile`: one scale for each 128 x 128 tile in both.  Either
     copy may be None with its scales.  Shapes: fp8_alloc.  A NaN or infinity stays one and does not touch its block's scale."""
     stream = _on_device(x, q, scale, qt, scale_t)
     cols = x.shape[-1] if x.dim() else 0
-    _need(cols >= 1, "x: [..., columns] expected")
+    if cols < 1 or (q is None and qt is None):
+        raise L.TecoHipError("x [..., columns] and at least one order of the result are expected")
     rows = x.numel() // cols
     px, ld = _rows(x, rows, cols, x.dtype, "x")
-    _need(q is not None or qt is not None, "neither order is asked for")
-    fmts = set()
-    for t, s, a, b, what in ((q, scale, rows, cols, "q"), (qt, scale_t, cols, rows, "qt")):
-        _need((t is None) == (s is None), "%s goes with its scales" % what)
-        if t is not None:
-            sq, ss = _fp8_shapes(a, b, tile)
-            _need(t.dtype in _FP8 and tuple(t.shape) == sq and t.is_contiguous(), "%s: contiguous 8-bit floats %s expected" % (what, sq))
-            _need(s.dtype == torch.uint8 and tuple(s.shape) == ss and s.is_contiguous(), "%s: contiguous uint8 scales %s expected" % (what, ss))
-            fmts.add(_FP8[t.dtype])
-    _need(len(fmts) == 1, "q and qt must have the same type")
-    check(lib().tg_fp8_quantize(px, dt(x), rows, cols, ld, fmts.pop(), int(bool(tile)), _at(q), _at(scale), _at(qt), _at(scale_t), stream),
-          "tg_fp8_quantize")
+    fmt = _fp8_result(q, scale, rows, cols, tile, "q")
+    fmt_t = _fp8_result(qt, scale_t, cols, rows, tile, "qt")
+    if q is not None and qt is not None and fmt != fmt_t:
+        raise L.TecoHipError("q and qt must have the same type")
+    check(lib().tg_fp8_quantize(px, dt(x), rows, cols, ld, fmt if q is not None else fmt_t, int(bool(tile)), _at(q), _at(scale), _at(qt),
+                                _at(scale_t), stream), "tg_fp8_quantize")
 
 
 def fp8_matmul(a, scale_a, b, scale_b, out, bias=None, accumulate=False):
@@ -803,10 +813,12 @@ def _steps(t, shape, dtype, what):
         raise L.TecoHipError("%s: %s of %s expected, got %s of %s" % (what, shape, dtype, tuple(t.shape), t.dtype))
     B, T, D = shape
     sb, st, sd = t.stride()
-    _need(sd == 1 or D == 1, "%s: channels must be contiguous" % what)
     st = D if T == 1 else st
     sb = T * st if B == 1 else sb
-    _need(st >= D and sb >= D, "%s: steps overlap" % what)
+    if sd != 1 and D != 1:
+        raise L.TecoHipError("%s: channels must be contiguous" % what)
+    if st < D or sb < D:
+        raise L.TecoHipError("%s: steps overlap" % what)
     return t.data_ptr(), st, sb
 
 
@@ -821,9 +833,9 @@ def gated_scan_forward(x, g, y, hT, carry, h0=None, floor=None, lengths=None, re
     """h[t] = f[t] h[t-1] + (1 - f[t]) x[t], f = floor + (1 - floor) sigmoid(g), along dimension 1 of x, g, y [B, T, D] (bf16 / f32,
     channels contiguous); y = h, hT [B, D] fp32 or None = the last state.  h0 [B, D] fp32: the state before (None: zero); floor [D]
     fp32 in [0, 1); lengths [B] int32: steps at and behind a row's length keep the state and write y = 0; reset [B, T] bytes: not 0
-    drops the state before the step (packed sequences).  carry: fp32, gated_scan_carry(B, T, D) values; with `keep` it holds what
-    gated_scan_backward needs.  Without, carry may be None where the
-    sequence needs no scratch (up to 64 steps always; longer ones are refused where they are cut into chunks).  Returns y."""
+    drops the state before the step (packed sequences).
+    carry: fp32, gated_scan_carry(B, T, D) values; with `keep` it holds what gated_scan_backward needs.  Without, carry may be None
+    where the sequence needs no scratch (up to 64 steps always; longer ones are refused where they are cut into chunks).  Returns y."""
     stream = _on_device(x, g, y, hT, carry, h0, floor, lengths, reset)
     _need(x.dim() == 3 and x.shape[1] >= 1, "x: [B, T, D] with T >= 1 expected")
     shape = tuple(x.shape)
