@@ -100,12 +100,18 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rsrc, unsigned char
 // up: b1, a1 of this block, then a0 and -- column by column, as (a1, b0) finishes with them -- b0 of the next.  The one barrier of a
 // block sits in its middle: there every wave has read the last of this stage and its own DMA of the next stage has landed; the DMA
 // of block kb + S goes out between the products of the second half.
-template <int FB, int FA, bool WIDE, int MF, int NF, int S>
-__global__ __launch_bounds__(256, MF * NF >= 64 ? 1 : 2) void fp8_tile_kernel(MmP p) {
+//
+// G groups of four waves share a tile: group j takes the blocks j, j + G, ... of K through stages of its own, and the groups' sums meet in
+// LDS in the groups' order.  A block of the smallest tile costs its waves
+// about 800 cycles, most of them waits (barrier, LDS, products, in turn); G groups wait at the same time.
+template <int FB, int FA, bool WIDE, int MF, int NF, int S, int G>
+__global__ __launch_bounds__(256 * G, MF * NF >= 64 || G > 1 ? 1 : 2) void fp8_tile_kernel(MmP p) {
   constexpr int TM = 32 * MF, TN = 32 * NF, STAGE = (TM + TN) * 132, HM = MF / 2, HN = NF / 2;
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g = lane >> 4;
+  extern __shared__ __attribute__((aligned(16))) unsigned char tile_lds[];
+  const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
+  const int grp = G > 1 ? __builtin_amdgcn_readfirstlane(tid >> 8) : 0, wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 3);
   const int wm = wave >> 1, wn = wave & 1;
+  unsigned char* const smem = tile_lds + grp * S * STAGE;
   // tile of this workgroup: XCD x (linear id % 8) owns consecutive tiles of an order that walks 8 tile rows down before the next column
   int t = blockIdx.x;
   {
@@ -116,7 +122,8 @@ __global__ __launch_bounds__(256, MF * NF >= 64 ? 1 : 2) void fp8_tile_kernel(Mm
   const int64_t m0 = (int64_t)__builtin_amdgcn_readfirstlane(band * 8 + rest % deep) * TM;
   const int64_t n0 = (int64_t)__builtin_amdgcn_readfirstlane(rest / deep) * TN;
 
-  const int rows_a = (int)(p.M - m0 < TM ? p.M - m0 : TM), rows_b = (int)(p.N - n0 < TN ? p.N - n0 : TN), nkb = p.K >> 7;
+  const int rows_a = (int)(p.M - m0 < TM ? p.M - m0 : TM), rows_b = (int)(p.N - n0 < TN ? p.N - n0 : TN);
+  const int all = p.K >> 7, turns = (all + G - 1) / G, nkb = (all - grp + G - 1) / G;   // blocks of K, of the busiest group, of this one
   const auto rsrcA = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.a + m0 * p.K), 0, rows_a * p.K, 0x00020000);
   const auto rsrcB = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.b + n0 * p.K), 0, rows_b * p.K, 0x00020000);
   int oa[MF], ob[NF];                                                 // DMA sources: rows past the end read the last one (not stored)
@@ -130,7 +137,8 @@ __global__ __launch_bounds__(256, MF * NF >= 64 ? 1 : 2) void fp8_tile_kernel(Mm
     const int row = (wave * NF + i) * 8 + (lane >> 3);
     ob[i] = (row < rows_b ? row : rows_b - 1) * p.K + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
   }
-  auto dma_at = [&](int q, int stage, int kb) {                       // instruction q of block kb into stage % S
+  auto dma_at = [&](int q, int stage, int i) {                        // instruction q of the group's block i into stage % S
+    const int kb = grp + G * i;
     unsigned char* const st = smem + (stage & (S - 1)) * STAGE;
     if (q < MF) dma16(rsrcA, st + (wave * MF + q) * 1024, oa[q < MF ? q : 0], kb * 128);
     else dma16(rsrcB, st + TM * 128 + (wave * NF + q - MF) * 1024, ob[q < MF ? 0 : q - MF], kb * 128);
@@ -146,13 +154,14 @@ __global__ __launch_bounds__(256, MF * NF >= 64 ? 1 : 2) void fp8_tile_kernel(Mm
     if (ch * 64 < TM) os[i] = ((row < rows_a ? row : rows_a - 1) >> p.sh_a) * p.sp;
     else os[i] = ((row < rows_b ? row : rows_b - 1) >> p.sh_b) * p.sp;
   }
-  auto dma_scales_at = [&](int stage, int kb) {
+  auto dma_scales_at = [&](int stage, int k) {
+    const int at = (grp + G * k) & ~3;
     unsigned char* const st = smem + (stage & (S - 1)) * STAGE + (TM + TN) * 128;
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
       const int ch = (wave + 4 * i) % NCH;
-      if (ch * 64 < TM) dma4(rsrcSA, st + ch * 256, os[i], kb & ~3);
-      else dma4(rsrcSB, st + ch * 256, os[i], kb & ~3);
+      if (ch * 64 < TM) dma4(rsrcSA, st + ch * 256, os[i], at);
+      else dma4(rsrcSB, st + ch * 256, os[i], at);
     }
   };
 
@@ -171,7 +180,7 @@ __global__ __launch_bounds__(256, MF * NF >= 64 ? 1 : 2) void fp8_tile_kernel(Mm
   const unsigned char* const bbh = smem + ((TM * 128 + wn * 16 * NF * 128 + la) ^ 64);
   const unsigned char* const psa = smem + (TM + TN) * 128 + (wm * 16 * MF + r16) * 4;
   const unsigned char* const psb = smem + (TM + TN) * 128 + (TM + wn * 16 * NF + r16) * 4;
-  const unsigned char *pal = bal, *pah = bah, *pbl = bbl, *pbh = bbh, *qsa = psa, *qsb = psb;
+  const unsigned char *pal = bal, *pah = bah, *pbl = bbl, *pbh = bbh, *qsa = psa + (G > 1 ? grp & 3 : 0), *qsb = psb + (G > 1 ? grp & 3 : 0);
   auto frag = [](const unsigned char* lo, const unsigned char* hi) {
     return __builtin_shufflevector(*reinterpret_cast<const i32x4m*>(lo), *reinterpret_cast<const i32x4m*>(hi), 0, 1, 2, 3, 4, 5, 6, 7);
   };
@@ -183,7 +192,7 @@ __global__ __launch_bounds__(256, MF * NF >= 64 ? 1 : 2) void fp8_tile_kernel(Mm
     fb[h][u] = frag(pbl + (h * HN + u) * 2048, pbh + (h * HN + u) * 2048);
     cb[h][u] = qsb[(h * HN + u) * 64];
   };
-  // what is read from here on is block kb
+  // what is read from here on is the group's block kb
   int shift = STAGE;
   auto turn = [&](int kb) {
     const int st = (kb & (S - 1)) * STAGE;
@@ -193,8 +202,8 @@ __global__ __launch_bounds__(256, MF * NF >= 64 ? 1 : 2) void fp8_tile_kernel(Mm
     } else {
       pal = bal + st; pah = bah + st; pbl = bbl + st; pbh = bbh + st;
     }
-    qsa = psa + st + (kb & 3);
-    qsb = psb + st + (kb & 3);
+    qsa = psa + st + ((grp + G * kb) & 3);
+    qsb = psb + st + ((grp + G * kb) & 3);
   };
   // A quarter's products, columns outermost; after(x) follows product x of HM HN
   auto quarter = [&](int ha, int hb, auto after) {
@@ -274,6 +283,18 @@ __global__ __launch_bounds__(256, MF * NF >= 64 ? 1 : 2) void fp8_tile_kernel(Mm
     asm volatile("s_waitcnt vmcnt(0)\n\ts_nop 15\n\ts_nop 15" ::: "memory");   // no DMA outlives the workgroup
 #pragma unroll
     for (int i = 0; i < MF; ++i) settle(acc[i]);
+  } else if (G > 1 && all > 0) {                                       // a group without a block: the barrier in front of the loop
+    __builtin_amdgcn_s_barrier();
+  }
+  if constexpr (G > 1) {
+    if (nkb < turns) __builtin_amdgcn_s_barrier();                     // a group with one block less than the others
+    __syncthreads();
+    f32x4* const mine = reinterpret_cast<f32x4*>(tile_lds) + (grp * 4 + wave) * MF * NF * 64 + lane;
+#pragma unroll
+    for (int i = 0; i < MF; ++i)
+#pragma unroll
+      for (int j = 0; j < NF; ++j) mine[(i * NF + j) * 64] = acc[i][j];
+    __syncthreads();
   }
 #pragma unroll
   for (int i = 0; i < MF; ++i) {
@@ -282,8 +303,14 @@ __global__ __launch_bounds__(256, MF * NF >= 64 ? 1 : 2) void fp8_tile_kernel(Mm
 #pragma unroll
     for (int j = 0; j < NF; ++j) {
       const int64_t n = n0 + wn * 16 * NF + 16 * j + 4 * g;
-      if (n >= p.N) continue;
+      if (n >= p.N || (G > 1 && (i * NF + j) % G != grp)) continue;     // each group writes its share
       f32x4 v = acc[i][j];
+      if constexpr (G > 1) {
+        const f32x4* const sums = reinterpret_cast<const f32x4*>(tile_lds) + (wave * MF * NF + i * NF + j) * 64 + lane;
+        v = sums[0];
+#pragma unroll
+        for (int q = 1; q < G; ++q) v += sums[q * 4 * MF * NF * 64];
+      }
       if (p.vec) {
         if (p.bias) v += *reinterpret_cast<const f32x4*>(p.bias + n);
         if constexpr (!WIDE) {
@@ -312,21 +339,30 @@ __global__ __launch_bounds__(256, MF * NF >= 64 ? 1 : 2) void fp8_tile_kernel(Mm
 }
 
 // hipFuncAttributeMaxDynamicSharedMemorySize is not needed on this device; a launch may ask for up to 160 KB.
-template <int FB, int FA, bool WIDE, int MF, int NF, int S>
+template <int FB, int FA, bool WIDE, int MF, int NF, int S, int G>
 void launch_tile(MmP p, const char* name, double flops, double bytes, hipStream_t st) {
   p.tiles_m = (int)cdiv64(p.M, 32 * MF);
   p.tiles_n = (int)cdiv64(p.N, 32 * NF);
   p.tiles = p.tiles_m * p.tiles_n;
-  constexpr int lds = S * (32 * MF + 32 * NF) * 132;
-  TG_LAUNCH(name, flops, bytes, (fp8_tile_kernel<FB, FA, WIDE, MF, NF, S>), dim3((unsigned)p.tiles), dim3(256), lds, st, p);
+  constexpr int lds = G * S * (32 * MF + 32 * NF) * 132;
+  static_assert(G == 1 || (MF * NF >= G && lds >= G * 4 * MF * NF * 1024), "the groups' sums lie in the stages");
+  TG_LAUNCH(name, flops, bytes, (fp8_tile_kernel<FB, FA, WIDE, MF, NF, S, G>), dim3((unsigned)p.tiles), dim3(256 * G), lds, st, p);
 }
 
+// The largest tile that still gives most compute units one, and what else of a unit it leaves free: with at most one tile a unit its LDS
+// holds more stages (1024 x 4096 x 4096, bf16 out: 28 us with two, 23 with four) or groups of waves (64 x 4096 x 4096: bf16 out 12.1 us with
+// one group, 10.8 with two, 12.5 with four of two stages; f32 out, where the widening takes its time, 20.6, 16.1 and 14.0; 512 rows, two
+// tiles a unit, 28 and 25).
 template <int FB, int FA, bool WIDE>
 void launch_formats(const MmP& p, const char* name, double flops, double bytes, hipStream_t st) {
   const int64_t cus = tg_num_cus();
-  if (cdiv64(p.M, 256) * cdiv64(p.N, 256) * 5 >= cus * 4) launch_tile<FB, FA, WIDE, 8, 8, 2>(p, name, flops, bytes, st);
-  else if (cdiv64(p.M, 128) * cdiv64(p.N, 128) * 5 >= cus * 4) launch_tile<FB, FA, WIDE, 4, 4, 2>(p, name, flops, bytes, st);
-  else launch_tile<FB, FA, WIDE, 2, 2, 4>(p, name, flops, bytes, st);
+  const int64_t t256 = cdiv64(p.M, 256) * cdiv64(p.N, 256), t128 = cdiv64(p.M, 128) * cdiv64(p.N, 128), t64 = cdiv64(p.M, 64) * cdiv64(p.N, 64);
+  if (t256 * 5 >= cus * 4) launch_tile<FB, FA, WIDE, 8, 8, 2, 1>(p, name, flops, bytes, st);
+  else if (t128 > cus || (WIDE && t128 * 5 >= cus * 4)) launch_tile<FB, FA, WIDE, 4, 4, 2, 1>(p, name, flops, bytes, st);
+  else if (t128 * 5 >= cus * 4) launch_tile<FB, FA, WIDE, 4, 4, WIDE ? 2 : 4, 1>(p, name, flops, bytes, st);
+  else if (t64 > (WIDE ? 2 * cus : cus)) launch_tile<FB, FA, WIDE, 2, 2, 4, 1>(p, name, flops, bytes, st);
+  else if (t64 > cus) launch_tile<FB, FA, WIDE, 2, 2, WIDE ? 2 : 4, WIDE ? 2 : 1>(p, name, flops, bytes, st);
+  else launch_tile<FB, FA, WIDE, 2, 2, WIDE ? 2 : 4, WIDE ? 4 : 2>(p, name, flops, bytes, st);
 }
 
 // Few rows of a: 16 columns n of the output for a workgroup, all M (at most 16 MF) rows.  Here the weight's bytes count: every wave

@@ -384,6 +384,13 @@ MATMUL = [
     (513, 770, 2049, "e4m3", False, "e4m3", True, BF, True),
     (1024, 512, 4096, "e4m3", False, "e4m3", False, F32, False),
     (33, 2048, 8192, "e4m3", False, "e4m3", True, BF, True),
+    (40, 70, 128, "e4m3", False, "e4m3", True, BF, False),        # one to five blocks of K for the groups of a tile to share
+    (40, 70, 256, "e4m3", False, "e5m2", True, F32, False),
+    (65, 130, 384, "e4m3", True, "e4m3", False, BF, True),
+    (70, 100, 640, "e5m2", False, "e4m3", True, F32, True),
+    (64, 64, 8320, "e4m3", False, "e4m3", True, F32, False),
+    (1030, 1700, 300, "e4m3", False, "e4m3", True, F32, True),    # two of the smallest tiles a compute unit
+    (2048, 2040, 1100, "e4m3", False, "e4m3", True, BF, False),   # one of the middle ones
 ]
 
 
