@@ -349,7 +349,9 @@ void launch_tile(MmP p, const char* name, double flops, double bytes, hipStream_
   TG_LAUNCH(name, flops, bytes, (fp8_tile_kernel<FB, FA, WIDE, MF, NF, S, G>), dim3((unsigned)p.tiles), dim3(256 * G), lds, st, p);
 }
 
-// The largest tile that still gives most compute units one, and what else of a unit it leaves free: with at most one tile a unit its LDS
+// The largest tile that still gives most compute units one -- of the two larger ones (one and two a unit) the one whose last round of
+// tiles is not the emptier by more than it is the faster (4096^3, one full round: 60 and 73 us; 4352 x 4096 x 4096, a second round of
+// 16 tiles: 103 and 95, f32 out 194 and 145) -- and what else of a unit it leaves free: with at most one tile a unit its LDS
 // holds more stages (1024 x 4096 x 4096, bf16 out: 28 us with two, 23 with four) or groups of waves (64 x 4096 x 4096: bf16 out 12.1 us with
 // one group, 10.8 with two, 12.5 with four of two stages; f32 out, where the widening takes its time, 20.6, 16.1 and 14.0; 512 rows, two
 // tiles a unit, 28 and 25).
@@ -357,7 +359,8 @@ template <int FB, int FA, bool WIDE>
 void launch_formats(const MmP& p, const char* name, double flops, double bytes, hipStream_t st) {
   const int64_t cus = tg_num_cus();
   const int64_t t256 = cdiv64(p.M, 256) * cdiv64(p.N, 256), t128 = cdiv64(p.M, 128) * cdiv64(p.N, 128), t64 = cdiv64(p.M, 64) * cdiv64(p.N, 64);
-  if (t256 * 5 >= cus * 4) launch_tile<FB, FA, WIDE, 8, 8, 2, 1>(p, name, flops, bytes, st);
+  const int64_t places256 = cdiv64(t256, cus) * cus, places128 = cdiv64(t128, 2 * cus) * 2 * cus;
+  if (t256 * 5 >= cus * 4 && 5 * t256 * places128 >= 4 * t128 * places256) launch_tile<FB, FA, WIDE, 8, 8, 2, 1>(p, name, flops, bytes, st);
   else if (t128 > cus || (WIDE && t128 * 5 >= cus * 4)) launch_tile<FB, FA, WIDE, 4, 4, 2, 1>(p, name, flops, bytes, st);
   else if (t128 * 5 >= cus * 4) launch_tile<FB, FA, WIDE, 4, 4, WIDE ? 2 : 4, 1>(p, name, flops, bytes, st);
   else if (t64 > (WIDE ? 2 * cus : cus)) launch_tile<FB, FA, WIDE, 2, 2, 4, 1>(p, name, flops, bytes, st);

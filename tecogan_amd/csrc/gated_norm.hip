@@ -22,7 +22,7 @@ typedef float f4v __attribute__((ext_vector_type(4)));
 
 // A lane's 8 values of a vector: neighbours (VEC: 16-byte loads), or, where a row's length, stride or address is no multiple of 8
 // values, every lpr-th: single loads in which a wave still reads one stretch of memory, and no case for a row's end (52600 rows of 775
-// bf16 values: 178 us; 16 bytes at a time from odd addresses 401, and 776 values 83).
+// bf16 values: 162 us; 16 bytes at a time from odd addresses 401, and 776 values 83).
 template <bool VEC> struct Cols {
   static __device__ __forceinline__ int first(int v, int lane, int lpr) { return VEC ? (v * lpr + lane) * 8 : v * lpr * 8 + lane; }
   static __device__ __forceinline__ int step(int lpr) { return VEC ? 1 : lpr; }
@@ -274,26 +274,25 @@ struct GnP {
 template <typename TO, typename TX, int NV, bool VEC, int MODE>
 __global__ __launch_bounds__(512) void gated_norm_fwd_kernel(GnP p) {
   __shared__ __attribute__((aligned(16))) float red[2 * 8 * 4];
-  constexpr bool KEEP = NV <= 2;                                  // wider rows: no registers for the parameters or a second row
+  constexpr bool KEEP = NV <= (VEC ? 2 : 1);                      // wider rows: no registers for the parameters or a second row
   const bool HO = MODE == 3 ? p.o != nullptr : MODE >= 1, HG = MODE == 3 ? p.gate != nullptr : MODE == 2;
   const tg_gated_norm_desc& d = p.d;
-  const int lpr = 1 << p.lpr_log2, lane = threadIdx.x & (lpr - 1), sub = threadIdx.x >> p.lpr_log2, rpb = blockDim.x >> p.lpr_log2;
+  const int lpr = NV > 1 ? GN_MAX_LPR : 1 << p.lpr_log2, lane = threadIdx.x & (lpr - 1), sub = threadIdx.x >> p.lpr_log2, rpb = blockDim.x >> p.lpr_log2;
   const int C = d.C, st = Cols<VEC>::step(lpr);
-  float wpo[NV][8], bpo[NV][8], sc[NV][8], wpr[NV][8], bpr[NV][8];
-  auto params = [&]() {
+  constexpr int NP = KEEP ? NV : 1;
+  float wpo[NP][8], bpo[NP][8], sc[NP][8], wpr[NP][8], bpr[NP][8];
+  auto params_post = [&](int v, int a) {
+    const int c = Cols<VEC>::first(v, lane, lpr);
+    param8<VEC>(p.w_post, c, st, C, 1.f, wpo[a]);
+    param8<VEC>(p.b_post, c, st, C, 0.f, bpo[a]);
+    param8<VEC>(p.scale, c, st, C, 1.f, sc[a]);
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int c = Cols<VEC>::first(v, lane, lpr);
-      if (HO) {
-        param8<VEC>(p.w_post, c, st, C, 1.f, wpo[v]);
-        param8<VEC>(p.b_post, c, st, C, 0.f, bpo[v]);
-        param8<VEC>(p.scale, c, st, C, 1.f, sc[v]);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) sc[v][k] *= d.alpha;
-      }
-      param8<VEC>(p.w_pre, c, st, C, 1.f, wpr[v]);
-      param8<VEC>(p.b_pre, c, st, C, 0.f, bpr[v]);
-    }
+    for (int k = 0; k < 8; ++k) sc[a][k] *= d.alpha;
+  };
+  auto params_pre = [&](int v, int a) {
+    const int c = Cols<VEC>::first(v, lane, lpr);
+    param8<VEC>(p.w_pre, c, st, C, 1.f, wpr[a]);
+    param8<VEC>(p.b_pre, c, st, C, 0.f, bpr[a]);
   };
   const int64_t row0 = (int64_t)blockIdx.x * rpb + sub, step = (int64_t)gridDim.x * rpb;
   const TX* px = static_cast<const TX*>(p.x) + row0 * d.ldx;      // the row that is fetched next
@@ -320,20 +319,25 @@ __global__ __launch_bounds__(512) void gated_norm_fwd_kernel(GnP p) {
   int64_t row = row0;
   if constexpr (KEEP) {
     fetch(row);
-    params();
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      if (HO) params_post(v, v);
+      params_pre(v, v);
+    }
   }
   for (int64_t base = (int64_t)blockIdx.x * rpb; base < d.rows; base += step, row += step, py += sy, ph += sh) {
     const int Cr = row < d.rows ? C : 0;
-    if constexpr (!KEEP) {
-      fetch(row);
-      params();
-    }
-    float x[NV][8], u[NV][8], g[NV][8];
+    if constexpr (!KEEP) fetch(row);
+    float x[NV][8], u[NV][8];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       rx[v].values(x[v]);
       if (HO) ro[v].values(u[v]);
-      if (HG) rg[v].values(g[v]);
+    }
+    float g[NP][8];
+    if (KEEP && HG) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) rg[v].values(g[KEEP ? v : 0]);
     }
     if (KEEP && base + step < d.rows) fetch(row + step);
     if (HO) {
@@ -365,11 +369,16 @@ __global__ __launch_bounds__(512) void gated_norm_fwd_kernel(GnP p) {
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         const int c = Cols<VEC>::first(v, lane, lpr);
-        if (HG) gate_values(g[v], d.gate_act);
+        const int a = KEEP ? v : 0;
+        if (!KEEP) {
+          params_post(v, 0);
+          if (HG) rg[v].values(g[0]);
+        }
+        if (HG) gate_values(g[a], d.gate_act);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const float t = (u[v][k] - mu) * (r * wpo[v][k]) + bpo[v][k];
-          x[v][k] += (HG ? sc[v][k] * g[v][k] : sc[v][k]) * t;
+          const float t = (u[v][k] - mu) * (r * wpo[a][k]) + bpo[a][k];
+          x[v][k] += (HG ? sc[a][k] * g[a][k] : sc[a][k]) * t;
         }
         store8<TX, VEC>(py, c, st, Cr, x[v]);
       }
@@ -405,8 +414,10 @@ __global__ __launch_bounds__(512) void gated_norm_fwd_kernel(GnP p) {
       const float r = rsqrtf(s[0] * p.inv_c + d.eps);
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
+        const int a = KEEP ? v : 0;
+        if (!KEEP) params_pre(v, 0);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[v][k] = (x[v][k] - mu) * (r * wpr[v][k]) + bpr[v][k];
+        for (int k = 0; k < 8; ++k) x[v][k] = (x[v][k] - mu) * (r * wpr[a][k]) + bpr[a][k];
         store8<TO, VEC>(ph, Cols<VEC>::first(v, lane, lpr), st, Cr, x[v]);
       }
     }
@@ -421,7 +432,7 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
   extern __shared__ __attribute__((aligned(16))) float join[];      // [rows of the workgroup][8 lpr]: only where it has several
   constexpr bool IN_LDS = NV > 1;                                   // the parameter sums of wide rows: no registers for them
   const tg_gated_norm_desc& d = p.d;
-  const int lpr = 1 << p.lpr_log2, lane = threadIdx.x & (lpr - 1), sub = threadIdx.x >> p.lpr_log2, rpb = blockDim.x >> p.lpr_log2;
+  const int lpr = NV > 1 ? GN_MAX_LPR : 1 << p.lpr_log2, lane = threadIdx.x & (lpr - 1), sub = threadIdx.x >> p.lpr_log2, rpb = blockDim.x >> p.lpr_log2;
   const int C = d.C, st = Cols<VEC>::step(lpr);
   const int64_t item = (int64_t)blockIdx.x * rpb + sub;
   int64_t start, end;
@@ -474,27 +485,29 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
       if (HG) rg[v].load(static_cast<const TO*>(p.gate) + (int64_t)p.gate_of.of((uint32_t)r) * d.ldg, c, st, Cr);
     }
   };
-  float ga[NV][8], gs[NV][8];                                       // the gate's activation and its derivative
+  float ga[8], gs[8];                                               // the gate's activation and its derivative
   int64_t gate_row = 0;
 #pragma unroll
-  for (int v = 0; v < NV; ++v)
-#pragma unroll
-    for (int k = 0; k < 8; ++k) { ga[v][k] = 1.f; gs[v][k] = 0.f; }
-  float wpre[NV][8], wpost[NV][8], bpost[NV][8], sc[NV][8];
-  auto params = [&]() {
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int c = Cols<VEC>::first(v, lane, lpr);
-      param8<VEC>(p.w_pre, c, st, C, 1.f, wpre[v]);
-      param8<VEC>(p.w_post, c, st, C, 1.f, wpost[v]);
-      param8<VEC>(p.b_post, c, st, C, 0.f, bpost[v]);
-      param8<VEC>(p.scale, c, st, C, 1.f, sc[v]);
-    }
+  for (int k = 0; k < 8; ++k) { ga[k] = 1.f; gs[k] = 0.f; }
+  // of one vector of a lane: wider rows have no registers for all of them, nor for a second row
+  float wpre[8], wpost[8], bpost[8], sc[8];
+  auto params_pre = [&](int v) { param8<VEC>(p.w_pre, Cols<VEC>::first(v, lane, lpr), st, C, 1.f, wpre); };
+  auto params_post = [&](int v) {
+    const int c = Cols<VEC>::first(v, lane, lpr);
+    param8<VEC>(p.w_post, c, st, C, 1.f, wpost);
+    param8<VEC>(p.b_post, c, st, C, 0.f, bpost);
+    param8<VEC>(p.scale, c, st, C, 1.f, sc);
+  };
+  auto gate_of = [&](int v) {
+    float g[8];
+    rg[v].values(g);
+    gate_slopes(g, d.gate_act, ga, gs);
   };
   int turn = 0;
-  if constexpr (NV == 1) {                                          // wider rows: no registers for the parameters or a second row
+  if constexpr (NV == 1) {
     fetch(start);
-    params();
+    params_pre(0);
+    params_post(0);
   }
   // the workgroup's longest item: without pieces its first one
   int jn = p.item_rows;
@@ -507,10 +520,7 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
     const int64_t row = on ? start + j : 0;
     const int Cr = on ? C : 0;
     const int64_t grow = p.gate_of.of((uint32_t)row);
-    if constexpr (NV > 1) {
-      fetch(start + j);
-      params();
-    }
+    if constexpr (NV > 1) fetch(start + j);
     float y[NV][8], o[NV][8], dh[NV][8], G[NV][8];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -525,14 +535,9 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
         if (!HO) o[v][k] = 0.f;
       }
     }
-    if (HG && (j == 0 || grow != gate_row)) {                   // a shared gate row: its activation once
+    if (NV == 1 && HG && (j == 0 || grow != gate_row)) {        // a shared gate row: its activation once
       gate_row = grow;
-#pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        float g[8];
-        rg[v].values(g);
-        gate_slopes(g, d.gate_act, ga[v], gs[v]);
-      }
+      gate_of(0);
     }
     if (NV == 1 && j + 1 < jn) fetch(start + j + 1);
     float mu_y = 0.f, mu_o = 0.f;
@@ -551,11 +556,12 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
     for (int v = 0; v < NV; ++v) {
       const int c = Cols<VEC>::first(v, lane, lpr);
       const float my = c < Cr ? mu_y : 0.f, mo = c < Cr ? mu_o : 0.f;   // values past the end are 0 and stay 0
+      if (NV > 1) params_pre(v);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         y[v][k] -= VEC || c + k * st < Cr ? my : 0.f;
         o[v][k] -= VEC || c + k * st < Cr ? mo : 0.f;
-        const float t = dh[v][k] * wpre[v][k];
+        const float t = dh[v][k] * wpre[k];
         s[0] += y[v][k] * y[v][k];
         s[1] += t * y[v][k];
         s[2] += t;
@@ -571,27 +577,32 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
       const int c = Cols<VEC>::first(v, lane, lpr);
       float dg[8], t0[8], t1[8], t2[8];
       const float mp = c < Cr ? m2 : 0.f;
+      if (NV > 1) params_pre(v);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {                                  // no pre norm: dh = 0
         const float n = y[v][k] * r_y;
         t0[k] = dh[v][k] * n;
-        G[v][k] += r_y * (dh[v][k] * wpre[v][k] - n * m1 - (VEC || c + k * st < Cr ? mp : 0.f));
+        G[v][k] += r_y * (dh[v][k] * wpre[k] - n * m1 - (VEC || c + k * st < Cr ? mp : 0.f));
       }
       add(3, v, t0);
       add(4, v, dh[v]);
       if (p.d_x) store8<TX, VEC>(static_cast<TX*>(p.d_x) + row * d.ldx, c, st, Cr, G[v]);
       if (HO) {
+        if (NV > 1) {
+          params_post(v);
+          if (HG) gate_of(v);
+        }
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const float n = o[v][k] * r_o;                             // no post norm: deviation 1, weight 1, bias 0
-          const float u = n * wpost[v][k] + bpost[v][k];
-          const float a = ga[v][k], D = d.alpha * G[v][k];
+          const float u = n * wpost[k] + bpost[k];
+          const float a = ga[k], D = d.alpha * G[v][k];
           t2[k] = D * a * u;
-          dg[k] = D * sc[v][k] * u * gs[v][k];
-          t1[k] = D * sc[v][k] * a;
+          dg[k] = D * sc[k] * u * gs[k];
+          t1[k] = D * sc[k] * a;
           t0[k] = t1[k] * n;
           o[v][k] = n;
-          G[v][k] = t1[k] * wpost[v][k];
+          G[v][k] = t1[k] * wpost[k];
           q[0] += G[v][k] * n;
           q[1] += G[v][k];
         }
@@ -723,17 +734,21 @@ void row_geometry(int C, int block, Geo* g) {
   g->rpb = g->block / g->lpr;
 }
 
-// The backward pass's split of the rows: workgroups of 512 lanes, about one per compute unit (their registers leave room for one or
-// two), at least 4 rows per sub-row: every workgroup writes up to 5 C partial values, a row of the operands is 5 - 8 times C values.
+// The backward pass's split of the rows: workgroups of 512 lanes, one per compute unit (their registers leave room for one or two), as
+// few rows as that gives to each: every row costs its workgroup 2 - 9 us of latency, while partial sums, up to 5 C values a workgroup,
+// are read once from near by (64 rows of 1024 bf16 values: at least one row an item 10.7 us, at least four 18.7; 2048 x 2048: 25 both).
+// A gate row that several rows share stays with one item, or is cut into even pieces where that would double the item (72352 x 88,
+// 13 rows a gate row: whole ones 37 us, 9 and 4 rows 75).
 void item_geometry(int64_t rows, int C, int64_t k, Geo* g) {
   row_geometry(C, 512, g);
-  int64_t m = cdiv64(rows, (int64_t)256 * g->rpb);
-  if (m < 4) m = 4;
+  int64_t m = rows > 0 ? cdiv64(rows, (int64_t)256 * g->rpb) : 1;
   g->pieces = 0;
-  if (k > 1 && k <= m) {
-    m = cdiv64(m, k) * k;
+  if (k > 1 && k <= 2 * m) {
+    m = k <= m ? cdiv64(m, k) * k : k;
   } else if (k > m) {
-    g->pieces = (int)cdiv64(k < rows ? k : rows, m);
+    k = k < rows ? k : rows;
+    g->pieces = (int)cdiv64(k, m);
+    m = cdiv64(k, g->pieces);
   }
   g->item_rows = (int)m;
   g->items = g->pieces > 0 ? cdiv64(rows, k) * g->pieces : cdiv64(rows, m);
@@ -778,10 +793,9 @@ bool eps_ok(const tg_gated_norm_desc* d) { return d->eps >= 1e-30f && d->eps <= 
   } while (0)
 #define GN_MODE(KERN, TO, TX, NVV, VECV, ...)                                                                   \
   do {                                                                                                          \
-    if (!VECV) { TG_LAUNCH(name, flops, bytes, (KERN<TO, TX, NVV, VECV, VECV ? 0 : 3>), __VA_ARGS__); }           \
-    else if (gate) { TG_LAUNCH(name, flops, bytes, (KERN<TO, TX, NVV, VECV, VECV ? 2 : 3>), __VA_ARGS__); }     \
-    else if (o) { TG_LAUNCH(name, flops, bytes, (KERN<TO, TX, NVV, VECV, VECV ? 1 : 3>), __VA_ARGS__); }        \
-    else { TG_LAUNCH(name, flops, bytes, (KERN<TO, TX, NVV, VECV, VECV ? 0 : 3>), __VA_ARGS__); }               \
+    if (gate) { TG_LAUNCH(name, flops, bytes, (KERN<TO, TX, NVV, VECV, 2>), __VA_ARGS__); }                     \
+    else if (o) { TG_LAUNCH(name, flops, bytes, (KERN<TO, TX, NVV, VECV, 1>), __VA_ARGS__); }                   \
+    else { TG_LAUNCH(name, flops, bytes, (KERN<TO, TX, NVV, VECV, 0>), __VA_ARGS__); }                          \
   } while (0)
 
 extern "C" int tg_gated_norm_forward(const tg_gated_norm_desc* d, const void* x, const void* o, const void* gate, const float* w_post,
