@@ -296,22 +296,26 @@ __global__ __launch_bounds__(256 * G, MF * NF >= 64 || G > 1 ? 1 : 2) void fp8_t
       for (int j = 0; j < NF; ++j) mine[(i * NF + j) * 64] = acc[i][j];
     __syncthreads();
   }
+  auto sum_of = [&](int i, int j) {
+    f32x4 v = acc[i][j];
+    if constexpr (G > 1) {
+      const f32x4* const sums = reinterpret_cast<const f32x4*>(tile_lds) + (wave * MF * NF + i * NF + j) * 64 + lane;
+      v = sums[0];
 #pragma unroll
-  for (int i = 0; i < MF; ++i) {
-    const int64_t m = m0 + wm * 16 * MF + 16 * i + r16;
-    if (m >= p.M) continue;
+      for (int q = 1; q < G; ++q) v += sums[q * 4 * MF * NF * 64];
+    }
+    return v;
+  };
+  if (p.vec) {
 #pragma unroll
-    for (int j = 0; j < NF; ++j) {
-      const int64_t n = n0 + wn * 16 * NF + 16 * j + 4 * g;
-      if (n >= p.N || (G > 1 && (i * NF + j) % G != grp)) continue;     // each group writes its share
-      f32x4 v = acc[i][j];
-      if constexpr (G > 1) {
-        const f32x4* const sums = reinterpret_cast<const f32x4*>(tile_lds) + (wave * MF * NF + i * NF + j) * 64 + lane;
-        v = sums[0];
+    for (int i = 0; i < MF; ++i) {
+      const int64_t m = m0 + wm * 16 * MF + 16 * i + r16;
+      if (m >= p.M) continue;
 #pragma unroll
-        for (int q = 1; q < G; ++q) v += sums[q * 4 * MF * NF * 64];
-      }
-      if (p.vec) {
+      for (int j = 0; j < NF; ++j) {
+        const int64_t n = n0 + wn * 16 * NF + 16 * j + 4 * g;
+        if (n >= p.N || (G > 1 && (i * NF + j) % G != grp)) continue;   // each group writes its share
+        f32x4 v = sum_of(i, j);
         if (p.bias) v += *reinterpret_cast<const f32x4*>(p.bias + n);
         if constexpr (!WIDE) {
           *reinterpret_cast<uint2*>(static_cast<u16*>(p.out) + m * p.ldo + n) =
@@ -321,19 +325,62 @@ __global__ __launch_bounds__(256 * G, MF * NF >= 64 || G > 1 ? 1 : 2) void fp8_t
           if (p.accumulate) v += *o;
           *o = v;
         }
-      } else {
+      }
+    }
+    return;
+  }
+  // Rows of odd lengths: 16 rows at a time through a piece of LDS of this wave, so that a store instruction writes whole stretches of a row
+  // ([6541, 2203] bf16, K = 128: 21 us, 2204 columns 15; values stored from where the products leave them, 2 bytes in 16 rows at once, 45)
+  constexpr int WC = G > 1 ? 16 : 16 * NF, PITCH = WC + 4;
+  f32x4 bias[NF];                                                      // here and not between the stores: its wait would be one for them
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (n + q >= p.N) break;
-          const float s = v[q] + (p.bias ? p.bias[n + q] : 0.f);
+  for (int j = 0; j < NF; ++j)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int64_t n = n0 + wn * 16 * NF + 16 * j + 4 * g + q;
+      bias[j][q] = p.bias ? p.bias[n < p.N ? n : p.N - 1] : 0.f;
+    }
+  __syncthreads();                                                     // the stages are free; the groups' sums stay
+  float* const slab = reinterpret_cast<float*>(tile_lds + (G > 1 ? G * 4 * MF * NF * 1024 : 0)) + (grp * 4 + wave) * 16 * PITCH;
+#pragma unroll
+  for (int i = 0; i < MF; ++i) {
+#pragma unroll
+    for (int j0 = 0; j0 < NF; j0 += WC / 16) {
+      if (G > 1 && (i * NF + j0) % G != grp) continue;
+#pragma unroll
+      for (int j = j0; j < j0 + WC / 16; ++j) *reinterpret_cast<f32x4*>(slab + r16 * PITCH + 16 * (j - j0) + 4 * g) = sum_of(i, j) + bias[j];
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");               // between the lanes of a wave: in order
+      const int64_t mr = m0 + wm * 16 * MF + 16 * i, nc = n0 + wn * 16 * NF + 16 * j0;
+      const int cols = (int)(p.N - nc < WC ? p.N - nc : WC), rows = (int)(p.M - mr < 16 ? p.M - mr : 16);
+      // this lane's columns (two where a row of the piece is wider than a wave) and, in every RS rows, its row
+      constexpr int NB = WC > 64 ? WC / 64 : 1, RS = WC < 64 ? 64 / WC : 1;
+      const int r0 = WC < 64 ? lane / WC : 0;
+#pragma unroll
+      for (int h = 0; h < NB; ++h) {
+        const int c = (WC < 64 ? lane % WC : lane) + 64 * h;
+        const float* const from = slab + r0 * PITCH + c;
+        const int64_t at = (mr + r0) * p.ldo + nc + c;
+        const int left = c < cols ? rows - r0 : 0;
+        float v[16 / RS];
+#pragma unroll
+        for (int r = 0; r < 16; r += RS) v[r / RS] = from[r * PITCH];
+        asm volatile("" ::: "memory");                                 // one wait for all of them
+#pragma unroll
+        for (int r = 0; r < 16; r += RS) {
           if constexpr (!WIDE) {
-            static_cast<u16*>(p.out)[m * p.ldo + n + q] = f2bf(s);
+            if (r < left) (static_cast<u16*>(p.out) + at)[r * p.ldo] = f2bf(v[r / RS]);
           } else {
-            float* const o = static_cast<float*>(p.out) + m * p.ldo + n + q;
-            *o = p.accumulate ? *o + s : s;
+            float* const o = static_cast<float*>(p.out) + at + r * p.ldo;
+            if (p.accumulate && r < left) v[r / RS] += *o;
           }
         }
+        if constexpr (WIDE) {
+#pragma unroll
+          for (int r = 0; r < 16; r += RS)
+            if (r < left) (static_cast<float*>(p.out) + at)[r * p.ldo] = v[r / RS];
+        }
       }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
   }
 }
@@ -346,6 +393,7 @@ void launch_tile(MmP p, const char* name, double flops, double bytes, hipStream_
   p.tiles = p.tiles_m * p.tiles_n;
   constexpr int lds = G * S * (32 * MF + 32 * NF) * 132;
   static_assert(G == 1 || (MF * NF >= G && lds >= G * 4 * MF * NF * 1024), "the groups' sums lie in the stages");
+  static_assert(lds >= (G > 1 ? G * 4 * MF * NF * 1024 : 0) + G * 4 * 16 * ((G > 1 ? 16 : 16 * NF) + 4) * 4, "and so do the rows on their way out");
   TG_LAUNCH(name, flops, bytes, (fp8_tile_kernel<FB, FA, WIDE, MF, NF, S, G>), dim3((unsigned)p.tiles), dim3(256 * G), lds, st, p);
 }
 
