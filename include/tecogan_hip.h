@@ -483,7 +483,8 @@ int tg_frame_to_u8(const float* frame /*[npix][3] in [0,1]*/, unsigned char* out
  * between two blocks, its projections in 8-bit floating point, a gated linear recurrence along the sequence.  No counterpart in the
  * reference, whose blocks are conv - ReLU - conv + skip (lib/frvsr.py:50-57) and whose recurrence is unrolled (lib/Teco.py:130-160).
  * Beside the header's conventions: rows may have a stride (in elements), sizes are free, a workspace belongs to the calls of one
- * stream at a time (two graphs that may run at once need one each), and results are the same bits for the same inputs (no atomics).
+ * stream at a time (two graphs that may run at once need one each), results are the same bits for the same inputs (no atomics), and
+ * outputs overlap no input and no other output except where it is said.
  * ------------------------------------------------------------------------ */
 #define TG_NORM_NONE  0
 #define TG_NORM_RMS   1   /* z / sqrt(mean(z^2) + eps) * w + b            */

@@ -34,7 +34,7 @@ struct GsP {
   void *y, *d_x, *d_g;
   float *hT, *d_h0;
   float *tiles;                              // [B][ntiles][D] state before each tile
-  float *agg_p, *agg_l;                      // [B][nc][D] the chunks' maps
+  float *agg_p, *agg_l;                      // [B][nc][D] the chunks' maps (in the last one's L the state in front of the sequence)
   float *rev_l;                              // [B][nc][D] backward: what a chunk adds to the gradient that leaves it in front
   float *floor_part;                         // [B * nc][D]
   int ncb, nc, tpc, ntiles, W;               // channel blocks, chunks, tiles of a chunk, tiles, waves
@@ -218,12 +218,16 @@ __global__ __launch_bounds__(256) void gated_scan_fwd_kernel(GsP p) {
   fetch<T, V>(rg, gr, t0, p.d.g_t, q.cl, live);
   fetch<T, V>(rx, xr, t0, p.d.x_t, q.cl, live);
   unsigned rr = q.resets(p, t0, live);
+  // The state in front: with chunks from the first launch's copy, since hT may lie over h0 and be written while other chunks begin.  The
+  // copy has the place of the last chunk's L, which nothing is composed with (its P the backward pass needs).
+  const int64_t last = ((int64_t)q.b * p.nc + p.nc - 1) * D;
+  const float* const start = p.nc > 1 ? p.agg_l + last : (p.h0 ? p.h0 + (int64_t)q.b * D : nullptr);
   float low[V], k[V], H[V], P[V], L[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     low[v] = p.floor ? p.floor[q.cl + v] : 0.f;
     k[v] = 1.f - low[v];
-    H[v] = OUT && p.h0 ? p.h0[(int64_t)q.b * D + q.cl + v] : 0.f;
+    H[v] = OUT && start ? start[q.cl + v] : 0.f;
     P[v] = 1.f;
     L[v] = 0.f;
   }
@@ -345,7 +349,7 @@ __global__ __launch_bounds__(256) void gated_scan_fwd_kernel(GsP p) {
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         p.agg_p[at + v] = P[v];
-        p.agg_l[at + v] = L[v];
+        p.agg_l[at + v] = q.chunk < p.nc - 1 ? L[v] : (p.h0 ? p.h0[(int64_t)q.b * D + q.c + v] : 0.f);
       }
     }
   }

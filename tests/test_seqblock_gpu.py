@@ -608,6 +608,23 @@ def test_gated_scan_step_by_step_is_the_sequence():
         within(got, ref, e + R.U32 * ref.abs(), "steps")
 
 
+def test_gated_scan_long_sequence_in_place():
+    """A sequence in chunks, more workgroups than run at once, its state handed on in place and y over x or g: as with tensors apart."""
+    B, T, D = 1, 4096, 16384
+    x, g = torch.randn(B, T, D, device=DEV).to(BF), torch.randn(B, T, D, device=DEV).to(BF) + 3
+    h0 = torch.randn(B, D, device=DEV) * 1e6                       # still there after 4096 steps of gates near 1
+    reset = torch.zeros(B, T, device=DEV, dtype=torch.uint8)
+    carry = torch.empty(K.gated_scan_carry(B, T, D), device=DEV)
+    y, hT = torch.empty_like(x), torch.empty(B, D, device=DEV)
+    for low in (None, torch.full((D,), 0.999, device=DEV)):
+        K.gated_scan_forward(x, g, y, hT, carry, h0=h0, floor=low, reset=reset, keep=False)
+        for over in "xg":
+            xc, gc, state = x.clone(), g.clone(), h0.clone()
+            out = xc if over == "x" else gc
+            K.gated_scan_forward(xc, gc, out, state, carry, h0=state, floor=low, reset=reset, keep=False)
+            assert torch.equal(out, y) and torch.equal(state, hT)
+
+
 def test_gated_scan_a_reset_stops_nan_and_a_zero_gate_is_kept_apart():
     B, T, D = 1, 200, 64
     x, g = rnd(B, T, D, seed=1), rnd(B, T, D, seed=2)
