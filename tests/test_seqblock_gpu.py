@@ -49,6 +49,10 @@ NORM_CASES = [
     (11, 5000, BF, F32, "layer", "layer", 3, "sigmoid", True, 1),    # more parameter sums than one pass over wide rows holds
     (40, 1003, BF, BF, "layer", "rms", 1, "tanh", True, 1),          # rows that begin at every alignment
     (40, 1003, F32, F32, "rms", "layer", 8, "silu", True, 1),
+    (29, 7740, BF, F32, "layer", "rms", 6, "tanh", True, 1),         # wide rows value by value, gate rows in pieces of one row
+    (6, 12001, BF, BF, "rms", "layer", 1, "silu", True, 1),
+    (30000, 88, BF, BF, "rms", "rms", 13, "sigmoid", False, 1),      # whole gate rows longer than an even share of the rows
+    (9000, 89, BF, F32, "none", "layer", None, "none", True, 1),
 ]
 
 
