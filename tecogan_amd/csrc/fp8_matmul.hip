@@ -14,6 +14,9 @@
 //     mantissa) and multiplied by v_mfma_f32_16x16x32_bf16, whose sums are fp32 throughout: half the rate, the accuracy that the type
 //     promises (a weight gradient that is accumulated).
 //
+// Measured on one device: bf16 out 8192 x 8192 x 4096 228 - 250 us = 2200 - 2400 TFLOP/s, 4096 x 4096 x 8192 103 us = 2670, 1 x 4096 x 4096 from
+// bf16 rows 9 us; f32 out 8192 x 8192 x 4096 445 us = 1240 TFLOP/s.
+//
 // The instruction's rows are n and its columns m: a lane holds four neighbouring n of one m.
 #include "fp8.h"
 #include <type_traits>

