@@ -18,13 +18,13 @@
 // does not get past.  In a composed map P = -1 says that a reset is inside (P is a product of values in [0, 1] otherwise).
 // Steps at and behind a row's length keep the state, write y = 0 and zero gradients, and their x, g, dy are not looked at.
 //
-// Measured on one device: [1, 65536, 1024] bf16 in chunks 141 us (its bytes once 78 us, as read 130); [64, 1, 4096] one step 5.4 us;
-// [8, 4096, 1536] bf16 forward 47 + 54, backward 37 + 108 + 5 us; [4, 19, 65536] fp32 in one pass 15.6 and 28 us.
+// Measured on one device: [1, 65536, 1024] bf16 in chunks 141 us (its bytes once 78 us, as read 130); [64, 1, 4096] one step 3.6 us;
+// [8, 4096, 1536] bf16 forward 47 + 54, backward 37 + 108 + 5 us; [4, 19, 65536] fp32 in one pass 14.9 and 25 us.
 #include "common.h"
 
 namespace {
 
-constexpr int GS_L = 8;                                            // steps of a wave in a tile
+constexpr int GS_L = 8;                                            // steps of a wave in a tile; N = 1 in the kernels where T = 1
 constexpr int GS_MAXW = 4;                                         // waves of a workgroup: two small ones on a unit cover each other's
                                                                    // barriers (backward pass 128 us with 8 waves, 109 us with 4)
 
@@ -163,16 +163,16 @@ struct Place {
   }
 };
 
-// 8 steps of one tensor; `base`: its row of the batch (the same for a wave), cl: the lane's channel
-template <typename T, int V>
-__device__ __forceinline__ void fetch(Raw<T, V> (&r)[GS_L], const T* base, int64_t t0, int64_t stride, int cl, int live) {
+// N steps of one tensor; `base`: its row of the batch (the same for a wave), cl: the lane's channel
+template <typename T, int V, int N>
+__device__ __forceinline__ void fetch(Raw<T, V> (&r)[N], const T* base, int64_t t0, int64_t stride, int cl, int live) {
   const T* at = base + t0 * stride;
-  if (live == GS_L) {
+  if (live == N) {
 #pragma unroll
-    for (int j = 0; j < GS_L; ++j) r[j].load(at + j * stride + cl);
+    for (int j = 0; j < N; ++j) r[j].load(at + j * stride + cl);
   } else {
 #pragma unroll
-    for (int j = 0; j < GS_L; ++j) {
+    for (int j = 0; j < N; ++j) {
       r[j].zero();
       if (j < live) r[j].load(at + j * stride + cl);
     }
@@ -205,7 +205,7 @@ __device__ __forceinline__ void enter(const GsP& p, const Place<V>& q, const flo
 }
 
 // Forward.  OUT false: the chunk's map only (each wave a contiguous part of it); true: states and outputs.
-template <typename T, int V, bool OUT>
+template <typename T, int V, bool OUT, int N>
 __global__ __launch_bounds__(256) void gated_scan_fwd_kernel(GsP p) {
   __shared__ float sP[GS_MAXW][64 * V], sL[GS_MAXW][64 * V];
   const Place<V> q(p, OUT ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x);
@@ -214,12 +214,12 @@ __global__ __launch_bounds__(256) void gated_scan_fwd_kernel(GsP p) {
   const T* const gr = static_cast<const T*>(p.g) + (int64_t)q.b * p.d.g_b;
   T* const yr = static_cast<T*>(p.y) + (int64_t)q.b * p.d.y_b;
   // OUT: tile i, wave after wave; otherwise this wave's i-th group of 8 steps of its contiguous part of the chunk
-  auto step0 = [&](int i) -> int64_t { return OUT ? ((q.first + i) * W + wave) * GS_L : (q.first * W + (int64_t)wave * q.ntiles + i) * GS_L; };
-  Raw<T, V> rx[GS_L], rg[GS_L];
+  auto step0 = [&](int i) -> int64_t { return OUT ? ((q.first + i) * W + wave) * N : (q.first * W + (int64_t)wave * q.ntiles + i) * N; };
+  Raw<T, V> rx[N], rg[N];
   int64_t t0 = step0(0);
   int live = q.live(t0);
-  fetch<T, V>(rg, gr, t0, p.d.g_t, q.cl, live);
-  fetch<T, V>(rx, xr, t0, p.d.x_t, q.cl, live);
+  fetch<T, V, N>(rg, gr, t0, p.d.g_t, q.cl, live);
+  fetch<T, V, N>(rx, xr, t0, p.d.x_t, q.cl, live);
   unsigned rr = q.resets(p, t0, live);
   // The state in front: with chunks from the first launch's copy, since hT may lie over h0 and be written while other chunks begin.  The
   // copy has the place of the last chunk's L, which nothing is composed with (its P the backward pass needs).
@@ -239,9 +239,9 @@ __global__ __launch_bounds__(256) void gated_scan_fwd_kernel(GsP p) {
     const unsigned fresh = p.reset ? (unsigned)__ballot(rr != 0) : 0;
     const int now = live;
     const int64_t tn = t0;
-    float f[GS_L][V], a[GS_L][V];
+    float f[N][V], a[N][V];
 #pragma unroll
-    for (int j = 0; j < GS_L; ++j) {
+    for (int j = 0; j < N; ++j) {
       float g[V], x[V];
       rg[j].values(g);
       rx[j].values(x);
@@ -256,13 +256,13 @@ __global__ __launch_bounds__(256) void gated_scan_fwd_kernel(GsP p) {
     if (i + 1 < q.ntiles) {
       t0 = step0(i + 1);
       live = q.live(t0);
-      fetch<T, V>(rg, gr, t0, p.d.g_t, q.cl, live);
-      fetch<T, V>(rx, xr, t0, p.d.x_t, q.cl, live);
+      fetch<T, V, N>(rg, gr, t0, p.d.g_t, q.cl, live);
+      fetch<T, V, N>(rx, xr, t0, p.d.x_t, q.cl, live);
       rr = q.resets(p, t0, live);
     }
-    if (now < GS_L) {
+    if (now < N) {
 #pragma unroll
-      for (int j = 0; j < GS_L; ++j)
+      for (int j = 0; j < N; ++j)
         if (j >= now) {
 #pragma unroll
           for (int v = 0; v < V; ++v) { f[j][v] = 1.f; a[j][v] = 0.f; }
@@ -277,7 +277,7 @@ __global__ __launch_bounds__(256) void gated_scan_fwd_kernel(GsP p) {
 #pragma unroll
       for (int v = 0; v < V; ++v) Q[v] = 1.f;
 #pragma unroll
-      for (int j = 0; j < GS_L; ++j)
+      for (int j = 0; j < N; ++j)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           L[v] = f[j][v] * L[v] + a[j][v];
@@ -287,7 +287,7 @@ __global__ __launch_bounds__(256) void gated_scan_fwd_kernel(GsP p) {
       for (int v = 0; v < V; ++v) P[v] = P[v] < 0.f ? -1.f : P[v] * Q[v];
     } else {
 #pragma unroll
-      for (int j = 0; j < GS_L; ++j)
+      for (int j = 0; j < N; ++j)
 #pragma unroll
         for (int v = 0; v < V; ++v) compose(P[v], L[v], fresh >> j & 1 ? -1.f : f[j][v], a[j][v]);
     }
@@ -319,7 +319,7 @@ __global__ __launch_bounds__(256) void gated_scan_fwd_kernel(GsP p) {
       }
       T* const out = yr + tn * p.d.y_t;
 #pragma unroll
-      for (int j = 0; j < GS_L; ++j) {
+      for (int j = 0; j < N; ++j) {
         float o[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -359,7 +359,7 @@ __global__ __launch_bounds__(256) void gated_scan_fwd_kernel(GsP p) {
 }
 
 // Backward.  OUT false: what a chunk adds to the gradient that leaves it in front; true: the gradients.
-template <typename T, int V, bool OUT>
+template <typename T, int V, bool OUT, int N>
 __global__ __launch_bounds__(256) void gated_scan_bwd_kernel(GsP p) {
   __shared__ float sP[GS_MAXW][64 * V], sL[GS_MAXW][64 * V], sR[GS_MAXW][64 * V];
   const Place<V> q(p, OUT ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x);
@@ -369,14 +369,14 @@ __global__ __launch_bounds__(256) void gated_scan_bwd_kernel(GsP p) {
   const T* const er = static_cast<const T*>(p.d_y) + (int64_t)q.b * p.d.dy_b;
   T* const dxr = static_cast<T*>(p.d_x) + (int64_t)q.b * p.d.dx_b;
   T* const dgr = static_cast<T*>(p.d_g) + (int64_t)q.b * p.d.dg_b;
-  auto step0 = [&](int i) -> int64_t { return OUT ? ((q.first + i) * W + wave) * GS_L : (q.first * W + (int64_t)wave * q.ntiles + i) * GS_L; };
-  Raw<T, V> rx[GS_L], rg[GS_L], re[GS_L];
+  auto step0 = [&](int i) -> int64_t { return OUT ? ((q.first + i) * W + wave) * N : (q.first * W + (int64_t)wave * q.ntiles + i) * N; };
+  Raw<T, V> rx[N], rg[N], re[N];
   float rH[V];
   auto fetch_all = [&](int i, int64_t t0, int live) {
-    fetch<T, V>(rg, gr, t0, p.d.g_t, q.cl, live);
-    fetch<T, V>(re, er, t0, p.d.dy_t, q.cl, p.d_y ? live : 0);
+    fetch<T, V, N>(rg, gr, t0, p.d.g_t, q.cl, live);
+    fetch<T, V, N>(re, er, t0, p.d.dy_t, q.cl, p.d_y ? live : 0);
     if (OUT) {
-      fetch<T, V>(rx, xr, t0, p.d.x_t, q.cl, live);
+      fetch<T, V, N>(rx, xr, t0, p.d.x_t, q.cl, live);
       const float* const st = p.tiles + ((int64_t)q.b * p.ntiles + q.first + i) * D + q.cl;
 #pragma unroll
       for (int v = 0; v < V; ++v) rH[v] = st[v];
@@ -400,9 +400,9 @@ __global__ __launch_bounds__(256) void gated_scan_bwd_kernel(GsP p) {
     const unsigned fresh = p.reset ? (unsigned)__ballot(rr != 0) : 0;
     const int now = live;
     const int64_t tn = t0;
-    float up[GS_L][V], down[GS_L][V], x[GS_L][V], e[GS_L][V], H[V];
+    float up[N][V], down[N][V], x[N][V], e[N][V], H[V];
 #pragma unroll
-    for (int j = 0; j < GS_L; ++j) {
+    for (int j = 0; j < N; ++j) {
       float g[V];
       rg[j].values(g);
       re[j].values(e[j]);
@@ -421,7 +421,7 @@ __global__ __launch_bounds__(256) void gated_scan_bwd_kernel(GsP p) {
     }
     if constexpr (!OUT) {
 #pragma unroll
-      for (int j = GS_L - 1; j >= 0; --j) {
+      for (int j = N - 1; j >= 0; --j) {
         if (j < now) {
           const bool r = fresh >> j & 1;
 #pragma unroll
@@ -436,9 +436,9 @@ __global__ __launch_bounds__(256) void gated_scan_bwd_kernel(GsP p) {
       float Lf[V], Lr[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) { P[v] = 1.f; Lf[v] = 0.f; Lr[v] = 0.f; }
-      if (now == GS_L && fresh == 0) {
+      if (now == N && fresh == 0) {
 #pragma unroll
-        for (int j = 0; j < GS_L; ++j)
+        for (int j = 0; j < N; ++j)
 #pragma unroll
           for (int v = 0; v < V; ++v) {
             const float f = low[v] + k[v] * up[j][v];
@@ -446,18 +446,18 @@ __global__ __launch_bounds__(256) void gated_scan_bwd_kernel(GsP p) {
             P[v] *= f;
           }
 #pragma unroll
-        for (int j = GS_L - 1; j >= 0; --j)
+        for (int j = N - 1; j >= 0; --j)
 #pragma unroll
           for (int v = 0; v < V; ++v) Lr[v] = (low[v] + k[v] * up[j][v]) * (e[j][v] + Lr[v]);
       } else {
 #pragma unroll
-        for (int j = 0; j < GS_L; ++j)
+        for (int j = 0; j < N; ++j)
           if (j < now) {
 #pragma unroll
             for (int v = 0; v < V; ++v) compose(P[v], Lf[v], fresh >> j & 1 ? -1.f : low[v] + k[v] * up[j][v], k[v] * down[j][v] * x[j][v]);
           }
 #pragma unroll
-        for (int j = GS_L - 1; j >= 0; --j)
+        for (int j = N - 1; j >= 0; --j)
           if (j < now) {
 #pragma unroll
             for (int v = 0; v < V; ++v) Lr[v] = fresh >> j & 1 ? 0.f : (low[v] + k[v] * up[j][v]) * (e[j][v] + Lr[v]);
@@ -494,9 +494,9 @@ __global__ __launch_bounds__(256) void gated_scan_bwd_kernel(GsP p) {
 #pragma unroll
         for (int v = 0; v < V; ++v) Rw[v] = R[v];
       }
-      float h[GS_L][V];
+      float h[N][V];
 #pragma unroll
-      for (int j = 0; j < GS_L; ++j) {                              // the state before each step
+      for (int j = 0; j < N; ++j) {                              // the state before each step
         const bool r = fresh >> j & 1;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -507,7 +507,7 @@ __global__ __launch_bounds__(256) void gated_scan_bwd_kernel(GsP p) {
       T* const ox = dxr + tn * p.d.dx_t;
       T* const og = dgr + tn * p.d.dg_t;
 #pragma unroll
-      for (int j = GS_L - 1; j >= 0; --j) {
+      for (int j = N - 1; j >= 0; --j) {
         float vx[V], vg[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) { vx[v] = 0.f; vg[v] = 0.f; }
@@ -599,7 +599,7 @@ struct Plan {
 // 0.8 us, a launch with its gap 4 us).  The fewest chunks at the least of it.
 Plan plan_of(int64_t B, int64_t T, int64_t D) {
   Plan p;
-  p.W = T <= 8 ? 1 : (T <= 16 ? 2 : 4);
+  p.W = T <= 24 ? (int)cdiv64(T, GS_L) : GS_MAXW;
   p.tile = p.W * GS_L;
   p.ntiles = (int)cdiv64(T, p.tile);
   const int64_t units = B * cdiv64(D, 128);
@@ -662,14 +662,14 @@ void set_plan(GsP* p, const Plan& pl, int V, float* carry) {
 }
 }  // namespace
 
-#define GS_PICK(KERN, OUTV, GRID)                                                                                                   \
+#define GS_PICK(KERN, OUTV, NV, GRID)                                                                                               \
   do {                                                                                                                              \
     if (d->dtype == TG_F32) {                                                                                                       \
-      if (V == 2) TG_LAUNCH(name, flops, bytes, (KERN<float, 2, OUTV>), dim3(GRID), dim3(64 * pl.W), 0, ST(stream), p);             \
-      else TG_LAUNCH(name, flops, bytes, (KERN<float, 1, OUTV>), dim3(GRID), dim3(64 * pl.W), 0, ST(stream), p);                    \
+      if (V == 2) TG_LAUNCH(name, flops, bytes, (KERN<float, 2, OUTV, NV>), dim3(GRID), dim3(64 * pl.W), 0, ST(stream), p);         \
+      else TG_LAUNCH(name, flops, bytes, (KERN<float, 1, OUTV, NV>), dim3(GRID), dim3(64 * pl.W), 0, ST(stream), p);                \
     } else {                                                                                                                        \
-      if (V == 2) TG_LAUNCH(name, flops, bytes, (KERN<u16, 2, OUTV>), dim3(GRID), dim3(64 * pl.W), 0, ST(stream), p);               \
-      else TG_LAUNCH(name, flops, bytes, (KERN<u16, 1, OUTV>), dim3(GRID), dim3(64 * pl.W), 0, ST(stream), p);                      \
+      if (V == 2) TG_LAUNCH(name, flops, bytes, (KERN<u16, 2, OUTV, NV>), dim3(GRID), dim3(64 * pl.W), 0, ST(stream), p);           \
+      else TG_LAUNCH(name, flops, bytes, (KERN<u16, 1, OUTV, NV>), dim3(GRID), dim3(64 * pl.W), 0, ST(stream), p);                  \
     }                                                                                                                               \
   } while (0)
 
@@ -697,11 +697,13 @@ extern "C" int tg_gated_scan_forward(const tg_gated_scan_desc* d, const void* x,
   if (pl.nc > 1) {
     const char* const name = "gated_scan_fwd<map>";
     const double flops = 10 * n, bytes = 2 * es * n;
-    GS_PICK(gated_scan_fwd_kernel, false, (unsigned)blocks);
+    GS_PICK(gated_scan_fwd_kernel, false, GS_L, (unsigned)blocks);
   }
   const char* const name = "gated_scan_fwd";
   const double flops = 14 * n, bytes = 3 * es * n;
-  GS_PICK(gated_scan_fwd_kernel, true, (unsigned)blocks);
+  // single steps: seven more that are not there cost their exponentials ([256, 1, 8192] bf16: 10.6 us, with them 17.6; backward 11.3 and 29.4)
+  if (d->T == 1) GS_PICK(gated_scan_fwd_kernel, true, 1, (unsigned)blocks);
+  else GS_PICK(gated_scan_fwd_kernel, true, GS_L, (unsigned)blocks);
   TG_CHECK_LAUNCH();
 }
 
@@ -723,7 +725,9 @@ extern "C" int tg_gated_scan_backward(const tg_gated_scan_desc* d, const void* x
     const int64_t cf = chunk_floats(pl, d->B, d->D), want = cf * (pl.nc > 1 ? 2 : 1);
     TG_CHECK_ARG((pl.nc == 1 && !d_floor) || (ws != nullptr && ws_floats >= want && al(ws, 16)), "a workspace of tg_gated_scan_sizes() floats is missing");
     const int es = d->dtype == TG_F32 ? 4 : 2;
-    const int V = lane_channels(d->D);
+    // Three waves of two channels: their 200 - 225 registers leave a quarter of a unit's places empty, one channel needs 122 ([64, 20, 8192]
+    // bf16 40.5 us with two, 35 with one; four waves 41; with 32 steps 37.5 and 41)
+    const int V = pl.W == 3 ? 1 : lane_channels(d->D);
     GsP p = {};
     p.d = *d;
     p.x = x; p.g = g; p.floor = floor; p.lengths = lengths; p.reset = reset; p.d_y = d_y; p.d_hT = d_hT;
@@ -736,11 +740,12 @@ extern "C" int tg_gated_scan_backward(const tg_gated_scan_desc* d, const void* x
     if (pl.nc > 1) {
       const char* const name = "gated_scan_bwd<map>";
       const double flops = 12 * n, bytes = 2 * es * n;
-      GS_PICK(gated_scan_bwd_kernel, false, (unsigned)blocks);
+      GS_PICK(gated_scan_bwd_kernel, false, GS_L, (unsigned)blocks);
     }
     const char* const name = "gated_scan_bwd";
     const double flops = 40 * n, bytes = 5 * es * n;
-    GS_PICK(gated_scan_bwd_kernel, true, (unsigned)blocks);
+    if (d->T == 1) GS_PICK(gated_scan_bwd_kernel, true, 1, (unsigned)blocks);
+    else GS_PICK(gated_scan_bwd_kernel, true, GS_L, (unsigned)blocks);
   }
   if (d_floor)
     hipLaunchKernelGGL(gated_scan_floor_kernel, dim3((unsigned)cdiv64(d->D, 64)), dim3(1024), 0, ST(stream), ws, d->B > 0 ? (int64_t)d->B * pl.nc : 0, d->D, d_floor);

@@ -475,6 +475,11 @@ SCAN_CASES = [
     (2, 500, 66, BF, False, 0.01, [500, 317], True, 2),
     (1, 1500, 40, F32, True, 0.0, None, False, 1),                    # many chunks
     (70, 70, 2048, BF, False, 0.02, None, True, 1),                   # enough channels for one chunk: two tiles
+    (4, 1, 130, F32, False, 0.3, [1, 0, 1, 1], True, 2),              # single steps
+    (300, 1, 258, BF, True, 0.2, None, False, 1),
+    (2, 20, 130, BF, True, 0.1, [20, 11], True, 1),                   # three waves
+    (3, 24, 258, F32, False, 0.05, None, True, 2),
+    (2, 25, 130, BF, True, 0.1, [17, 25], False, 1),
 ]
 
 
