@@ -270,7 +270,7 @@ struct GnP {
   float inv_c;
 };
 
-// MODE: what there is beside x -- 0 nothing, 1 a block's output, 2 that and a gate, 3 asked at run time (the rarer shapes).  A norm
+// MODE: what there is beside x -- 0 nothing, 1 a block's output, 2 that and a gate, 3 asked at run time (the widest rows).  A norm
 // that is not wanted is one with mean 0 and deviation 1: no branches around the values.
 // Parameters stay in registers over a workgroup's rows where they fit (one or two vectors a lane), and the next row's tensors are on
 // their way while a row's sums are made.
@@ -884,7 +884,7 @@ extern "C" int tg_gated_norm_backward(const tg_gated_norm_desc* d, const void* d
     p.item_rows = g.item_rows; p.pieces = g.pieces; p.items = g.items;
     p.want = want;
     p.inv_c = 1.f / (float)C;
-  p.gate_of = divide_by((uint32_t)d->rows_per_gate);
+    p.gate_of = divide_by((uint32_t)d->rows_per_gate);
     const bool vec = C % 8 == 0 && al16(d_y) && al16(d_h) && al16(y) && al16(o) && al16(gate) && al16(w_post) && al16(b_post) &&
                      al16(scale) && al16(w_pre) && al16(d_x) && al16(d_o) && al16(d_gate) && (!d_y || d->ld_dy % 8 == 0) &&
                      (!d_h || d->ldh % 8 == 0) && d->ldy % 8 == 0 && (!o || d->ldo % 8 == 0) && (!gate || d->ldg % 8 == 0) &&
