@@ -433,16 +433,20 @@ void launch_tile(MmP p, const char* name, double flops, double bytes, hipStream_
 
 // The largest tile that still gives most compute units one -- of the two larger ones (one and two a unit) the one whose last round of
 // tiles is not the emptier by more than it is the faster (4096^3, one full round: 60 and 73 us; 4352 x 4096 x 4096, a second round of
-// 16 tiles: 103 and 95, f32 out 194 and 145) -- and what else of a unit it leaves free: with at most one tile a unit its LDS
-// holds more stages (1024 x 4096 x 4096, bf16 out: 28 us with two, 23 with four) or groups of waves (64 x 4096 x 4096: bf16 out 12.1 us with
-// one group, 10.8 with two, 12.5 with four of two stages; f32 out, where the widening takes its time, 20.6, 16.1 and 14.0; 512 rows, two
-// tiles a unit, 28 and 25).
+// 16 tiles: 103 and 95, f32 out 194 and 145).  Over few blocks of K it is faster by less, since two tiles a unit hide each other's way out
+// (K = 384, 6207 x 5696: 48 and 42), for f32 outputs of several rounds not at all (8192 x 8192 x 1024: 173 and 155).
+// And what else of a unit a tile leaves free: with at most one a unit its LDS holds more stages (1024 x 4096 x 4096, bf16 out: 28 us with
+// two, 23 with four) or groups of waves (64 x 4096 x 4096: bf16 out 12.1 us with one group, 10.8 with two, 12.5 with four of two stages; f32
+// out, where the widening takes its time, 20.6, 16.1 and 14.0; 512 rows, two tiles a unit, 28 and 25).
 template <int FB, int FA, bool WIDE>
 void launch_formats(const MmP& p, const char* name, double flops, double bytes, hipStream_t st) {
   const int64_t cus = tg_num_cus();
   const int64_t t256 = cdiv64(p.M, 256) * cdiv64(p.N, 256), t128 = cdiv64(p.M, 128) * cdiv64(p.N, 128), t64 = cdiv64(p.M, 64) * cdiv64(p.N, 64);
   const int64_t places256 = cdiv64(t256, cus) * cus, places128 = cdiv64(t128, 2 * cus) * 2 * cus;
-  if (t256 * 5 >= cus * 4 && 5 * t256 * places128 >= 4 * t128 * places256) launch_tile<FB, FA, WIDE, 8, 8, 2, 1>(p, name, flops, bytes, st);
+  const bool brief = p.K <= 1024;
+  const int64_t gain = brief ? 114 : 125;                              // per cent
+  const bool large = t256 * 5 >= cus * 4 && gain * t256 * places128 >= 100 * t128 * places256 && !(WIDE && brief && t256 > cus);
+  if (large) launch_tile<FB, FA, WIDE, 8, 8, 2, 1>(p, name, flops, bytes, st);
   else if (t128 > cus || (WIDE && t128 * 5 >= cus * 4)) launch_tile<FB, FA, WIDE, 4, 4, 2, 1>(p, name, flops, bytes, st);
   else if (t128 * 5 >= cus * 4) launch_tile<FB, FA, WIDE, 4, 4, WIDE ? 2 : 4, 1>(p, name, flops, bytes, st);
   else if (t64 > (WIDE ? 2 * cus : cus)) launch_tile<FB, FA, WIDE, 2, 2, 4, 1>(p, name, flops, bytes, st);
