@@ -534,9 +534,11 @@ typedef struct tg_fp8_matmul_desc {
   int32_t a_tile, b_tile;  /* scales per 128 x 128 tile instead of per row */
   int32_t out_dtype;       /* TG_F32, TG_BF16 */
   int32_t accumulate;      /* out += (f32 only) */
+  int32_t fast;            /* bf16 only: the 8-bit matrix instruction's sums, see below */
 } tg_fp8_matmul_desc;
-/* out[M][N] = a[M][K] b[N][K]^T (+ bias[N]) (+ out).  f32 outputs: fp32 sums of exact products.  bf16 outputs of more than 32 rows: the 8-bit
- * matrix instruction cuts the products of 8 neighbouring k below 2^-13 of the largest of them before it adds them in fp32. */
+/* out[M][N] = a[M][K] b[N][K]^T (+ bias[N]) (+ out): fp32 sums of exact products (scaled operands in fp32's normal range), in an order that
+ * depends on the sizes.  fast != 0: the 8-bit matrix instruction adds, up to twice as fast; it cuts the products of 8 neighbouring k below
+ * 2^-13 of the largest of them first, so that where large ones cancel the small ones are lost.  Up to 32 rows are summed in fp32 either way. */
 int tg_fp8_matmul(const tg_fp8_matmul_desc* d, const void* a, const void* scale_a, const void* b, const void* scale_b,
                   const float* bias /*nullable*/, void* out, void* stream);
 /* out = q(x) w^T + bias: tg_fp8_quantize (e4m3, a scale per row and block) and tg_fp8_matmul with a weight of tile scales; few rows

@@ -33,7 +33,7 @@ class GatedNormDesc(C.Structure):
 
 class Fp8MatmulDesc(C.Structure):
     _fields_ = [(n, C.c_int64) for n in ("M", "N", "K", "ldo")] + \
-               [(n, C.c_int32) for n in ("a_fmt", "b_fmt", "a_tile", "b_tile", "out_dtype", "accumulate")]
+               [(n, C.c_int32) for n in ("a_fmt", "b_fmt", "a_tile", "b_tile", "out_dtype", "accumulate", "fast")]
 
 
 class GatedScanDesc(C.Structure):

@@ -1,18 +1,17 @@
 // out[m][n] = sum over blocks kb of 128 of 2^(ea[m, kb] + eb[n, kb]) sum_k a[m][k] b[n][k]  (+ bias[n]) (+ out[m][n])
 //
 // a [M][K], b [N][K] in 8-bit floating point (e4m3 or e5m2 each), K a multiple of 128 (tg_fp8_quantize pads rows with zeros); the
-// scales' biased exponents one byte for a row and 128 columns, or for a tile of 128 x 128.  Two ways through the matrix unit, chosen
-// by the output's type:
+// scales' biased exponents one byte for a row and 128 columns, or for a tile of 128 x 128.  Two ways through the matrix unit:
 //
-//   bf16 outputs: v_mfma_scale_f32_16x16x128 covers 16 x 16 outputs over exactly one block of K with the scales of its 16 rows and 16
-//     columns as operands (4.2 PFLOP/s issued back to back on one device).  The products of 8 neighbouring k are aligned to the largest
-//     sum of exponents E among them and cut to multiples of 2^(E - 13) before they are added (found by adding small products to a
-//     large one; the unscaled 8-bit instructions do the same): measured 1.5e-5 of the result for normal operands, 7e-5 where a few
-//     channels carry it, the same for any K.  That is 25 - 100 times less than the rounding of the result to bf16; the sums over
-//     the groups and blocks are fp32.
-//   f32 outputs: the operands are widened to bf16 with their scales in registers (v_cvt_scalef32_pk_bf16_fp8: exact, 4 bits of
-//     mantissa) and multiplied by v_mfma_f32_16x16x32_bf16, whose sums are fp32 throughout: half the rate, the accuracy that the type
-//     promises (a weight gradient that is accumulated).
+//   whole sums: the operands are widened to bf16 with their scales in registers (v_cvt_scalef32_pk_bf16_fp8: exact, 4 bits of mantissa,
+//     as long as the scaled values lie in fp32's normal range) and multiplied by v_mfma_f32_16x16x32_bf16, whose sums are fp32
+//     throughout: half the rate of the 8-bit instruction.
+//   fast (bf16 outputs, asked for by the caller): v_mfma_scale_f32_16x16x128 covers 16 x 16 outputs over exactly one block of K with the
+//     scales of its 16 rows and 16 columns as operands (4.2 PFLOP/s issued back to back on one device).  The products of 8 neighbouring
+//     k are aligned to the largest sum of exponents E among them and cut to multiples of 2^(E - 13) before they are added (found by
+//     adding small products to a large one; the unscaled 8-bit instructions do the same); the sums over the groups and blocks are
+//     fp32.  Measured 1.5e-5 of the result for normal operands, 7e-5 where a few channels carry it, the same for any K -- but where large
+//     products of one group cancel, what is left of the others is lost (256 - 256 + 6 x 15 x 2^-9: 0, not 0.18).  Hence the caller's choice.
 //
 // Measured on one device: bf16 out 8192 x 8192 x 4096 228 - 250 us = 2200 - 2400 TFLOP/s, 4096 x 4096 x 8192 103 us = 2670, 1 x 4096 x 4096 from
 // bf16 rows 9 us; f32 out 8192 x 8192 x 4096 445 us = 1240 TFLOP/s.
@@ -116,6 +115,7 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rsrc, unsigned char
 // G groups of four waves share a tile: group j takes the blocks j, j + G, ... of K through stages of its own, and the groups' sums meet in
 // LDS in the groups' order.  A block of the smallest tile costs its waves
 // about 800 cycles, most of them waits (barrier, LDS, products, in turn); G groups wait at the same time.
+// WIDE: whole sums, either output type; otherwise the 8-bit instruction's, bf16 outputs.
 template <int FB, int FA, bool WIDE, int MF, int NF, int S, int G>
 __global__ __launch_bounds__(256 * G, MF * NF >= 64 || G > 1 ? 1 : 2) void fp8_tile_kernel(MmP p) {
   constexpr int TM = 32 * MF, TN = 32 * NF, STAGE = (TM + TN) * 132, HM = MF / 2, HN = NF / 2;
@@ -356,7 +356,7 @@ __global__ __launch_bounds__(256 * G, MF * NF >= 64 || G > 1 ? 1 : 2) void fp8_t
         const int64_t n = n0 + wn * 16 * NF + 16 * j + 4 * g;
         if (n >= p.N || (G > 1 && (i * NF + j) % G != grp)) continue;   // each group writes its share
         f32x4 v = sum_of(i, j) + bias[j];
-        if constexpr (!WIDE) {
+        if (!WIDE || p.out_bf16) {
           const bf16x2m lo = {(__bf16)v[0], (__bf16)v[1]}, hi = {(__bf16)v[2], (__bf16)v[3]};
           *reinterpret_cast<uint2*>(static_cast<u16*>(p.out) + m * p.ldo + n) = make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
         } else {
@@ -396,7 +396,7 @@ __global__ __launch_bounds__(256 * G, MF * NF >= 64 || G > 1 ? 1 : 2) void fp8_t
         for (int r = 0; r < 16; r += RS) v[r / RS] = from[r * PITCH];
         asm volatile("" ::: "memory");                                 // one wait for all of them
         if (left <= 0) continue;
-        if constexpr (!WIDE) {
+        if (!WIDE || p.out_bf16) {
 #pragma unroll
           for (int r = 0; r < 16; r += RS)
             if (r < left) (static_cast<u16*>(p.out) + at)[r * p.ldo] = f2bf(v[r / RS]);
@@ -615,6 +615,7 @@ extern "C" int tg_fp8_matmul(const tg_fp8_matmul_desc* d, const void* a, const v
   TG_CHECK_ARG(fmt_ok(d->a_fmt) && fmt_ok(d->b_fmt), "bad 8-bit type");
   TG_CHECK_ARG(d->out_dtype == TG_F32 || d->out_dtype == TG_BF16, "bad output type");
   TG_CHECK_ARG(!d->accumulate || d->out_dtype == TG_F32, "accumulation needs an f32 output");
+  TG_CHECK_ARG(!d->fast || d->out_dtype == TG_BF16, "fast sums are for bf16 outputs");
   if (d->M == 0 || d->N == 0) return TG_OK;
   TG_CHECK_ARG(out && (d->K == 0 || (a && scale_a && b && scale_b)), "null pointer");   // K == 0: the empty sum
   TG_CHECK_ARG(al16m(a) && al16m(b) && ((((uintptr_t)scale_a | (uintptr_t)scale_b) & 3) == 0), "a, b must be 16-byte and their scales 4-byte aligned");
@@ -652,7 +653,7 @@ extern "C" int tg_fp8_matmul(const tg_fp8_matmul_desc* d, const void* a, const v
     else if (fb) launch_formats<1, 0, WIDEV>(p, name, flops, bytes, ST(stream));           \
     else launch_formats<0, 0, WIDEV>(p, name, flops, bytes, ST(stream));                   \
   } while (0)
-  if (p.out_bf16) MM_PICK(false);
+  if (d->fast) MM_PICK(false);
   else MM_PICK(true);
   TG_CHECK_LAUNCH();
 }
