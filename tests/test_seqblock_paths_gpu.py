@@ -41,3 +41,85 @@ def test_fp8_sums_are_whole_where_products_cancel(M, N, Kc, odt):
     out.fill_(float("nan"))
     K.fp8_linear(dev(x), wq, ws, out, torch.empty(K.fp8_linear_ws(M, N, Kc), device=DEV, dtype=torch.uint8))
     within(out, want, bound, "linear")
+
+
+def tile_of(M, N, Kc, fast):
+    """The product kernel (fragments of 16 in each direction, stages, groups) that the launcher's rule takes, restated: a case below has to
+    reach the one that it stands for."""
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+
+    def up(n, d):
+        return -(-n // d)
+    t256, t128, t64 = (up(M, t) * up(N, t) for t in (256, 128, 64))
+    brief, whole = up(Kc, 128) * 128 <= 1024, not fast
+    gain = 114 if brief else 125
+    if t256 * 5 >= cus * 4 and gain * t256 * up(t128, 2 * cus) * 2 * cus >= 100 * t128 * up(t256, cus) * cus and not (whole and brief and t256 > cus):
+        return 8, 8, 2, 1
+    if whole:
+        return (4, 4, 2, 1) if t128 * 5 >= cus * 4 else (2, 2, 4, 1) if t64 > 2 * cus else (2, 2, 2, 2) if t64 > cus else (2, 2, 2, 4)
+    return (4, 4, 2, 1) if t128 > cus else (4, 4, 4, 1) if t128 * 5 >= cus * 4 else (2, 2, 4, 1) if t64 > cus else (2, 2, 4, 2)
+
+
+TILES = [
+    # kernel, fast, M, N, K, format and tile of a, of b, bias.  Odd N: the way out through LDS, rows wider than a wave at 8 fragments;
+    # K: odd and even numbers of blocks, one block
+    ((8, 8, 2, 1), False, 3700, 3701, 1300, "e5m2", False, "e4m3", True, True),
+    ((8, 8, 2, 1), False, 3844, 3700, 100, "e4m3", True, "e5m2", False, False),
+    ((4, 4, 2, 1), False, 2100, 2101, 700, "e4m3", False, "e4m3", True, True),
+    ((4, 4, 2, 1), False, 1990, 2104, 1409, "e5m2", False, "e5m2", False, False),
+    ((2, 2, 4, 1), False, 1500, 1501, 700, "e4m3", False, "e5m2", True, True),
+    ((2, 2, 4, 1), False, 1501, 1500, 1200, "e5m2", True, "e4m3", False, False),
+    ((2, 2, 2, 2), False, 1030, 1700, 900, "e5m2", False, "e4m3", True, True),
+    ((2, 2, 2, 4), False, 130, 257, 1153, "e5m2", False, "e4m3", True, True),
+    ((8, 8, 2, 1), True, 3700, 3701, 1300, "e5m2", False, "e4m3", True, True),
+    ((8, 8, 2, 1), True, 3844, 3700, 100, "e4m3", True, "e5m2", False, False),
+    ((4, 4, 2, 1), True, 2100, 2101, 700, "e5m2", False, "e4m3", True, True),
+    ((4, 4, 2, 1), True, 2600, 2100, 1409, "e4m3", False, "e5m2", False, False),
+    ((4, 4, 4, 1), True, 1920, 2041, 1100, "e5m2", False, "e5m2", True, True),
+    ((4, 4, 4, 1), True, 2048, 2040, 500, "e4m3", True, "e4m3", False, False),
+    ((2, 2, 4, 1), True, 1100, 1101, 700, "e5m2", False, "e4m3", True, True),
+    ((2, 2, 4, 1), True, 1101, 1100, 1250, "e4m3", True, "e5m2", False, False),
+    ((2, 2, 4, 2), True, 130, 257, 1153, "e5m2", False, "e4m3", True, True),
+    ((2, 2, 4, 2), True, 64, 72, 128, "e4m3", False, "e4m3", True, False),
+]
+
+
+def cut_of(a, b):
+    """What the 8-bit instruction may cut: 7 of 8 neighbouring products to 2^-13 of a power of two that is at most the largest of the 8."""
+    total = torch.zeros(a.shape[0], b.shape[0], device=DEV)
+    for k in range(0, a.shape[1], 8):
+        most = torch.zeros_like(total)
+        for j in range(k, k + 8):
+            most = torch.maximum(most, a[:, j, None] * b[None, :, j])
+        total += most
+    return 7 * 2.0 ** -13 * 1.001 * total.double()
+
+
+@pytest.mark.parametrize("case", TILES)
+def test_fp8_matmul_in_each_tile(case):
+    tile, fast, M, N, Kc, fa, ta, fb, tb, has_bias = case
+    assert tile_of(M, N, Kc, fast) == tile
+    (qa, sa), a = S.operand(M, Kc, fa, ta, 1)
+    (qb, sb), b = S.operand(N, Kc, fb, tb, 2)
+    bias = rnd(N, seed=9) if has_bias else None
+    a, b = a.to(DEV), b.to(DEV)
+    want = a @ b.t()
+    if has_bias:
+        want += bias.double().to(DEV)
+    sums = (a.shape[1] + 8) * R.U32 * (a.abs() @ b.abs().t()) + 1e-30
+    if fast:
+        sums += cut_of(a.abs().float(), b.abs().float())
+    for odt in ((BF,) if fast else (BF, F32)):
+        bound = sums + 1.01 * R.HALF[odt] * want.abs()
+        out = torch.full((M, N), float("nan"), device=DEV, dtype=odt)
+        K.fp8_matmul(qa, sa, qb, sb, out, bias=dev(bias), fast=fast)
+        within(out, want, bound, "product %s %s" % (case, odt))
+        if odt == F32:
+            prior = torch.randn(M, N, device=DEV)
+            acc = prior.clone()
+            K.fp8_matmul(qa, sa, qb, sb, acc, bias=dev(bias), accumulate=True)
+            total = want + prior.double()
+            within(acc, total, bound + R.U32 * (total.abs() + prior.double().abs()), "accumulated %s" % (case,))
+        wide = torch.full((M + 1, 2 * N + 3), 5.0, device=DEV, dtype=odt)
+        K.fp8_matmul(qa, sa, qb, sb, wide[:M, 1:N + 1], bias=dev(bias), fast=fast)
+        assert torch.equal(wide[:M, 1:N + 1], out) and (wide[:, N + 1:] == 5).all() and (wide[:, 0] == 5).all() and (wide[M] == 5).all()
