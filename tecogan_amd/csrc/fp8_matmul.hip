@@ -92,6 +92,17 @@ __device__ __forceinline__ bf16x8 widen(int lo, int hi, float scale) {
   return bf16x8{v[0][0], v[0][1], v[1][0], v[1][1], v[2][0], v[2][1], v[3][0], v[3][1]};
 }
 
+// the lane's number, counted anew where this stands
+__device__ __forceinline__ int lane_again() {
+#ifdef __HIP_DEVICE_COMPILE__
+  uint32_t all = ~0u;
+  asm volatile("" : "+s"(all));
+  return (int)__builtin_amdgcn_mbcnt_hi(all, __builtin_amdgcn_mbcnt_lo(all, 0u));
+#else
+  return 0;
+#endif
+}
+
 typedef __attribute__((address_space(3))) void lds_void_m;
 // 16 (4) bytes a lane from rsrc[voff + soff] to lds + 16 (4) lane
 __device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t rsrc, unsigned char* lds, int voff, int soff) {   // 4 bytes a lane
@@ -120,7 +131,8 @@ template <int FB, int FA, bool WIDE, int MF, int NF, int S, int G>
 __global__ __launch_bounds__(256 * G, MF * NF >= 64 || G > 1 ? 1 : 2) void fp8_tile_kernel(MmP p) {
   constexpr int TM = 32 * MF, TN = 32 * NF, STAGE = (TM + TN) * 132, HM = MF / 2, HN = NF / 2;
   extern __shared__ __attribute__((aligned(16))) unsigned char tile_lds[];
-  const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x;
+  int lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int grp = G > 1 ? __builtin_amdgcn_readfirstlane(tid >> 8) : 0, wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 3);
   const int wm = wave >> 1, wn = wave & 1;
   unsigned char* const smem = tile_lds + grp * S * STAGE;
@@ -298,6 +310,9 @@ __global__ __launch_bounds__(256 * G, MF * NF >= 64 || G > 1 ? 1 : 2) void fp8_t
   } else if (G > 1 && all > 0) {                                       // a group without a block: the barrier in front of the loop
     __builtin_amdgcn_s_barrier();
   }
+  lane = lane_again();                                                  // not kept over the loop: the largest tile has no register for it
+  r16 = lane & 15;
+  g = lane >> 4;
   if constexpr (G > 1) {
     if (nkb < turns) __builtin_amdgcn_s_barrier();                     // a group with one block less than the others
     __syncthreads();
