@@ -13,8 +13,8 @@
 //     fp32.  Measured 1.5e-5 of the result for normal operands, 7e-5 where a few channels carry it, the same for any K -- but where large
 //     products of one group cancel, what is left of the others is lost (256 - 256 + 6 x 15 x 2^-9: 0, not 0.18).  Hence the caller's choice.
 //
-// Measured on one device: bf16 out 8192 x 8192 x 4096 228 - 250 us = 2200 - 2400 TFLOP/s, 4096 x 4096 x 8192 103 us = 2670, 1 x 4096 x 4096 from
-// bf16 rows 9 us; f32 out 8192 x 8192 x 4096 445 us = 1240 TFLOP/s.
+// Measured on one device, 8192 x 8192 x 4096: whole sums 394 us = 1400 TFLOP/s (bf16 out), 416 us (f32 out); fast 228 - 250 us = 2200 - 2400.
+// 1 x 4096 x 4096 from bf16 rows 9 us.
 //
 // The instruction's rows are n and its columns m: a lane holds four neighbouring n of one m.
 #include "fp8.h"
@@ -447,12 +447,13 @@ void launch_tile(MmP p, const char* name, double flops, double bytes, hipStream_
 }
 
 // The largest tile that still gives most compute units one -- of the two larger ones (one and two a unit) the one whose last round of
-// tiles is not the emptier by more than it is the faster (4096^3, one full round: 60 and 73 us; 4352 x 4096 x 4096, a second round of
-// 16 tiles: 103 and 95, f32 out 194 and 145).  Over few blocks of K it is faster by less, since two tiles a unit hide each other's way out
-// (K = 384, 6207 x 5696: 48 and 42), for f32 outputs of several rounds not at all (8192 x 8192 x 1024: 173 and 155).
-// And what else of a unit a tile leaves free: with at most one a unit its LDS holds more stages (1024 x 4096 x 4096, bf16 out: 28 us with
-// two, 23 with four) or groups of waves (64 x 4096 x 4096: bf16 out 12.1 us with one group, 10.8 with two, 12.5 with four of two stages; f32
-// out, where the widening takes its time, 20.6, 16.1 and 14.0; 512 rows, two tiles a unit, 28 and 25).
+// tiles is not the emptier by more than it is the faster (bf16 out, whole sums: 8192 x 8192 x 4096 394 and 438 us, 4096^3, one full round,
+// 98 and 109; 4352 x 4096 x 4096, a second round of 16 tiles, 182 and 129, fast sums 103 and 95).  Over few blocks of K it is faster by
+// less, since two tiles a unit hide each other's way out (K = 384, 6207 x 5696: 60 and 45, fast 48 and 42), for whole sums of several
+// rounds not enough to count on (8192 x 8192 x 1024: f32 out 189 and 161, bf16 out 130 and 138).
+// And what else of a unit a tile leaves free.  Fast sums: with at most one tile a unit its LDS holds more stages (1024 x 4096 x 4096: 28 us
+// with two, 23 with four; whole sums 37 both) or a second group of waves (64 x 4096 x 4096: 12.1 us with one group, 10.8 with two, 12.5 with
+// four of two stages).  Whole sums, where the widening takes its time: 19.5, 16.9 and 14.9; 512 rows, two tiles a unit, 26.5, 24 and 28.
 template <int FB, int FA, bool WIDE>
 void launch_formats(const MmP& p, const char* name, double flops, double bytes, hipStream_t st) {
   const int64_t cus = tg_num_cus();
@@ -461,12 +462,19 @@ void launch_formats(const MmP& p, const char* name, double flops, double bytes, 
   const bool brief = p.K <= 1024;
   const int64_t gain = brief ? 114 : 125;                              // per cent
   const bool large = t256 * 5 >= cus * 4 && gain * t256 * places128 >= 100 * t128 * places256 && !(WIDE && brief && t256 > cus);
-  if (large) launch_tile<FB, FA, WIDE, 8, 8, 2, 1>(p, name, flops, bytes, st);
-  else if (t128 > cus || (WIDE && t128 * 5 >= cus * 4)) launch_tile<FB, FA, WIDE, 4, 4, 2, 1>(p, name, flops, bytes, st);
-  else if (t128 * 5 >= cus * 4) launch_tile<FB, FA, WIDE, 4, 4, WIDE ? 2 : 4, 1>(p, name, flops, bytes, st);
-  else if (t64 > (WIDE ? 2 * cus : cus)) launch_tile<FB, FA, WIDE, 2, 2, 4, 1>(p, name, flops, bytes, st);
-  else if (t64 > cus) launch_tile<FB, FA, WIDE, 2, 2, WIDE ? 2 : 4, WIDE ? 2 : 1>(p, name, flops, bytes, st);
-  else launch_tile<FB, FA, WIDE, 2, 2, WIDE ? 2 : 4, WIDE ? 4 : 2>(p, name, flops, bytes, st);
+  if (large) {
+    launch_tile<FB, FA, WIDE, 8, 8, 2, 1>(p, name, flops, bytes, st);
+  } else if constexpr (WIDE) {
+    if (t128 * 5 >= cus * 4) launch_tile<FB, FA, true, 4, 4, 2, 1>(p, name, flops, bytes, st);
+    else if (t64 > 2 * cus) launch_tile<FB, FA, true, 2, 2, 4, 1>(p, name, flops, bytes, st);
+    else if (t64 > cus) launch_tile<FB, FA, true, 2, 2, 2, 2>(p, name, flops, bytes, st);
+    else launch_tile<FB, FA, true, 2, 2, 2, 4>(p, name, flops, bytes, st);
+  } else {
+    if (t128 > cus) launch_tile<FB, FA, false, 4, 4, 2, 1>(p, name, flops, bytes, st);
+    else if (t128 * 5 >= cus * 4) launch_tile<FB, FA, false, 4, 4, 4, 1>(p, name, flops, bytes, st);
+    else if (t64 > cus) launch_tile<FB, FA, false, 2, 2, 4, 1>(p, name, flops, bytes, st);
+    else launch_tile<FB, FA, false, 2, 2, 4, 2>(p, name, flops, bytes, st);
+  }
 }
 
 // Few rows of a: 16 columns n of the output for a workgroup, all M (at most 16 MF) rows.  Here the weight's bytes count: every wave
