@@ -557,7 +557,7 @@ typedef struct tg_gated_scan_desc {
 /* fp32 values of `carry` (written by the forward pass, read by the backward pass) and of the backward pass's workspace */
 int tg_gated_scan_sizes(int B, int T, int D, int64_t* carry_floats, int64_t* ws_floats);
 /* h[t] = f[t] h[t-1] + (1 - f[t]) x[t], f = floor + (1 - floor) sigmoid(g); y = h, hT = the last state (fp32 [B][D]).
- * Nullable: h0 (fp32 [B][D], zero), floor (fp32 [D] in [0, 1), zero), lengths (int32 [B]: steps at and behind a row's length keep the
+ * Nullable: h0 (fp32 [B][D], zero), floor (fp32 [D], zero; in [0, 1) it keeps f in [0, 1]), lengths (int32 [B]: steps at and behind a row's length keep the
  * state, y = 0 there, their x and g are not looked at), reset (bytes [B][T]: not 0 = a new sequence begins at this step, the state
  * before it is dropped), hT, carry (only where keep == 0 and tg_gated_scan_sizes' carry serves no chunks, i.e. short sequences over
  * many channels).  hT may be h0 itself where no backward pass follows; y may be x or g itself. */

@@ -15,7 +15,8 @@
 // again from it instead of reading rounded ones.
 //
 // A reset (a new sequence begins at step t) drops the state by selection, not by a product with 0: what was in it, NaN included,
-// does not get past.  In a composed map P = -1 says that a reset is inside (P is a product of values in [0, 1] otherwise).
+// does not get past.  In a composed map one NaN of its own says that a reset is inside; P may have any other value (a floor outside [0, 1)
+// makes f one outside [0, 1]).
 // Steps at and behind a row's length keep the state, write y = 0 and zero gradients, and their x, g, dy are not looked at.
 //
 // Measured on one device: [1, 65536, 1024] bf16 in chunks 141 us (its bytes once 78 us, as read 130); [64, 1, 4096] one step 3.6 us;
@@ -95,11 +96,16 @@ __device__ __forceinline__ void sigmoids(float g, float& up, float& down) {
   down = e > 0x1p100f ? 1.f : e * up;
 }
 
-// state -> P state + L; P = -1: a reset inside
-__device__ __forceinline__ float apply(float P, float L, float h) { return P < 0.f ? L : P * h + L; }
+// state -> P state + L; P = the NaN of these bits: a reset inside.  Only selected, stored and compared, never calculated with; a NaN of g or of
+// the floor has other bits, as long as nobody chooses these.
+constexpr uint32_t GS_RESET = 0x7fd1c3a5u;
+__device__ __forceinline__ float reset_inside() { return __uint_as_float(GS_RESET); }
+__device__ __forceinline__ bool has_reset(float P) { return __float_as_uint(P) == GS_RESET; }
+__device__ __forceinline__ float apply(float P, float L, float h) { return has_reset(P) ? L : P * h + L; }
+__device__ __forceinline__ float product(float P, float P2) { return has_reset(P) || has_reset(P2) ? reset_inside() : P * P2; }
 __device__ __forceinline__ void compose(float& P, float& L, float P2, float L2) {
   L = apply(P2, L2, L);
-  P = P < 0.f || P2 < 0.f ? -1.f : P * P2;
+  P = product(P, P2);
 }
 
 // The waves' maps of a tile, read at once (the chain over them waits for LDS one time); where there are fewer than 4 waves the others'
@@ -284,12 +290,12 @@ __global__ __launch_bounds__(256) void gated_scan_fwd_kernel(GsP p) {
           Q[v] *= f[j][v];
         }
 #pragma unroll
-      for (int v = 0; v < V; ++v) P[v] = P[v] < 0.f ? -1.f : P[v] * Q[v];
+      for (int v = 0; v < V; ++v) P[v] = has_reset(P[v]) ? P[v] : P[v] * Q[v];
     } else {
 #pragma unroll
       for (int j = 0; j < N; ++j)
 #pragma unroll
-        for (int v = 0; v < V; ++v) compose(P[v], L[v], fresh >> j & 1 ? -1.f : f[j][v], a[j][v]);
+        for (int v = 0; v < V; ++v) compose(P[v], L[v], fresh >> j & 1 ? reset_inside() : f[j][v], a[j][v]);
     }
     if constexpr (OUT) {
       float h[V];
@@ -428,7 +434,7 @@ __global__ __launch_bounds__(256) void gated_scan_bwd_kernel(GsP p) {
           for (int v = 0; v < V; ++v) {
             const float f = low[v] + k[v] * up[j][v];
             R[v] = r ? 0.f : f * (e[j][v] + R[v]);
-            P[v] = r || P[v] < 0.f ? -1.f : P[v] * f;
+            P[v] = r || has_reset(P[v]) ? reset_inside() : P[v] * f;
           }
         }
       }
@@ -454,7 +460,7 @@ __global__ __launch_bounds__(256) void gated_scan_bwd_kernel(GsP p) {
         for (int j = 0; j < N; ++j)
           if (j < now) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) compose(P[v], Lf[v], fresh >> j & 1 ? -1.f : low[v] + k[v] * up[j][v], k[v] * down[j][v] * x[j][v]);
+            for (int v = 0; v < V; ++v) compose(P[v], Lf[v], fresh >> j & 1 ? reset_inside() : low[v] + k[v] * up[j][v], k[v] * down[j][v] * x[j][v]);
           }
 #pragma unroll
         for (int j = N - 1; j >= 0; --j)

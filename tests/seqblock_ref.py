@@ -105,3 +105,51 @@ def quantized(x, fmt, tile):
     q = to8(t * power(-e), fmt).reshape(pad.shape)[:R]
     code = e[:, 0, :, 0] if tile else e[..., 0].reshape(pad.shape[0], -1)[:R]
     return q, code
+
+
+def scan_with_bounds(i, d_y, d_hT, delta):
+    """Outputs and gradients of the recurrence for a dict of inputs (x, g, h0, floor, reset, lengths; None: not given), any floor, and what an
+    evaluation may be off by: an error e of the state goes on as |f| e, and every step adds delta times the size of its terms, the
+    gate's two among them (they cancel where the floor is negative)."""
+    B, T, D = i["x"].shape
+    x, g = i["x"].double().requires_grad_(), i["g"].double().requires_grad_()
+    h0 = (torch.zeros(B, D, dtype=torch.float64) if i["h0"] is None else i["h0"].double()).requires_grad_()
+    low = (torch.zeros(D, dtype=torch.float64) if i["floor"] is None else i["floor"].double()).requires_grad_()
+    ends = torch.full((B,), T) if i["lengths"] is None else i["lengths"].long()
+    fresh = torch.zeros(B, T, dtype=torch.bool) if i["reset"] is None else i["reset"] != 0
+    y, hT = scan_forward(x, g, h0, low, ends, fresh)
+    grads = torch.autograd.grad((y, hT), (x, g, h0, low), (d_y.double(), d_hT.double()))
+    want = dict(y=y, hT=hT, d_x=grads[0], d_g=grads[1], d_h0=grads[2], d_floor=grads[3])
+    with torch.no_grad():
+        zero = torch.zeros((), dtype=torch.float64)
+        runs = (torch.arange(T)[None] < ends[:, None])[..., None]
+        cut = fresh[..., None] & runs
+        up, down, k = torch.sigmoid(g), torch.sigmoid(-g), (1 - low).abs()
+        f, terms = (low + (1 - low) * up).abs(), low.abs() + k * up
+        f, terms = (torch.where(runs, torch.where(cut, zero, v), zero + 1) for v in (f, terms))
+        a = torch.where(runs, k * down * x.abs(), zero)
+        M, E, e_y, came_M, came_E = h0.abs(), torch.zeros(B, D, dtype=torch.float64), [], [], []
+        for t in range(T):
+            came_M.append(torch.where(cut[:, t], zero, M))
+            came_E.append(torch.where(cut[:, t], zero, E))
+            E = f[:, t] * E + delta * (terms[:, t] * M + a[:, t])
+            M = f[:, t] * M + a[:, t]
+            e_y.append(torch.where(runs[:, t], E, zero))
+        bound = dict(y=torch.stack(e_y, 1), hT=E)
+        Dm, De = d_hT.double().abs(), torch.zeros(B, D, dtype=torch.float64)
+        ex, eg = torch.zeros(B, T, D, dtype=torch.float64), torch.zeros(B, T, D, dtype=torch.float64)
+        e_low, m_low = torch.zeros(D, dtype=torch.float64), torch.zeros(D, dtype=torch.float64)
+        for t in range(T - 1, -1, -1):
+            live = runs[:, t]
+            m = Dm + d_y[:, t].double().abs()
+            e = De + delta * m
+            s = came_M[t] + x[:, t].abs()                               # |h - x| at most
+            ef = e * s + m * (came_E[t] + delta * s) + delta * m * s
+            ex[:, t] = torch.where(live, k * down[:, t] * (e + delta * m), zero)
+            eg[:, t] = torch.where(live, k * up[:, t] * down[:, t] * ef, zero)
+            e_low += torch.where(live, down[:, t] * ef, zero).sum(0)
+            m_low += torch.where(live, down[:, t] * m * s, zero).sum(0)
+            De = torch.where(live, f[:, t] * e + delta * terms[:, t] * m, De)
+            Dm = torch.where(live, f[:, t] * m, Dm)
+        bound.update(d_x=ex, d_g=eg, d_h0=De, d_floor=e_low + (T + 64) * U32 * m_low)   # a lane adds up to T steps, then partial sums
+    return want, bound

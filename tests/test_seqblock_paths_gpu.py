@@ -123,3 +123,45 @@ def test_fp8_matmul_in_each_tile(case):
         wide = torch.full((M + 1, 2 * N + 3), 5.0, device=DEV, dtype=odt)
         K.fp8_matmul(qa, sa, qb, sb, wide[:M, 1:N + 1], bias=dev(bias), fast=fast)
         assert torch.equal(wide[:M, 1:N + 1], out) and (wide[:, N + 1:] == 5).all() and (wide[:, 0] == 5).all() and (wide[M] == 5).all()
+
+
+# ---- gated scan ----------------------------------------------------------------------------------------------------------------
+def scan_both_ways(i, B, T, D, dt, f, what):
+    """Forward and backward of `i` against 64 bits, twice (the same bits), with nothing but NaN in the scratch buffers before."""
+    d_y, d_hT = rnd(B, T, D, seed=5, dtype=dt), rnd(B, D, seed=6)
+    if i["lengths"] is not None:
+        for b, n in enumerate(i["lengths"].tolist()):
+            d_y[b, n:] = 0
+    want, bound = R.scan_with_bounds(i, d_y, d_hT, S.DELTA)
+    how = S.scan_how(i)
+    x, g = S.dev3(i["x"], f), S.dev3(i["g"], f)
+    got = dict(y=S.dev3(torch.zeros(B, T, D, dtype=dt), f), hT=torch.full((B, D), float("nan"), device=DEV))
+    carry = torch.full((K.gated_scan_carry(B, T, D),), float("nan"), device=DEV)
+    K.gated_scan_forward(x, g, got["y"], got["hT"], carry, **how)
+    got.update(d_x=S.dev3(torch.zeros(B, T, D, dtype=dt), f), d_g=S.dev3(torch.zeros(B, T, D, dtype=dt), f))
+    if i["h0"] is not None:
+        got["d_h0"] = torch.full((B, D), float("nan"), device=DEV)
+    if i["floor"] is not None:
+        got["d_floor"] = torch.full((D,), float("nan"), device=DEV)
+    ws = torch.full((K.gated_scan_ws(B, T, D),), float("nan"), device=DEV)
+    for again in (False, True):
+        first = {n: v.clone() for n, v in got.items()}
+        K.gated_scan_backward(x, g, S.dev3(d_y, f), dev(d_hT), carry, got["d_x"], got["d_g"], ws, d_h0=got.get("d_h0"),
+                              d_floor=got.get("d_floor"), **how)
+        if again:
+            assert all(torch.equal(v, first[n]) for n, v in got.items()), "the same inputs give other bits"
+    for n, v in got.items():
+        within(v, want[n], bound[n] + 1.01 * R.HALF[v.dtype] * want[n].abs() + 1e-30, "%s %s" % (n, what))
+
+
+@pytest.mark.parametrize("B,T,D,dt,rate", [(2, 1, 70, F32, 0.3), (2, 9, 70, F32, 0.0), (3, 100, 66, BF, 0.05), (1, 700, 40, F32, 0.01),
+                                           (2, 700, 130, BF, 0.0)])
+def test_gated_scan_with_floors_outside_their_range(B, T, D, dt, rate):
+    """A floor is a trained parameter: below 0 (the gate's value then is too where it closes) the formula still holds, however the steps are
+    split over waves, tiles and chunks, and a reset still drops what came before."""
+    case = (B, T, D, dt, True, rate, None, True, 1)
+    i = S.scan_inputs(case)
+    gen = torch.Generator().manual_seed(8)
+    i["floor"] = torch.rand(D, generator=gen) * 1.6 - 0.6                # -0.6 .. 1
+    i["g"] = (i["g"].float() - 3).to(dt)
+    scan_both_ways(i, B, T, D, dt, 1, case)
