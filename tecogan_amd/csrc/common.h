@@ -101,6 +101,18 @@ __device__ __forceinline__ uint4 ld128_any(const void* p) {
                     __builtin_amdgcn_alignbyte(w[3], w[2], r), __builtin_amdgcn_alignbyte(w[4], w[3], r));
 }
 
+// exp(x) for the gates of values of type T.  The base-2 exponential's argument x log2(e) is rounded relative to itself, so that the result's
+// error is |x| 2^-24 of it.  fp32: the argument in two parts, the second as a factor 1 + lo ln 2 (2 to 3 units at any x whose exponential is
+// a normal number).  bf16 values are themselves rounded by |x| 2^-9 of the result: one part.
+template <typename T>
+__device__ __forceinline__ float gate_exp(float x) {
+  constexpr float L2E = 1.44269502e+0f, L2E_REST = 1.92596299e-8f, LN2 = 6.93147182e-1f;
+  const float hi = x * L2E, e = __builtin_amdgcn_exp2f(hi);
+  if constexpr (sizeof(T) == 2) return e;
+  const float lo = __builtin_fmaf(x, L2E_REST, __builtin_fmaf(x, L2E, -hi));
+  return __builtin_fabsf(hi) < 126.f ? __builtin_fmaf(e, lo * LN2, e) : e;   // beyond: 0, infinity or NaN, lo has no meaning
+}
+
 template <typename T> struct Elem;
 template <> struct Elem<float> {
   static __device__ __forceinline__ float ld(const float* p) { return *p; }

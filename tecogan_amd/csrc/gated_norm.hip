@@ -106,8 +106,9 @@ __device__ __forceinline__ void param8(const float* __restrict__ p, int c, int s
 }
 
 // sigmoid(v) and sigmoid(-v) without a difference: e = exp(-|v|), 1 / (1 + e) and e / (1 + e)
+template <typename T>
 __device__ __forceinline__ void sigmoids(float v, float& up, float& down) {
-  const float e = __expf(-fabsf(v)), r = __builtin_amdgcn_rcpf(1.f + e), q = e * r;
+  const float e = gate_exp<T>(-fabsf(v)), r = __builtin_amdgcn_rcpf(1.f + e), q = e * r;
   up = v >= 0.f ? r : (v != v ? v : q);
   down = v >= 0.f ? q : r;
 }
@@ -118,38 +119,40 @@ __device__ __forceinline__ float tanh_of(float v, float e, float r) {
   const float small = v + v * s * (-0.333333333f + s * (0.133333333f + s * (-0.0539682540f + s * 0.0218694885f)));
   return fabsf(v) < 0.3f ? small : copysignf((1.f - e) * r, v);
 }
-// g = act(g), one choice for the eight
+// g = act(g), one choice for the eight; T: the gate's type
+template <typename T>
 __device__ __forceinline__ void gate_values(float (&g)[8], int act) {
   if (act == TG_ACT_SIGMOID || act == TG_ACT_SILU) {
     const bool silu = act == TG_ACT_SILU;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const float up = __builtin_amdgcn_rcpf(1.f + __expf(-g[k]));
+      const float up = __builtin_amdgcn_rcpf(1.f + gate_exp<T>(-g[k]));
       g[k] = silu ? g[k] * up : up;
     }
   } else if (act == TG_ACT_TANH) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const float e = __expf(-2.f * fabsf(g[k]));
+      const float e = gate_exp<T>(-2.f * fabsf(g[k]));
       g[k] = tanh_of(g[k], e, __builtin_amdgcn_rcpf(1.f + e));
     }
   }
 }
 // value = act(g), slope = act'(g)
+template <typename T>
 __device__ __forceinline__ void gate_slopes(const float (&g)[8], int act, float (&value)[8], float (&slope)[8]) {
   if (act == TG_ACT_SIGMOID || act == TG_ACT_SILU) {
     const bool silu = act == TG_ACT_SILU;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       float up, down;
-      sigmoids(g[k], up, down);
+      sigmoids<T>(g[k], up, down);
       value[k] = silu ? g[k] * up : up;
       slope[k] = silu ? up + g[k] * up * down : up * down;
     }
   } else if (act == TG_ACT_TANH) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const float e = __expf(-2.f * fabsf(g[k])), r = __builtin_amdgcn_rcpf(1.f + e);
+      const float e = gate_exp<T>(-2.f * fabsf(g[k])), r = __builtin_amdgcn_rcpf(1.f + e);
       value[k] = tanh_of(g[k], e, r);
       slope[k] = 4.f * e * r * r;                                   // 1 - tanh^2
     }
@@ -377,7 +380,7 @@ __global__ __launch_bounds__(512) void gated_norm_fwd_kernel(GnP p) {
           params_post(v, 0);
           if (HG) rg[v].values(g[0]);
         }
-        if (HG) gate_values(g[a], d.gate_act);
+        if (HG) gate_values<TO>(g[a], d.gate_act);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const float t = (u[v][k] - mu) * (r * wpo[a][k]) + bpo[a][k];
@@ -504,7 +507,7 @@ __global__ __launch_bounds__(512) void gated_norm_bwd_kernel(GnP p) {
   auto gate_of = [&](int v) {
     float g[8];
     rg[v].values(g);
-    gate_slopes(g, d.gate_act, ga, gs);
+    gate_slopes<TO>(g, d.gate_act, ga, gs);
   };
   int turn = 0;
   if constexpr (NV == 1) {

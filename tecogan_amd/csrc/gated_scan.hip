@@ -90,8 +90,9 @@ template <> struct Raw<float, 2> {
 };
 
 // sigmoid(g) and sigmoid(-g) without a difference: e = exp(-g), 1 / (1 + e) and e / (1 + e); e past 2^100: 1 (e may be infinite)
+template <typename T>
 __device__ __forceinline__ void sigmoids(float g, float& up, float& down) {
-  const float e = __expf(-g);
+  const float e = gate_exp<T>(-g);
   up = __builtin_amdgcn_rcpf(1.f + e);
   down = e > 0x1p100f ? 1.f : e * up;
 }
@@ -254,7 +255,7 @@ __global__ __launch_bounds__(256) void gated_scan_fwd_kernel(GsP p) {
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         float up, down;
-        sigmoids(g[v], up, down);
+        sigmoids<T>(g[v], up, down);
         f[j][v] = low[v] + k[v] * up;
         a[j][v] = k[v] * down * x[v];
       }
@@ -415,7 +416,7 @@ __global__ __launch_bounds__(256) void gated_scan_bwd_kernel(GsP p) {
       if (OUT) rx[j].values(x[j]);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        sigmoids(g[v], up[j][v], down[j][v]);
+        sigmoids<T>(g[v], up[j][v], down[j][v]);
         H[v] = rH[v];
       }
     }

@@ -165,3 +165,63 @@ def test_gated_scan_with_floors_outside_their_range(B, T, D, dt, rate):
     i["floor"] = torch.rand(D, generator=gen) * 1.6 - 0.6                # -0.6 .. 1
     i["g"] = (i["g"].float() - 3).to(dt)
     scan_both_ways(i, B, T, D, dt, 1, case)
+
+
+# ---- gates far from zero -------------------------------------------------------------------------------------------------------
+# Roundings of sigmoid(g) or sigmoid(-g) times one value, relative to the result, in units of 2^-24: the exponential 3 (its instruction one
+# step, its argument's two parts), 1 + e one, the reciprocal two, the product of both one, two more factors and one sum at most four;
+# one to spare
+N_GATE = 12
+FAR = torch.linspace(12.0, 80.0, 2048)
+
+
+def test_gated_scan_gates_far_from_zero():
+    """fp32, one step: a closed gate lets (1 - f) x through, an open one f h0; both keep their value to a few last bits, however small."""
+    D = FAR.numel()
+    one, zero = torch.ones(1, 1, D, device=DEV), torch.zeros(1, 1, D, device=DEV)
+    y = torch.empty(1, 1, D, device=DEV)
+    K.gated_scan_forward(one, dev(FAR)[None, None], y, None, None, keep=False)             # f near 1: y = sigmoid(-g)
+    want = torch.sigmoid(-FAR.double())
+    within(y[0, 0], want, N_GATE * R.U32 * want, "1 - f")
+    K.gated_scan_forward(zero, -dev(FAR)[None, None], y, None, None, h0=one[0], keep=False)   # f near 0: y = sigmoid(g)
+    within(y[0, 0], want, N_GATE * R.U32 * want, "f")
+    carry = torch.empty(K.gated_scan_carry(1, 1, D), device=DEV)
+    K.gated_scan_forward(zero, dev(FAR)[None, None], y, None, carry, h0=one[0])
+    dx, dg = torch.empty_like(y), torch.empty_like(y)
+    K.gated_scan_backward(zero, dev(FAR)[None, None], one, None, carry, dx, dg, torch.empty(K.gated_scan_ws(1, 1, D), device=DEV), h0=one[0])
+    within(dx[0, 0], want, N_GATE * R.U32 * want, "d_x")
+    slope = want * torch.sigmoid(FAR.double())
+    within(dg[0, 0], slope, (N_GATE + 4) * R.U32 * slope, "d_g")                            # both sigmoids
+
+
+@pytest.mark.parametrize("act", ["sigmoid", "silu"])
+def test_gated_norm_gates_far_from_zero(act):
+    """fp32, no norm in front: y = act(gate) o for closed gates, and the gate's gradient."""
+    C = FAR.numel()
+    gate, one = -dev(FAR)[None], torch.ones(1, C, device=DEV)
+    y = torch.empty(1, C, device=DEV)
+    K.gated_norm_forward(torch.zeros(1, C, device=DEV), one, gate, y, None, pre=K.NORM_NONE, gate_act=S.ACTS[act])
+    g = -FAR.double()
+    want = R.act(act, g)
+    within(y[0], want, N_GATE * R.U32 * want.abs(), "y")
+    d_gate, d_o = torch.empty(1, C, device=DEV), torch.empty(1, C, device=DEV)
+    K.gated_norm_backward(one, None, y, one, gate, None, d_o, d_gate, torch.empty(K.gated_norm_ws(1, C), device=DEV), pre=K.NORM_NONE,
+                          gate_act=S.ACTS[act])
+    within(d_o[0], want, N_GATE * R.U32 * want.abs(), "d_o")
+    slope = R.act_slope(act, g)
+    within(d_gate[0], slope, (N_GATE + 8) * R.U32 * slope.abs(), "d_gate")                  # silu: s + g s (1 - s), terms 1 to 1 - g
+
+
+def test_gated_norm_tanh_gates_far_from_zero():
+    """The slope 1 - tanh^2 = 1 / cosh^2 keeps its value where tanh is 1 to the last bit."""
+    v = FAR / 8
+    C = v.numel()
+    gate, one = dev(v)[None], torch.ones(1, C, device=DEV)
+    y, d_gate, d_o = (torch.empty(1, C, device=DEV) for _ in range(3))
+    K.gated_norm_forward(torch.zeros(1, C, device=DEV), one, gate, y, None, pre=K.NORM_NONE, gate_act=K.ACT_TANH)
+    want = torch.tanh(v.double())
+    within(y[0], want, N_GATE * R.U32 * want, "y")
+    K.gated_norm_backward(one, None, y, one, gate, None, d_o, d_gate, torch.empty(K.gated_norm_ws(1, C), device=DEV), pre=K.NORM_NONE,
+                          gate_act=K.ACT_TANH)
+    slope = torch.cosh(v.double()) ** -2
+    within(d_gate[0], slope, (N_GATE + 4) * R.U32 * slope, "d_gate")                        # the reciprocal squared
