@@ -225,3 +225,17 @@ def test_gated_norm_tanh_gates_far_from_zero():
                           gate_act=K.ACT_TANH)
     slope = torch.cosh(v.double()) ** -2
     within(d_gate[0], slope, (N_GATE + 4) * R.U32 * slope, "d_gate")                        # the reciprocal squared
+
+
+# ---- chunks of several tiles ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("B,T,D,dt,floor,rate,lengths,f", [
+    (4, 1100, 1000, F32, True, 0.01, [1100, 0, 517, 1099], 1),           # 12 chunks of 3 tiles of 32 steps, the last of 2
+    (4, 1100, 1000, BF, True, 0.0, None, 2),
+    (4, 1100, 1000, BF, False, 0.05, [700, 1, 1100, 96], 1),             # ends inside a chunk, in its first step, at a chunk's end
+    (40, 1000, 51, F32, True, 0.01, None, 1),                            # one channel a lane; 11 chunks of 3 tiles, the last of 2
+])
+def test_gated_scan_in_chunks_of_several_tiles(B, T, D, dt, floor, rate, lengths, f):
+    tiles, chunks = -(-T // 32), K.gated_scan_ws(B, T, D) // (2 * B * D)
+    assert chunks > 1 and -(-tiles // chunks) > 1                        # scratch for two values a chunk and channel: it is cut, into tiles
+    case = (B, T, D, dt, floor, rate, lengths, True, f)
+    scan_both_ways(S.scan_inputs(case), B, T, D, dt, f, case)
