@@ -239,3 +239,40 @@ def test_gated_scan_in_chunks_of_several_tiles(B, T, D, dt, floor, rate, lengths
     assert chunks > 1 and -(-tiles // chunks) > 1                        # scratch for two values a chunk and channel: it is cut, into tiles
     case = (B, T, D, dt, floor, rate, lengths, True, f)
     scan_both_ways(S.scan_inputs(case), B, T, D, dt, f, case)
+
+
+# ---- several rows an item ------------------------------------------------------------------------------------------------------
+def item_of(rows, C, k):
+    """Rows of an item of the norm's backward pass and (0: whole gate rows) pieces of a gate row, the split's rule restated."""
+    lanes = 1
+    while lanes < -(-C // 8) and lanes < 512:
+        lanes *= 2
+    m = -(-rows // (256 * (512 // lanes)))
+    if 1 < k <= 2 * m:
+        return (-(-m // k) * k if k <= m else k), 0
+    if k > m:
+        k = min(k, rows)
+        pieces = -(-k // m)
+        return -(-k // pieces), pieces
+    return m, 0
+
+
+# rows, C, dtype, res, post, pre, gate (None / rows per gate), act, scale, row stride factor; (rows an item, pieces)
+ITEMS = [
+    ((4999, 520, BF, F32, "rms", "layer", 3, "silu", True, 1), (6, 0)),       # two gate rows an item; the last item one row of a short one
+    ((5000, 520, F32, F32, "layer", "rms", 1, "tanh", True, 1), (5, 0)),
+    ((1501, 2104, BF, BF, "layer", "layer", 2, "sigmoid", True, 1), (6, 0)),   # a row over eight waves: sums through LDS row after row
+    ((1500, 2104, F32, F32, "rms", "rms", 100, "silu", True, 1), (6, 17)),     # pieces of six rows, the last of four
+    ((1499, 2104, BF, F32, "none", "layer", None, "none", True, 2), (6, 0)),
+    ((1501, 4104, BF, BF, "rms", "layer", 3, "tanh", True, 1), (6, 0)),        # parameter sums in LDS over several rows
+    ((1301, 8200, BF, F32, "layer", "rms", 2, "silu", True, 1), (6, 0)),
+    ((70001, 24, F32, F32, "rms", "rms", 3, "sigmoid", True, 1), (3, 0)),      # 128 items a workgroup
+    ((2999, 1003, BF, BF, "rms", "rms", 2, "silu", True, 1), (4, 0)),          # rows that begin at every alignment
+]
+
+
+@pytest.mark.parametrize("case,split", ITEMS)
+def test_gated_norm_with_several_rows_an_item(case, split):
+    assert item_of(case[0], case[1], case[6] or 1) == split
+    S.test_gated_norm_forward(case)
+    S.test_gated_norm_backward(case)
