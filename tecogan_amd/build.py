@@ -17,6 +17,11 @@ SCALAR_FP32_SOURCES = ["gated_norm.hip", "gated_scan.hip", "fp8_quantize.hip", "
 SOURCES += SCALAR_FP32_SOURCES
 
 
+def flags_for(src):
+    """The compiler flags of one source."""
+    return FLAGS + (SCALAR_FP32 if src in SCALAR_FP32_SOURCES else [])
+
+
 def _newer(a, b):
     return (not os.path.exists(b)) or os.path.getmtime(a) > os.path.getmtime(b)
 
@@ -30,7 +35,7 @@ def build(force=False, verbose=True):
         o = os.path.join(CSRC, src.replace(".hip", ".o"))
         objs.append(o)
         if force or _newer(s, o) or any(_newer(d, o) for d in deps):
-            cmd = [hipcc] + FLAGS + (SCALAR_FP32 if src in SCALAR_FP32_SOURCES else []) + ["-c", s, "-o", o]
+            cmd = [hipcc] + flags_for(src) + ["-c", s, "-o", o]
             if verbose:
                 print(" ".join(cmd), flush=True)
             procs.append((src, subprocess.Popen(cmd)))

@@ -1,15 +1,30 @@
-"""What the compiler made of the fp8 product: its matrix instructions stand in inline assembly, where the compiler knows neither that a result
+"""How the sequence-block sources are built, and what the compiler made of the fp8 product: its matrix instructions stand in inline assembly, where the compiler knows neither that a result
 takes its passes to arrive nor that it may not be looked at before.  Read from the built library."""
 import os
 import re
+import runpy
 import struct
 import subprocess
+import sys
 
 import pytest
 
 from tecogan_amd import _lib as L
+from tecogan_amd import build as B
 
 OBJDUMP = "/opt/rocm/llvm/bin/llvm-objdump"
+
+
+@pytest.mark.parametrize("src", B.SOURCES)
+def test_a_variant_of_a_source_is_built_with_that_sources_flags(src, monkeypatch):
+    """tools/build_variant.py against the build itself: an A/B of the two compares nothing but what -D changes."""
+    calls, tool = [], os.path.join(os.path.dirname(B.HERE), "tools", "build_variant.py")
+    monkeypatch.setattr(subprocess, "check_call", lambda cmd, **kw: calls.append(cmd))
+    monkeypatch.setattr(B, "build", lambda **kw: None)
+    monkeypatch.setattr(sys, "argv", [tool, src, "-DX=1"])
+    runpy.run_path(tool)
+    assert calls[0][1:-5] == B.flags_for(src) and calls[0][-5] == "-DX=1"
+    assert ("-packed-fp32-ops" in calls[0]) == (src in B.SCALAR_FP32_SOURCES)
 
 
 def code_objects(path):

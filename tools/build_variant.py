@@ -16,7 +16,7 @@ os.makedirs(out, exist_ok=True)
 tag = src.replace(".hip", "") + "".join(d.replace("-D", "_").replace("=", "") for d in defs)
 obj, so = os.path.join(out, tag + ".o"), os.path.join(out, "libtecogan_%s.so" % tag)
 csrc = os.path.join(ROOT, "tecogan_amd", "csrc")
-subprocess.check_call(["/opt/rocm/bin/hipcc"] + B.FLAGS + defs + ["-c", os.path.join(csrc, src), "-o", obj])
+subprocess.check_call(["/opt/rocm/bin/hipcc"] + B.flags_for(src) + defs + ["-c", os.path.join(csrc, src), "-o", obj])
 others = [os.path.join(csrc, s.replace(".hip", ".o")) for s in B.SOURCES if s != src]
 subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-shared", "-fPIC", "-o", so, obj] + others)
 print(so)
