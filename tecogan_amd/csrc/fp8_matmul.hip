@@ -624,6 +624,7 @@ bool skinny_fuses(int64_t M, int64_t N, int64_t nkb) {
 }
 
 bool al16m(const void* p) { return ((uintptr_t)p & 15) == 0; }
+bool tiles_ok(int64_t M, int64_t N) { return cdiv64(M, 64) * cdiv64(N, 64) < ((int64_t)1 << 27); }
 bool fmt_ok(int f) { return f == TG_FP8_E4M3 || f == TG_FP8_E5M2; }
 
 }  // namespace
@@ -656,7 +657,7 @@ extern "C" int tg_fp8_matmul(const tg_fp8_matmul_desc* d, const void* a, const v
   p.accumulate = d->accumulate;
   const char* const name = "fp8_matmul";
   const double flops = 2.0 * d->M * d->N * d->K, bytes = (double)d->M * d->K + (double)d->N * d->K + (double)d->M * d->N * (p.out_bf16 ? 2 : 4);
-  TG_CHECK_ARG(cdiv64(d->M, 64) * cdiv64(d->N, 64) < ((int64_t)1 << 27), "too many output tiles");
+  TG_CHECK_ARG(tiles_ok(d->M, d->N), "too many output tiles");
   const int oe = p.out_bf16 ? 2 : 4;
   p.vec = d->N % 4 == 0 && ((uintptr_t)out & (4 * oe - 1)) == 0 && d->ldo % 4 == 0 && al16m(bias);
   const int fa = d->a_fmt == TG_FP8_E5M2, fb = d->b_fmt == TG_FP8_E5M2;
@@ -710,6 +711,7 @@ extern "C" int tg_fp8_linear(const void* x, int dtype, int64_t M, int64_t K, int
   d.a_fmt = TG_FP8_E4M3; d.b_fmt = w_fmt; d.b_tile = 1; d.out_dtype = out_dtype;
   TG_CHECK_ARG(fmt_ok(w_fmt) && w && scale_w && out && al16m(w) && ((uintptr_t)scale_w & 3) == 0 && ldo >= N &&
                    (out_dtype == TG_F32 || out_dtype == TG_BF16), "bad weight or output");
+  TG_CHECK_ARG(tiles_ok(M, N), "too many output tiles");
   if (skinny_fuses(M, N, kb)) {
     TG_CHECK_ARG(x != nullptr && ldx >= K && (dtype == TG_F32 || dtype == TG_BF16), "x is missing, its type unknown or its row stride below K");
     SkP k = {};
