@@ -637,6 +637,11 @@ bool sizes_ok(int64_t B, int64_t T, int64_t D) {
 int64_t tile_floats(const Plan& pl, int64_t B, int64_t D) { return (B * pl.ntiles * D + 3) / 4 * 4; }
 int64_t chunk_floats(const Plan& pl, int64_t B, int64_t D) { return (B * pl.nc * D + 3) / 4 * 4; }
 
+// rows of D values at strides t (T of them) and b (B of them): no two share one.  Outputs only: inputs may be windows over one another.
+bool apart(int64_t t, int64_t b, int64_t B, int64_t T, int64_t D) {
+  return (B == 1 || b >= D) && (B == 1 || T == 1 || b >= (T - 1) * t + D || t >= (B - 1) * b + D);
+}
+
 template <typename P>
 bool al(const P* p, int n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
@@ -692,6 +697,7 @@ extern "C" int tg_gated_scan_forward(const tg_gated_scan_desc* d, const void* x,
   const Plan pl = plan_of(d->B, d->T, d->D);
   const int64_t need = tile_floats(pl, d->B, d->D) + (pl.nc > 1 ? 2 * chunk_floats(pl, d->B, d->D) : 0);
   TG_CHECK_ARG((pl.nc == 1 && !keep) || (carry != nullptr && carry_floats >= need && al(carry, 16)), "the carry of tg_gated_scan_sizes() floats is missing");
+  TG_CHECK_ARG(apart(d->y_t, d->y_b, d->B, d->T, d->D), "batch rows of y overlap");
   const int es = d->dtype == TG_F32 ? 4 : 2;
   const int V = lane_channels(d->D);
   GsP p = {};
@@ -731,6 +737,7 @@ extern "C" int tg_gated_scan_backward(const tg_gated_scan_desc* d, const void* x
     TG_CHECK_ARG(carry != nullptr && carry_floats >= need && al(carry, 16), "the carry of the forward pass is missing");
     const int64_t cf = chunk_floats(pl, d->B, d->D), want = cf * (pl.nc > 1 ? 2 : 1);
     TG_CHECK_ARG((pl.nc == 1 && !d_floor) || (ws != nullptr && ws_floats >= want && al(ws, 16)), "a workspace of tg_gated_scan_sizes() floats is missing");
+    TG_CHECK_ARG(apart(d->dx_t, d->dx_b, d->B, d->T, d->D) && apart(d->dg_t, d->dg_b, d->B, d->T, d->D), "batch rows of d_x or d_g overlap");
     const int es = d->dtype == TG_F32 ? 4 : 2;
     // Three waves of two channels: their 200 - 225 registers leave a quarter of a unit's places empty, one channel needs 122 ([64, 20, 8192]
     // bf16 40.5 us with two, 35 with one; four waves 41; with 32 steps 37.5 and 41)

@@ -276,3 +276,24 @@ def test_gated_norm_with_several_rows_an_item(case, split):
     assert item_of(case[0], case[1], case[6] or 1) == split
     S.test_gated_norm_forward(case)
     S.test_gated_norm_backward(case)
+
+
+@pytest.mark.parametrize("B,T,D,dt", [(3, 70, 66, BF), (5, 300, 33, F32)])
+def test_gated_scan_layouts(B, T, D, dt):
+    """Steps outside the batch ([T, B, D] in memory), inputs as windows over one another, x beside g in one tensor: the same bits as with
+    tensors of their own."""
+    def time_major():
+        return torch.zeros(T, B, D, device=DEV, dtype=dt).transpose(0, 1)
+    both = dev(rnd(B + T, 2 * D, seed=1, dtype=dt))
+    x, g = (torch.as_strided(both, (B, T, D), (2 * D, 2 * D, 1), at) for at in (0, D))      # batch row b begins one step later
+    d_y, d_hT = dev(rnd(B, T, D, seed=2, dtype=dt)), dev(rnd(B, D, seed=3))
+    carry, ws = torch.empty(K.gated_scan_carry(B, T, D), device=DEV), torch.empty(K.gated_scan_ws(B, T, D), device=DEV)
+
+    def run(x, g, make):
+        y, dx, dg, hT = make(), make(), make(), torch.empty(B, D, device=DEV)
+        K.gated_scan_forward(x, g, y, hT, carry)
+        K.gated_scan_backward(x, g, d_y, d_hT, carry, dx, dg, ws)
+        return y, hT, dx, dg
+    apart = run(x.contiguous(), g.contiguous(), lambda: torch.zeros(B, T, D, device=DEV, dtype=dt))
+    for a, b in zip(apart, run(x, g, time_major)):
+        assert torch.equal(a, b)
