@@ -743,11 +743,14 @@ void row_geometry(int C, int block, Geo* g) {
 // The backward pass's split of the rows: workgroups of 512 lanes, one per compute unit (their registers leave room for one or two), as
 // few rows as that gives to each: every row costs its workgroup 2 - 9 us of latency, while partial sums, up to 5 C values a workgroup,
 // are read once from near by (64 rows of 1024 bf16 values: at least one row an item 10.7 us, at least four 18.7; 2048 x 2048: 25 both).
+// The split fixes the workspace's size and the order of the sums, which a host may ask for where no device is: it takes the 256 compute
+// units of a whole MI355X instead of asking (a partition of one gets the same results, several rounds of workgroups).
 // A gate row that several rows share stays with one item, or is cut into even pieces where that would double the item (72352 x 88,
 // 13 rows a gate row: whole ones 37 us, 9 and 4 rows 75).
+constexpr int64_t GN_UNITS = 256;
 void item_geometry(int64_t rows, int C, int64_t k, Geo* g) {
   row_geometry(C, 512, g);
-  int64_t m = rows > 0 ? cdiv64(rows, (int64_t)256 * g->rpb) : 1;
+  int64_t m = rows > 0 ? cdiv64(rows, GN_UNITS * g->rpb) : 1;
   g->pieces = 0;
   if (k > 1 && k <= 2 * m) {
     m = k <= m ? cdiv64(m, k) * k : k;

@@ -603,7 +603,9 @@ struct Plan {
 // Waves of a tile by the sequence's length.  Chunks: the time goes as tiles of a chunk x rounds of 512 workgroups (two a compute unit:
 // 128 channels x one chunk each; fewer than four a unit reach about 1 / 1.3 of the bandwidth) x bytes a value (3 tensors in one pass,
 // 5 in two), and the second launch of a chunked pass costs about as much as 13 of these units (measured: a tile and a round about
-// 0.8 us, a launch with its gap 4 us).  The fewest chunks at the least of it.
+// 0.8 us, a launch with its gap 4 us).  The fewest chunks at the least of it.  The plan fixes the scratch buffers' sizes and the order of the
+// sums, which a host may ask for where no device is: it takes the 256 compute units of a whole MI355X instead of asking.
+constexpr int GS_PLACES = 2 * 256;
 Plan plan_of(int64_t B, int64_t T, int64_t D) {
   Plan p;
   p.W = T <= 24 ? (int)cdiv64(T, GS_L) : GS_MAXW;
@@ -614,8 +616,8 @@ Plan plan_of(int64_t B, int64_t T, int64_t D) {
   p.nc = p.tpc = 0;
   for (int64_t n = 1, tpc = p.ntiles; n == 1 || units * n <= 4096; n = cdiv64(p.ntiles, tpc - 1), tpc = cdiv64(p.ntiles, n)) {
     const int64_t blocks = units * n;                              // n: the fewest chunks of tpc tiles
-    const double rounds = (double)cdiv64(blocks, 512);
-    const double cost = tpc * rounds * (blocks < 1024 ? 1.3 : 1.0) * (n == 1 ? 3 : 5) + (n == 1 ? 0 : 13 + 0.08 * n * rounds);
+    const double rounds = (double)cdiv64(blocks, GS_PLACES);
+    const double cost = tpc * rounds * (blocks < 2 * GS_PLACES ? 1.3 : 1.0) * (n == 1 ? 3 : 5) + (n == 1 ? 0 : 13 + 0.08 * n * rounds);
     if (p.nc == 0 || cost < best) {
       best = cost;
       p.nc = (int)n;
