@@ -7,14 +7,13 @@
 //     as long as the scaled values lie in fp32's normal range) and multiplied by v_mfma_f32_16x16x32_bf16, whose sums are fp32
 //     throughout: half the rate of the 8-bit instruction.
 //   fast (bf16 outputs, asked for by the caller): v_mfma_scale_f32_16x16x128 covers 16 x 16 outputs over exactly one block of K with the
-//     scales of its 16 rows and 16 columns as operands (4.2 PFLOP/s issued back to back on one device).  The products of 8 neighbouring
-//     k are aligned to the largest sum of exponents E among them and cut to multiples of 2^(E - 13) before they are added (found by
-//     adding small products to a large one; the unscaled 8-bit instructions do the same); the sums over the groups and blocks are
-//     fp32.  Measured 1.5e-5 of the result for normal operands, 7e-5 where a few channels carry it, the same for any K -- but where large
+//     scales of its 16 rows and 16 columns as operands.  The products of 8 neighbouring k are aligned to the largest sum of exponents E
+//     among them and cut to multiples of 2^(E - 13) before they are added (found by adding small products to a large one; the unscaled
+//     8-bit instructions do the same); the sums over the groups and blocks are fp32.  Measured 1.5e-5 of the result for normal operands, 7e-5 where a few channels carry it, the same for any K -- but where large
 //     products of one group cancel, what is left of the others is lost (256 - 256 + 6 x 15 x 2^-9: 0, not 0.18).  Hence the caller's choice.
 //
-// Measured on one device, 8192 x 8192 x 4096: whole sums 394 us = 1400 TFLOP/s (bf16 out), 416 us (f32 out); fast 228 - 250 us = 2200 - 2400.
-// 1 x 4096 x 4096 from bf16 rows 9 us.
+// Measured on one device, 8192 x 8192 x 4096: whole sums 371 - 394 us = 1480 - 1400 TFLOP/s (bf16 out), 398 - 416 us (f32 out);
+// fast 212 - 250 us = 2600 - 2200.  1 x 4096 x 4096 from bf16 rows 9 us.
 //
 // The instruction's rows are n and its columns m: a lane holds four neighbouring n of one m.
 #include "fp8.h"
@@ -615,7 +614,7 @@ void launch_skinny(const SkP& s, const char* name, double flops, double bytes, h
     if (mf == 2) TG_LAUNCH(name, flops, bytes, (fp8_skinny_kernel<FB, SRC, 2>), grid, block, 0, st, s);
   }
 }
-// Up to 32 rows (4096 x 4096: 6.5 us with 1, 10 with 32 rows; with 64 the 64 x 64 tiles take 12, this kernel 15).  Quantising on the way
+// Up to 32 rows (4096 x 4096: 6.5 us with 1, 10 with 32 rows; with 64 the 64 x 64 tiles take 13, this kernel 15).  Quantising on the way
 // costs every workgroup the whole of x again: with 4 blocks of K a wave in one round of workgroups 3.6 us, twice or four times that 8 - 12,
 // against about 4.5 us for a launch of the quantiser.
 constexpr int SK_ROWS = 32, SK_FUSED = 16;

@@ -20,7 +20,7 @@
 // Steps at and behind a row's length keep the state, write y = 0 and zero gradients, and their x, g, dy are not looked at.
 //
 // Measured on one device: [1, 65536, 1024] bf16 in chunks 141 us (its bytes once 78 us, as read 130); [64, 1, 4096] one step 3.6 us;
-// [8, 4096, 1536] bf16 forward 47 + 54, backward 37 + 108 + 5 us; [4, 19, 65536] fp32 in one pass 14.9 and 25 us.
+// [8, 4096, 1536] bf16 forward 47 + 54, backward 37 + 108 + 5 us; [4, 19, 65536] fp32 in one pass 15.5 and 25.5 us.
 #include "common.h"
 
 namespace {
