@@ -297,3 +297,40 @@ def test_gated_scan_layouts(B, T, D, dt):
     apart = run(x.contiguous(), g.contiguous(), lambda: torch.zeros(B, T, D, device=DEV, dtype=dt))
     for a, b in zip(apart, run(x, g, time_major)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("T", [20, 100, 700])
+def test_gated_scan_a_reset_stops_a_gate_of_nan(T, dt):
+    """A gate that is NaN makes the state NaN up to the next reset, and the gradients up to the one before, in one wave, tile or chunk and
+    across them: the mark of a reset is not taken for it, nor it for a reset."""
+    B, D, at, first, second = 2, 66, T // 2, T // 4, 3 * T // 4
+    x, g = rnd(B, T, D, seed=1, dtype=dt), rnd(B, T, D, seed=2, dtype=dt)
+    g[:, at] = float("nan")
+    reset = torch.zeros(B, T, dtype=torch.uint8)
+    reset[0, first] = reset[0, second] = 1                              # row 1 has none
+    y, hT, carry = torch.empty(B, T, D, device=DEV, dtype=dt), torch.empty(B, D, device=DEV), torch.empty(K.gated_scan_carry(B, T, D), device=DEV)
+    K.gated_scan_forward(dev(x), dev(g), y, hT, carry, reset=dev(reset))
+    dx, dg = torch.empty_like(y), torch.empty_like(y)
+    K.gated_scan_backward(dev(x), dev(g), torch.ones_like(y), None, carry, dx, dg, torch.empty(K.gated_scan_ws(B, T, D), device=DEV), reset=dev(reset))
+    bad, steps = torch.isnan(y.cpu()), torch.arange(T)
+    assert torch.equal(bad[0], ((steps >= at) & (steps < second))[:, None].expand(T, D)) and not torch.isnan(hT[0]).any()
+    assert torch.equal(bad[1], (steps >= at)[:, None].expand(T, D)) and torch.isnan(hT[1]).all()
+    bad = torch.isnan(dx.cpu())
+    assert torch.equal(bad[0], ((steps >= first) & (steps <= at))[:, None].expand(T, D))
+    assert torch.equal(bad[1], (steps <= at)[:, None].expand(T, D))
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_gates_of_infinity(dt):
+    """A gate of infinity keeps the state, one of minus infinity takes the input: exactly, and with gradients that are numbers."""
+    x, h0 = rnd(1, 2, 130, seed=1, dtype=dt), rnd(1, 130, seed=2)
+    g = torch.zeros(1, 2, 130, dtype=dt)
+    g[:, 0], g[:, 1] = float("inf"), float("-inf")
+    y, hT = torch.empty(1, 2, 130, device=DEV, dtype=dt), torch.empty(1, 130, device=DEV)
+    carry, ws = torch.empty(K.gated_scan_carry(1, 2, 130), device=DEV), torch.empty(K.gated_scan_ws(1, 2, 130), device=DEV)
+    K.gated_scan_forward(dev(x), dev(g), y, hT, carry, h0=dev(h0))
+    assert torch.equal(y[0, 0].cpu(), h0[0].to(dt)) and torch.equal(y[0, 1].cpu(), x[0, 1]) and torch.equal(hT.cpu(), x[:, 1].float())
+    dx, dg, dh0 = torch.empty_like(y), torch.empty_like(y), torch.empty(1, 130, device=DEV)
+    K.gated_scan_backward(dev(x), dev(g), torch.ones_like(y), torch.ones(1, 130, device=DEV), carry, dx, dg, ws, h0=dev(h0), d_h0=dh0)
+    assert (dx[0, 0] == 0).all() and (dx[0, 1] == 2).all() and (dg == 0).all() and (dh0 == 1).all()
