@@ -9,8 +9,9 @@
 //   fast (bf16 outputs, asked for by the caller): v_mfma_scale_f32_16x16x128 covers 16 x 16 outputs over exactly one block of K with the
 //     scales of its 16 rows and 16 columns as operands.  The products of 8 neighbouring k are aligned to the largest sum of exponents E
 //     among them and cut to multiples of 2^(E - 13) before they are added (found by adding small products to a large one; the unscaled
-//     8-bit instructions do the same); the sums over the groups and blocks are fp32.  Measured 1.5e-5 of the result for normal operands, 7e-5 where a few channels carry it, the same for any K -- but where large
-//     products of one group cancel, what is left of the others is lost (256 - 256 + 6 x 15 x 2^-9: 0, not 0.18).  Hence the caller's choice.
+//     8-bit instructions do the same); the sums over the groups and blocks are fp32.  Measured 1.5e-5 of the result for normal operands,
+//     7e-5 where a few channels carry it, the same for any K -- but where large products of one group cancel, what is left of the others
+//     is lost (256 - 256 + 6 x 15 x 2^-9: 0, not 0.18).  Hence the caller's choice.
 //
 // Measured on one device, 8192 x 8192 x 4096: whole sums 371 - 394 us = 1480 - 1400 TFLOP/s (bf16 out), 398 - 416 us (f32 out);
 // fast 212 - 250 us = 2600 - 2200.  1 x 4096 x 4096 from bf16 rows 9 us.

@@ -836,8 +836,8 @@ def _scan_masks(B, T, lengths, reset):
 def gated_scan_forward(x, g, y, hT, carry, h0=None, floor=None, lengths=None, reset=None, keep=True):
     """h[t] = f[t] h[t-1] + (1 - f[t]) x[t], f = floor + (1 - floor) sigmoid(g), along dimension 1 of x, g, y [B, T, D] (bf16 / f32,
     channels contiguous); y = h, hT [B, D] fp32 or None = the last state.  h0 [B, D] fp32: the state before (None: zero); floor [D]
-    fp32, in [0, 1) where f is to stay in [0, 1]; lengths [B] int32: steps at and behind a row's length keep the state and write y = 0; reset [B, T] bytes: not 0
-    drops the state before the step (packed sequences).
+    fp32, in [0, 1) where f is to stay in [0, 1]; lengths [B] int32: steps at and behind a row's length keep the state and write y = 0;
+    reset [B, T] bytes: not 0 drops the state before the step (packed sequences).  Rows of y may not overlap.
     carry: fp32, gated_scan_carry(B, T, D) values; with `keep` it holds what gated_scan_backward needs.  Without, carry may be None
     where the sequence needs no scratch (up to 64 steps always; longer ones are refused where they are cut into chunks).  Returns y."""
     stream = _on_device(x, g, y, hT, carry, h0, floor, lengths, reset)
